@@ -72,6 +72,21 @@ def build_td3_kernels(force=False):
     return TD3_OUT
 
 
+REG_SRC = os.path.join(CSRC, "regularise.hip")
+REG_OUT = os.path.join(CSRC, "libplenreg.so")
+# without packed float instructions: some of their forms have given wrong results on this chip now and then
+REG_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
+def build_regularise(force=False):
+    """Compile regularise.hip -> csrc/libplenreg.so (gfx950): dropout and group norm of the Q networks' hidden layers (include/plenreg.h)."""
+    deps = [REG_SRC, os.path.join(CSRC, "philox.h"), os.path.join(os.path.dirname(_HERE), "include", "plenreg.h")]
+    if not force and os.path.exists(REG_OUT) and all(os.path.getmtime(REG_OUT) >= os.path.getmtime(d) for d in deps):
+        return REG_OUT
+    subprocess.check_call([hipcc_path()] + REG_FLAGS + ["-o", REG_OUT, REG_SRC], cwd=CSRC)
+    return REG_OUT
+
+
 # The A/B partner of the shipped env library (csrc/variants/nospec.so; tests/test_env_gpu.py holds the two to bitwise equality): every round-4/5 restructuring switched off --
 # run-time point tests instead of the count-specialised solver loops (with their hoisted commits), the Delassus matrix as vector multiply-adds from broadcast LDS reads instead of
 # matrix-core tiles.  (Not the mass matrix: -DPLENVEC_MFMA_MASS=0 changes how the compiler contracts the rest of that phase -- even the bias force, which the switch does not
