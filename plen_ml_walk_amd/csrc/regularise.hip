@@ -3,6 +3,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include "../../include/plenreg.h"
+#ifdef __HIP_DEVICE_COMPILE__
+#define PHILOX_XOR3(a, b, c) __builtin_amdgcn_bitop3_b32((a), (b), (c), 0x96)          // one instruction instead of two
+#endif
 #include "philox.h"
 
 // ---- element types: arithmetic is in 32 bits, each result is rounded once, when it is stored
@@ -21,27 +24,108 @@ static __device__ __forceinline__ void store_param(void *p, int dtype, int i, fl
     else ((_Float16 *)p)[i] = (_Float16)v;
 }
 
-// ---- the mask (plenreg.h): is element i of draw `site` kept?
+// ---- 8 neighbouring elements, the unit of every kernel: 16 bytes of a 16-bit type, 32 of float32; aligned like one element only (rows of odd
+//      widths begin anywhere; the wide loads take any address)
+template <int DT> struct Chunk { typename Elem<DT>::T v[8]; };
+template <int DT> static __device__ __forceinline__ Chunk<DT> load_chunk(const typename Elem<DT>::T *p, int valid) {
+    Chunk<DT> c;
+    if (valid >= 8) __builtin_memcpy(&c, p, sizeof c);
+    else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) c.v[e] = e < valid ? p[e] : (typename Elem<DT>::T)0.f;
+    }
+    return c;
+}
+template <int DT> static __device__ __forceinline__ void store_chunk(typename Elem<DT>::T *p, int valid, const float (&v)[8]) {
+    Chunk<DT> c;
+#pragma unroll
+    for (int e = 0; e < 8; e++) c.v[e] = (typename Elem<DT>::T)v[e];
+    if (valid >= 8) __builtin_memcpy(p, &c, sizeof c);
+    else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < valid) p[e] = c.v[e];
+    }
+}
+
+// ---- the mask (plenreg.h): 16 bits of the stream per element, so one generator call serves a chunk.  Ten rounds of two 32 x 32 -> 64-bit products
+//      per 8 elements stay below the memory time of 8 16-bit elements; 32 bits per element would not.
 struct Draw { uint32_t call_lo, call_hi, tag, key_lo, key_hi, cut; float scale; };
 static __device__ __forceinline__ Draw make_draw(const uint64_t *rng, int site, uint32_t cut) {
     const uint64_t seed = rng[0], call = rng[1];
     return Draw{(uint32_t)call, (uint32_t)(call >> 32), 16u + (uint32_t)site, (uint32_t)seed, (uint32_t)(seed >> 32), cut,
                 cut < 65536u ? (float)(65536.0 / (65536.0 - (double)cut)) : 0.f};
 }
-static __device__ __forceinline__ bool kept(const Draw &d, int64_t i) {
-    const u4 w = philox4x32((uint32_t)(i >> 3), d.call_lo, d.call_hi, d.tag, d.key_lo, d.key_hi);
-    const uint32_t k = (uint32_t)i & 7u, word = (k >> 1) == 0 ? w.x : (k >> 1) == 1 ? w.y : (k >> 1) == 2 ? w.z : w.w;
-    return ((k & 1 ? word >> 16 : word) & 0xffffu) >= d.cut;
+static __device__ __forceinline__ u4 block_words(const Draw &d, uint32_t block) { return philox4x32(block, d.call_lo, d.call_hi, d.tag, d.key_lo, d.key_hi); }
+// bit e: is element e of the block of 8 elements kept?
+static __device__ __forceinline__ uint32_t block_mask(const Draw &d, uint32_t block) {
+    const u4 w = block_words(d, block);
+    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) m |= ((words[k] & 0xffffu) >= d.cut ? 1u << (2 * k) : 0u) | ((words[k] >> 16) >= d.cut ? 2u << (2 * k) : 0u);
+    return m;
 }
+// v[e] = kept ? v[e] scale : 0 for a whole block of 8 elements
+static __device__ __forceinline__ void drop_block(const Draw &d, uint32_t block, float (&v)[8]) {
+    const u4 w = block_words(d, block);
+    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float s = v[e] * d.scale;
+        v[e] = ((e & 1 ? words[e >> 1] >> 16 : words[e >> 1] & 0xffffu) >= d.cut) ? s : 0.f;
+    }
+}
+// ... of the 8 elements from element i on; aligned: i is known to be a multiple of 8
+static __device__ __forceinline__ uint32_t chunk_mask(const Draw &d, int64_t i, bool aligned) {
+    const uint32_t block = (uint32_t)(i >> 3), shift = (uint32_t)i & 7u;
+    if (aligned || shift == 0) return block_mask(d, block);
+    return (block_mask(d, block) | block_mask(d, block + 1) << 8) >> shift;
+}
+static __device__ __forceinline__ bool kept(const Draw &d, int64_t i) { return block_mask(d, (uint32_t)(i >> 3)) >> (i & 7) & 1u; }
 
-template <int DT> __global__ __launch_bounds__(256) void k_dropout(PlenRegDropout A) {
+// ---- dropout.  U chunks per thread: all loads are issued before the first mask is drawn.  In rows that are not contiguous (ROWS) a chunk that crosses
+//      the end of a row is loaded element by element.
+template <int DT, int U, bool ROWS> __global__ __launch_bounds__(256) void k_dropout(PlenRegDropout A) {
     typedef typename Elem<DT>::T T;
+    const T *x = (const T *)A.x;
+    T *y = (T *)A.y;
     const Draw d = make_draw(A.rng, A.site, A.cut);
     if (A.used && blockIdx.x == 0 && threadIdx.x == 0) { A.used[0] = A.rng[0]; A.used[1] = A.rng[1]; }
-    const int64_t n = A.rows * A.cols;
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-        const float v = (float)((const T *)A.x)[i / A.cols * A.x_stride + i % A.cols];
-        ((T *)A.y)[i] = (T)(kept(d, i) ? v * d.scale : 0.f);
+    const int64_t n = A.rows * A.cols, first = (int64_t)blockIdx.x * (256 * U);
+    if (!ROWS && (first + 256 * U) * 8 <= n) {                     // every chunk of the workgroup is whole
+        Chunk<DT> c[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) c[u] = load_chunk<DT>(x + (first + u * 256 + threadIdx.x) * 8, 8);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = (float)c[u].v[e];
+            drop_block(d, (uint32_t)(first + u * 256 + threadIdx.x), v);
+            store_chunk<DT>(y + (first + u * 256 + threadIdx.x) * 8, 8, v);
+        }
+        return;
+    }
+    for (int u = 0; u < U; u++) {
+        const int64_t j = first + u * 256 + threadIdx.x, i = j << 3;
+        if (i >= n) return;
+        const int valid = n - i < 8 ? (int)(n - i) : 8;
+        Chunk<DT> c;
+        if (ROWS) {
+            int64_t row = n >> 32 ? i / A.cols : (int64_t)((uint32_t)i / (uint32_t)A.cols), col = i - row * A.cols;
+            if (col + valid <= A.cols) c = load_chunk<DT>(x + row * A.x_stride + col, valid);
+            else
+                for (int e = 0; e < 8; e++) {
+                    c.v[e] = e < valid ? x[row * A.x_stride + col] : (T)0.f;
+                    if (++col == A.cols) { col = 0; row++; }
+                }
+        } else c = load_chunk<DT>(x + i, valid);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = (float)c.v[e];
+        drop_block(d, (uint32_t)j, v);
+        store_chunk<DT>(y + i, valid, v);
     }
 }
 
@@ -153,6 +237,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_norm_params(PlenRegNo
     }
 }
 
+#define DROPOUT_SMALL (1 << 18)
 #define PLENREG_REFUSE (-(int)hipErrorInvalidValue)
 #define PLENREG_BY_TYPE(dtype, call)                  \
     switch (dtype) {                                  \
@@ -176,9 +261,12 @@ extern "C" {
 int plenreg_dropout(const PlenRegDropout *a, void *stream) {
     if (!a || !a->x || !a->y || !a->rng || a->rows < 1 || a->cols < 1 || a->rows > ((int64_t)1 << 35) / a->cols || a->x_stride < 0 || bad_type(a->dtype)
         || bad_draw(a->rng, a->cut, a->site, a->rows * a->cols)) return PLENREG_REFUSE;
-    const int64_t blocks = (a->rows * a->cols + 255) / 256;
-    const dim3 grid((unsigned)(blocks < 16384 ? blocks : 16384));
-#define CALL(DT) k_dropout<DT><<<grid, 256, 0, (hipStream_t)stream>>>(*a)
+    const int64_t chunks = (a->rows * a->cols + 7) / 8;
+    const bool rows = a->rows > 1 && a->x_stride != a->cols, small = chunks <= DROPOUT_SMALL;
+    const dim3 grid((unsigned)((chunks + (small ? 255 : 1023)) / (small ? 256 : 1024)));
+#define CALL(DT)                                                                                                                              \
+    small ? (rows ? k_dropout<DT, 1, true><<<grid, 256, 0, (hipStream_t)stream>>>(*a) : k_dropout<DT, 1, false><<<grid, 256, 0, (hipStream_t)stream>>>(*a)) \
+          : (rows ? k_dropout<DT, 4, true><<<grid, 256, 0, (hipStream_t)stream>>>(*a) : k_dropout<DT, 4, false><<<grid, 256, 0, (hipStream_t)stream>>>(*a))
     PLENREG_BY_TYPE(a->dtype, CALL)
 #undef CALL
     return launched();
