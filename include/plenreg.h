@@ -45,9 +45,10 @@ int plenreg_dropout(const PlenRegDropout *args, void *stream);
 typedef struct PlenRegNorm {
     const void *x;             /* N slabs of L x C contiguous elements, x_stride elements apart */
     const void *dy;            /* backward: likewise, dy_stride apart */
-    const void *w, *b;         /* [C] of type w_dtype; NULL: ones / zeros */
+    const void *w, *b;         /* [C] of type w_dtype, which is PLENREG_F32 or dtype; NULL: ones / zeros */
     void *out;                 /* forward: y, backward: dx; [N][L][C] contiguous */
-    double *stats;             /* [N][G][2] = mean and 1 / sqrt(variance + eps) of the (dropped-out) input: written by the forward pass (NULL: not wanted), read by the backward pass */
+    double *stats;             /* [N][G][2], 16-byte aligned: mean m of the masked but unscaled input and r = scale / sqrt(scale^2 variance + eps), so that the normalised
+                                * value is (x - m) r, with dropout or without; written by the forward pass (NULL: not wanted), read by the backward pass */
     void *dw, *db;             /* backward: [C] of type w_dtype, written; NULL: not wanted */
     void *ws;                  /* plenreg_norm_workspace() bytes, 16-byte aligned; contents need not be preserved or cleared */
     const uint64_t *rng;       /* cut > 0 only; backward: the forward's `used` */

@@ -39,23 +39,27 @@ def parse_resource_remarks(text):
     return out
 
 
-def build_extension(force=False, verbose=False):
-    """Compile plenvec.hip -> csrc/libplenvec.so (gfx950 only).  Returns the output path.  The compiler's resource report of every kernel (registers, spilled SGPRs,
-    scratch, LDS, occupancy) is kept next to the library as libplenvec.resources.json: tests/test_cabi_cpu.py holds the env kernels to their budgets."""
+def _build_with_report(cmd, report, verbose=False):
+    """Run hipcc and keep the resource report of every kernel."""
     import json
-    if not force and os.path.exists(OUT) and os.path.exists(RESOURCES) and all(os.path.getmtime(OUT) >= os.path.getmtime(d) for d in DEPS):
-        return OUT
-    # -fno-slp-vectorize: the SLP vectoriser pairs the 3x3 kinematics products into v_pk_* ops but pays for it with more
-    # v_mov shuffles than it saves (measured: -200 VALU instructions per substep, -3.6 % step time, 13 -> 5 spilled VGPRs);
-    # the packed Delassus build uses explicit vector types and is unaffected.
-    cmd = [hipcc_path(), "-Rpass-analysis=kernel-resource-usage"] + FLAGS + ["-o", OUT, SRC]
     r = subprocess.run(cmd, cwd=CSRC, stderr=subprocess.PIPE, text=True)
     if r.returncode != 0:
         raise RuntimeError("hipcc failed:\n" + r.stderr[-4000:])
     if verbose:
         print(r.stderr)
-    with open(RESOURCES, "w") as f:
+    with open(report, "w") as f:
         json.dump(parse_resource_remarks(r.stderr), f, indent=1, sort_keys=True)
+
+
+def build_extension(force=False, verbose=False):
+    """Compile plenvec.hip -> csrc/libplenvec.so (gfx950 only).  Returns the output path.  The compiler's resource report of every kernel (registers, spilled SGPRs,
+    scratch, LDS, occupancy) is kept next to the library as libplenvec.resources.json: tests/test_cabi_cpu.py holds the env kernels to their budgets."""
+    if not force and os.path.exists(OUT) and os.path.exists(RESOURCES) and all(os.path.getmtime(OUT) >= os.path.getmtime(d) for d in DEPS):
+        return OUT
+    # -fno-slp-vectorize: the SLP vectoriser pairs the 3x3 kinematics products into v_pk_* ops but pays for it with more
+    # v_mov shuffles than it saves (measured: -200 VALU instructions per substep, -3.6 % step time, 13 -> 5 spilled VGPRs);
+    # the packed Delassus build uses explicit vector types and is unaffected.
+    _build_with_report([hipcc_path(), "-Rpass-analysis=kernel-resource-usage"] + FLAGS + ["-o", OUT, SRC], RESOURCES, verbose)
     return OUT
 
 
@@ -72,19 +76,43 @@ def build_td3_kernels(force=False):
     return TD3_OUT
 
 
-REG_SRC = os.path.join(CSRC, "regularise.hip")
+REG_SRC, REG_NORM_SRC = os.path.join(CSRC, "regularise.hip"), os.path.join(CSRC, "regularise_norm.hip")
 REG_OUT = os.path.join(CSRC, "libplenreg.so")
+REG_RESOURCES = os.path.join(CSRC, "libplenreg.resources.json")
 # without packed float instructions: some of their forms have given wrong results on this chip now and then
-REG_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+REG_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+REG_TYPES = [("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16"), ("f16", "f32"), ("f16", "f16")]            # x and results, parameters
 
 
-def build_regularise(force=False):
-    """Compile regularise.hip -> csrc/libplenreg.so (gfx950): dropout and group norm of the Q networks' hidden layers (include/plenreg.h)."""
-    deps = [REG_SRC, os.path.join(CSRC, "philox.h"), os.path.join(os.path.dirname(_HERE), "include", "plenreg.h")]
-    if not force and os.path.exists(REG_OUT) and all(os.path.getmtime(REG_OUT) >= os.path.getmtime(d) for d in deps):
+def build_regularise(force=False, flags=(), out=None):
+    """Compile regularise.hip and, once per pair of element types, regularise_norm.hip -> csrc/libplenreg.so (gfx950): dropout and group norm of the Q networks' hidden
+    layers (include/plenreg.h).  The compiler's resource report goes to libplenreg.resources.json: tests/test_regularise_cpu.py holds every kernel to no scratch memory."""
+    import json
+    import tempfile
+    from concurrent.futures import ThreadPoolExecutor
+    deps = [REG_SRC, REG_NORM_SRC, os.path.join(CSRC, "regularise.h"), os.path.join(CSRC, "philox.h"), os.path.join(os.path.dirname(_HERE), "include", "plenreg.h")]
+    if out is None and not force and os.path.exists(REG_OUT) and os.path.exists(REG_RESOURCES) and all(os.path.getmtime(REG_OUT) >= os.path.getmtime(d) for d in deps):
         return REG_OUT
-    subprocess.check_call([hipcc_path()] + REG_FLAGS + ["-o", REG_OUT, REG_SRC], cwd=CSRC)
-    return REG_OUT
+    with tempfile.TemporaryDirectory() as tmp:
+        units = [([REG_SRC], os.path.join(tmp, "regularise.o"))]
+        for dt, wt in REG_TYPES:
+            units.append(([REG_NORM_SRC, "-DREG_DT=PLENREG_" + dt.upper(), "-DREG_WT=PLENREG_" + wt.upper(), "-DREG_ENTRY=plenreg_norm_%s_%s" % (dt, wt)],
+                          os.path.join(tmp, "norm_%s_%s.o" % (dt, wt))))
+        compile_unit = lambda u: subprocess.run([hipcc_path(), "-Rpass-analysis=kernel-resource-usage", "-c"] + REG_FLAGS + list(flags) + u[0] + ["-o", u[1]], cwd=CSRC,  # noqa: E731
+                                                stderr=subprocess.PIPE, text=True)
+        with ThreadPoolExecutor(6) as pool:
+            done = list(pool.map(compile_unit, units))
+        report = {}
+        for (_, obj), r in zip(units, done):
+            if r.returncode != 0:
+                raise RuntimeError("hipcc failed:\n" + r.stderr[-4000:])
+            for name, v in parse_resource_remarks(r.stderr).items():
+                report[os.path.basename(obj)[:-2] + ":" + name] = v
+        subprocess.check_call([hipcc_path(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out or REG_OUT] + [u[1] for u in units])
+    if out is None:
+        with open(REG_RESOURCES, "w") as f:
+            json.dump(report, f, indent=1, sort_keys=True)
+    return out or REG_OUT
 
 
 # The A/B partner of the shipped env library (csrc/variants/nospec.so; tests/test_env_gpu.py holds the two to bitwise equality): every round-4/5 restructuring switched off --

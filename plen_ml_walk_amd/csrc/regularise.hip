@@ -1,92 +1,25 @@
-// regularise.hip -- dropout from the counter-based generator, group norm with an activation over channels-last data, and the two in one pass,
-// with their gradients (gfx950).  C ABI: include/plenreg.h.  All three are bound by memory traffic at size and by launch latency when small.
-#include <hip/hip_runtime.h>
-#include <stdint.h>
-#include "../../include/plenreg.h"
-#ifdef __HIP_DEVICE_COMPILE__
-#define PHILOX_XOR3(a, b, c) __builtin_amdgcn_bitop3_b32((a), (b), (c), 0x96)          // one instruction instead of two
-#endif
-#include "philox.h"
+// regularise.hip -- the C ABI of include/plenreg.h (argument checks, launch plans) and the dropout kernel; the group-norm kernels are in regularise_norm.hip.
+// All of it is bound by memory traffic at size and by launch latency when small.
+#include "regularise.h"
 
-// ---- element types: arithmetic is in 32 bits, each result is rounded once, when it is stored
-template <int DT> struct Elem;
-template <> struct Elem<PLENREG_F32> { typedef float T; };
-template <> struct Elem<PLENREG_BF16> { typedef __bf16 T; };
-template <> struct Elem<PLENREG_F16> { typedef _Float16 T; };
+#define DROPOUT_SMALL (1 << 18)
+#define ROW_MAX_FORWARD 8192            // widest group that the lanes of one workgroup hold: 256 lanes of 4 chunks, or in the backward pass (which holds four times as much) 512 of one
+#define ROW_MAX_BACKWARD 4096
 
-static __device__ __forceinline__ float load_param(const void *p, int dtype, int i, float otherwise) {
-    if (!p) return otherwise;
-    return dtype == PLENREG_F32 ? ((const float *)p)[i] : dtype == PLENREG_BF16 ? (float)((const __bf16 *)p)[i] : (float)((const _Float16 *)p)[i];
-}
-static __device__ __forceinline__ void store_param(void *p, int dtype, int i, float v) {
-    if (dtype == PLENREG_F32) ((float *)p)[i] = v;
-    else if (dtype == PLENREG_BF16) ((__bf16 *)p)[i] = (__bf16)v;
-    else ((_Float16 *)p)[i] = (_Float16)v;
-}
-
-// ---- 8 neighbouring elements, the unit of every kernel: 16 bytes of a 16-bit type, 32 of float32; aligned like one element only (rows of odd
-//      widths begin anywhere; the wide loads take any address)
-template <int DT> struct Chunk { typename Elem<DT>::T v[8]; };
-template <int DT> static __device__ __forceinline__ Chunk<DT> load_chunk(const typename Elem<DT>::T *p, int valid) {
-    Chunk<DT> c;
-    if (valid >= 8) __builtin_memcpy(&c, p, sizeof c);
-    else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) c.v[e] = e < valid ? p[e] : (typename Elem<DT>::T)0.f;
-    }
-    return c;
-}
-template <int DT> static __device__ __forceinline__ void store_chunk(typename Elem<DT>::T *p, int valid, const float (&v)[8]) {
-    Chunk<DT> c;
-#pragma unroll
-    for (int e = 0; e < 8; e++) c.v[e] = (typename Elem<DT>::T)v[e];
-    if (valid >= 8) __builtin_memcpy(p, &c, sizeof c);
-    else {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (e < valid) p[e] = c.v[e];
-    }
-}
-
-// ---- the mask (plenreg.h): 16 bits of the stream per element, so one generator call serves a chunk.  Ten rounds of two 32 x 32 -> 64-bit products
-//      per 8 elements stay below the memory time of 8 16-bit elements; 32 bits per element would not.
-struct Draw { uint32_t call_lo, call_hi, tag, key_lo, key_hi, cut; float scale; };
-static __device__ __forceinline__ Draw make_draw(const uint64_t *rng, int site, uint32_t cut) {
-    const uint64_t seed = rng[0], call = rng[1];
-    return Draw{(uint32_t)call, (uint32_t)(call >> 32), 16u + (uint32_t)site, (uint32_t)seed, (uint32_t)(seed >> 32), cut,
-                cut < 65536u ? (float)(65536.0 / (65536.0 - (double)cut)) : 0.f};
-}
-static __device__ __forceinline__ u4 block_words(const Draw &d, uint32_t block) { return philox4x32(block, d.call_lo, d.call_hi, d.tag, d.key_lo, d.key_hi); }
-// bit e: is element e of the block of 8 elements kept?
-static __device__ __forceinline__ uint32_t block_mask(const Draw &d, uint32_t block) {
-    const u4 w = block_words(d, block);
-    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-    uint32_t m = 0;
-#pragma unroll
-    for (int k = 0; k < 4; k++) m |= ((words[k] & 0xffffu) >= d.cut ? 1u << (2 * k) : 0u) | ((words[k] >> 16) >= d.cut ? 2u << (2 * k) : 0u);
-    return m;
-}
+// ---- dropout.  U chunks per thread: all loads are issued before the first mask is drawn.  In rows that are not contiguous (ROWS) a chunk that crosses
+//      the end of a row is loaded element by element.
+struct DropArgs { const void *x; void *y; const uint64_t *rng; uint64_t *used; int64_t rows, cols, x_stride; uint32_t cut; int site; float scale; };
 // v[e] = kept ? v[e] scale : 0 for a whole block of 8 elements
-static __device__ __forceinline__ void drop_block(const Draw &d, uint32_t block, float (&v)[8]) {
+static __device__ __forceinline__ void drop_block(const Draw &d, uint32_t block, float scale, float (&v)[8]) {
     const u4 w = block_words(d, block);
     const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        const float s = v[e] * d.scale;
+        const float s = v[e] * scale;
         v[e] = ((e & 1 ? words[e >> 1] >> 16 : words[e >> 1] & 0xffffu) >= d.cut) ? s : 0.f;
     }
 }
-// ... of the 8 elements from element i on; aligned: i is known to be a multiple of 8
-static __device__ __forceinline__ uint32_t chunk_mask(const Draw &d, int64_t i, bool aligned) {
-    const uint32_t block = (uint32_t)(i >> 3), shift = (uint32_t)i & 7u;
-    if (aligned || shift == 0) return block_mask(d, block);
-    return (block_mask(d, block) | block_mask(d, block + 1) << 8) >> shift;
-}
-static __device__ __forceinline__ bool kept(const Draw &d, int64_t i) { return block_mask(d, (uint32_t)(i >> 3)) >> (i & 7) & 1u; }
-
-// ---- dropout.  U chunks per thread: all loads are issued before the first mask is drawn.  In rows that are not contiguous (ROWS) a chunk that crosses
-//      the end of a row is loaded element by element.
-template <int DT, int U, bool ROWS> __global__ __launch_bounds__(256) void k_dropout(PlenRegDropout A) {
+template <int DT, int U, bool ROWS> __global__ __launch_bounds__(256) void k_dropout(DropArgs A) {
     typedef typename Elem<DT>::T T;
     const T *x = (const T *)A.x;
     T *y = (T *)A.y;
@@ -96,14 +29,14 @@ template <int DT, int U, bool ROWS> __global__ __launch_bounds__(256) void k_dro
     if (!ROWS && (first + 256 * U) * 8 <= n) {                     // every chunk of the workgroup is whole
         Chunk<DT> c[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) c[u] = load_chunk<DT>(x + (first + u * 256 + threadIdx.x) * 8, 8);
+        for (int u = 0; u < U; u++) c[u] = load_whole<DT>(x + (first + u * 256 + threadIdx.x) * 8);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = (float)c[u].v[e];
-            drop_block(d, (uint32_t)(first + u * 256 + threadIdx.x), v);
-            store_chunk<DT>(y + (first + u * 256 + threadIdx.x) * 8, 8, v);
+            drop_block(d, (uint32_t)(first + u * 256 + threadIdx.x), A.scale, v);
+            store_whole<DT>(y + (first + u * 256 + threadIdx.x) * 8, v);
         }
         return;
     }
@@ -124,180 +57,168 @@ template <int DT, int U, bool ROWS> __global__ __launch_bounds__(256) void k_dro
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] = (float)c.v[e];
-        drop_block(d, (uint32_t)j, v);
+        drop_block(d, (uint32_t)j, A.scale, v);
         store_chunk<DT>(y + i, valid, v);
     }
 }
 
-static __device__ __forceinline__ double block_sum(double v, double *lds) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double s = 0;
-    for (int k = 0; k < (int)blockDim.x / 64; k++) s += lds[k];
-    return s;
-}
-
-static __device__ __forceinline__ float activate(float z, int act) {
-    if (act == PLENREG_ACT_RELU) return z <= 0.f ? 0.f : z;               // (a NaN stays one)
-    if (act == PLENREG_ACT_SILU) return z / (1.f + expf(-z));
-    return z;
-}
-// derivative of the activation at z
-static __device__ __forceinline__ float slope(double z, int act) {
-    if (act == PLENREG_ACT_RELU) return z > 0 ? 1.f : 0.f;
-    if (act == PLENREG_ACT_SILU) { const float s = 1.f / (1.f + expf(-(float)z)); return s * (1.f + (float)z * (1.f - s)); }
-    return 1.f;
-}
-
-// element l, c of group g of slab n after dropout
-template <int DT> static __device__ __forceinline__ double element(const PlenRegNorm &A, const Draw &d, int64_t n, int64_t l, int c, bool &keep) {
-    typedef typename Elem<DT>::T T;
-    const double v = (double)(float)((const T *)A.x)[n * A.x_stride + l * A.C + c];
-    keep = A.cut == 0 || kept(d, (n * A.L + l) * A.C + c);
-    return !keep ? 0.0 : A.cut ? v * (65536.0 / (65536.0 - (double)A.cut)) : v;
-}
-
-// one workgroup per (n, group): mean, centred squares, result
-template <int DT> __global__ __launch_bounds__(256) void k_norm_forward(PlenRegNorm A) {
-    typedef typename Elem<DT>::T T;
-    __shared__ double lds[4];
-    const int D = A.C / A.G, g = blockIdx.x % A.G;
-    const int64_t n = blockIdx.x / A.G, count = A.L * D;
-    Draw d = {};
-    if (A.cut) {
-        d = make_draw(A.rng, A.site, A.cut);
-        if (A.used && blockIdx.x == 0 && threadIdx.x == 0) { A.used[0] = A.rng[0]; A.used[1] = A.rng[1]; }
-    }
-    bool keep;
-    double s = 0;
-    for (int64_t e = threadIdx.x; e < count; e += 256) s += element<DT>(A, d, n, e / D, g * D + (int)(e % D), keep);
-    const double mean = block_sum(s, lds) / count;
-    s = 0;
-    for (int64_t e = threadIdx.x; e < count; e += 256) { const double v = element<DT>(A, d, n, e / D, g * D + (int)(e % D), keep) - mean; s += v * v; }
-    const double rstd = 1.0 / sqrt(block_sum(s, lds) / count + (double)A.eps);
-    if (A.stats && threadIdx.x == 0) { A.stats[2 * (n * A.G + g)] = mean; A.stats[2 * (n * A.G + g) + 1] = rstd; }
-    for (int64_t e = threadIdx.x; e < count; e += 256) {
-        const int64_t l = e / D; const int c = g * D + (int)(e % D);
-        const float xh = (float)((element<DT>(A, d, n, l, c, keep) - mean) * rstd);
-        const float z = xh * load_param(A.w, A.w_dtype, c, 1.f) + load_param(A.b, A.w_dtype, c, 0.f);
-        ((T *)A.out)[(n * A.L + l) * A.C + c] = (T)activate(z, A.act);
-    }
-}
-
-// dz and xh of one element
-template <int DT> static __device__ __forceinline__ void gradients(const PlenRegNorm &A, const Draw &d, int64_t n, int64_t l, int c, bool &keep, float &dz, float &xh) {
-    typedef typename Elem<DT>::T T;
-    const double *st = A.stats + 2 * (n * A.G + c / (A.C / A.G));
-    const double h = (element<DT>(A, d, n, l, c, keep) - st[0]) * st[1];
-    const double z = h * (double)load_param(A.w, A.w_dtype, c, 1.f) + (double)load_param(A.b, A.w_dtype, c, 0.f);
-    xh = (float)h;
-    dz = (float)((const T *)A.dy)[n * A.dy_stride + l * A.C + c] * slope(z, A.act);
-}
-template <int DT> __global__ __launch_bounds__(256) void k_norm_backward(PlenRegNorm A) {
-    typedef typename Elem<DT>::T T;
-    __shared__ double lds[4];
-    const int D = A.C / A.G, g = blockIdx.x % A.G;
-    const int64_t n = blockIdx.x / A.G, count = A.L * D;
-    Draw d = {};
-    if (A.cut) d = make_draw(A.rng, A.site, A.cut);
-    bool keep; float dz, xh;
-    double s1 = 0, s2 = 0;
-    for (int64_t e = threadIdx.x; e < count; e += 256) {
-        const int c = g * D + (int)(e % D);
-        gradients<DT>(A, d, n, e / D, c, keep, dz, xh);
-        const float gw = dz * load_param(A.w, A.w_dtype, c, 1.f);
-        s1 += gw; s2 += (double)gw * xh;
-    }
-    const float m1 = (float)(block_sum(s1, lds) / count), m2 = (float)(block_sum(s2, lds) / count), rstd = (float)A.stats[2 * (n * A.G + g) + 1];
-    for (int64_t e = threadIdx.x; e < count; e += 256) {
-        const int64_t l = e / D; const int c = g * D + (int)(e % D);
-        gradients<DT>(A, d, n, l, c, keep, dz, xh);
-        const float v = rstd * (dz * load_param(A.w, A.w_dtype, c, 1.f) - m1 - xh * m2);
-        ((T *)A.out)[(n * A.L + l) * A.C + c] = (T)(!keep ? 0.f : A.cut ? v * d.scale : v);
-    }
-}
-// one workgroup per channel: dw, db
-template <int DT> __global__ __launch_bounds__(256) void k_norm_params(PlenRegNorm A) {
-    __shared__ double lds[4];
-    const int c = blockIdx.x;
-    Draw d = {};
-    if (A.cut) d = make_draw(A.rng, A.site, A.cut);
-    bool keep; float dz, xh;
-    double s1 = 0, s2 = 0;
-    for (int64_t e = threadIdx.x; e < A.N * A.L; e += 256) {
-        gradients<DT>(A, d, e / A.L, e % A.L, c, keep, dz, xh);
-        s1 += dz; s2 += (double)dz * xh;
-    }
-    s1 = block_sum(s1, lds); s2 = block_sum(s2, lds);
-    if (threadIdx.x == 0) {
-        if (A.db) store_param(A.db, A.w_dtype, c, (float)s1);
-        if (A.dw) store_param(A.dw, A.w_dtype, c, (float)s2);
-    }
-}
-
-#define DROPOUT_SMALL (1 << 18)
+// ---- argument checks
 #define PLENREG_REFUSE (-(int)hipErrorInvalidValue)
-#define PLENREG_BY_TYPE(dtype, call)                  \
-    switch (dtype) {                                  \
-    case PLENREG_F32: call(PLENREG_F32); break;       \
-    case PLENREG_BF16: call(PLENREG_BF16); break;     \
-    default: call(PLENREG_F16); break;                \
-    }
-
 static int launched() { return -(int)hipGetLastError(); }
 static bool bad_type(int t) { return t < PLENREG_F32 || t > PLENREG_F16; }
 // the mask counts blocks of 8 elements in 32 bits
-static bool bad_draw(const uint64_t *rng, uint32_t cut, int site, int64_t n) { return cut > 65536u || site < 0 || (cut && (!rng || n > ((int64_t)1 << 35))); }
+static bool bad_draw(uint32_t cut, int site, int64_t n) { return cut > 65536u || site < 0 || (cut && n > ((int64_t)1 << 35)); }
 static bool bad_norm(const PlenRegNorm *a) {
-    return !a || a->N < 1 || a->L < 1 || a->C < 1 || a->G < 1 || a->C % a->G || a->C > (a->L > 1 ? PLENREG_MAX_C_LONG : PLENREG_MAX_C) || bad_type(a->dtype) || bad_type(a->w_dtype)
-           || a->act < PLENREG_ACT_NONE || a->act > PLENREG_ACT_SILU || !(a->eps > 0.f) || a->N > ((int64_t)1 << 31) - 1 || a->L > ((int64_t)1 << 40) / a->C || a->N > ((int64_t)1 << 40) / (a->L * a->C)
-           || a->N * (int64_t)a->G > ((int64_t)1 << 31) - 1 || bad_draw(a->cut ? (const uint64_t *)1 : nullptr, a->cut, a->site, a->N * a->L * a->C);
+    return !a || a->N < 1 || a->L < 1 || a->C < 1 || a->G < 1 || a->C % a->G || a->C > (a->L > 1 ? PLENREG_MAX_C_LONG : PLENREG_MAX_C) || bad_type(a->dtype)
+           || (a->w_dtype != PLENREG_F32 && a->w_dtype != a->dtype) || a->act < PLENREG_ACT_NONE || a->act > PLENREG_ACT_SILU || !(a->eps > 0.f) || a->N > ((int64_t)1 << 31) - 1
+           || a->L > ((int64_t)1 << 40) / a->C || a->N > ((int64_t)1 << 40) / (a->L * a->C) || a->N * (int64_t)a->G > ((int64_t)1 << 31) - 1 || bad_draw(a->cut, a->site, a->N * a->L * a->C);
+}
+static double drop_scale(uint32_t cut) { return cut < 65536u ? 65536.0 / (65536.0 - (double)cut) : 0.0; }
+
+// ---- launch plans: functions of the sizes alone, so that a workspace asked for and the launch that uses it agree
+static int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+static int log2_up(int64_t v) { int k = 0; while (((int64_t)1 << k) < v) k++; return k; }
+
+static bool by_rows(const PlenRegNorm &a, bool backward) { return a.L == 1 && a.C / a.G <= (backward ? ROW_MAX_BACKWARD : ROW_MAX_FORWARD); }
+static RowLaunch row_plan(const PlenRegNorm &a, bool backward) {
+    const int64_t chunks = div_up(a.C / a.G, 8);
+    RowLaunch r;
+    // forward: up to 4 chunks per lane, so that rows of up to 2048 elements need no barrier
+    r.K = backward || chunks <= 64 ? 1 : chunks <= 128 ? 2 : 4;
+    r.NT = backward ? 512 : 256;
+    r.P.team_log = log2_up(div_up(chunks, r.K));
+    const int teams = r.NT >> r.P.team_log;
+    r.P.gb = a.G < teams ? a.G : teams;
+    r.P.inv_gb = 1.f / (float)r.P.gb;
+    r.P.rb = teams / r.P.gb;
+    const int64_t gy = div_up(a.G, r.P.gb), need = div_up(a.N, r.P.rb);
+    // as many workgroups as are resident at a time, each over several rows; in the backward pass at most 256 rows per lane (its 32-bit sums)
+    int64_t gx = div_up(backward ? 512 : 2048, gy);
+    if (backward && gx < div_up(need, 256)) gx = div_up(need, 256);
+    if (gx > need) gx = need;
+    r.P.trips = (int)div_up(need, gx);
+    r.grid = dim3((unsigned)gx, (unsigned)gy);
+    return r;
+}
+// threads (a multiple of 64) of which the fewest idle when `ncol` of them make a row
+static int fill_threads(int ncol, int lo, int hi) {
+    int best = lo;
+    double most = 0.0;
+    for (int nt = lo; nt <= hi; nt += 64) {
+        const double used = (double)(nt / ncol * ncol) / nt;
+        if (used > most + 1e-9) { most = used; best = nt; }
+    }
+    return best;
+}
+static MapLaunch map_plan(const PlenRegNorm &a) {
+    MapLaunch m;
+    const int D = a.C / a.G;
+    int q = 1;
+    while (q < 8 && (int64_t)q * a.C % 8) q *= 2;
+    if ((int64_t)q * a.C / 8 > 512 || q > a.L) q = 1;
+    m.P.q = q;
+    m.P.ncol = (int)div_up((int64_t)q * a.C, 8);
+    m.P.rows = div_up(a.L, q);
+    m.P.col_blocks = (int)div_up(m.P.ncol, 512);
+    m.P.bcol = (int)div_up(m.P.ncol, m.P.col_blocks);
+    m.P.inv_bcol = 1.f / (float)m.P.bcol;
+    m.NT = fill_threads(m.P.bcol, 256, 512);
+    m.P.R = m.NT / m.P.bcol;
+    // ~4 workgroups per compute unit, at least 4 rows per thread
+    const int64_t turns = div_up(m.P.rows, (int64_t)m.P.R * 4), wanted = div_up(1024, m.P.col_blocks);
+    int64_t splits = a.N >= wanted ? 1 : div_up(wanted, a.N);
+    if (splits > turns) splits = turns;
+    m.P.rows_per = div_up(m.P.rows, splits);
+    m.P.splits = (int)div_up(m.P.rows, m.P.rows_per);
+    m.P.lanes_log = log2_up(div_up((int64_t)m.P.R * q * (a.C % 8 || D % 8 ? D : D / 8), 4));
+    if (m.P.lanes_log > 6) m.P.lanes_log = 6;
+    m.sums = dim3((unsigned)(a.N * m.P.splits < 2048 ? a.N * m.P.splits : 2048), (unsigned)m.P.col_blocks);
+    m.stat_blocks = (unsigned)(a.N * a.G < 4 * 65536 ? div_up(a.N * a.G, 4) : 65536);
+    int64_t blocks = div_up(2048, a.N * m.P.col_blocks);
+    if (blocks > turns) blocks = turns;
+    m.P.apply_rows = div_up(m.P.rows, blocks);
+    m.P.row_blocks = (int)div_up(m.P.rows, m.P.apply_rows);
+    const int64_t items = a.N * m.P.col_blocks * m.P.row_blocks;
+    m.apply_blocks = (unsigned)(items < 65536 ? items : 65536);
+    return m;
+}
+// bytes of the partial pairs of a map launch
+static int64_t part_bytes(const PlenRegNorm &a, const MapLaunch &m) { return a.N * a.G * m.P.splits * m.P.col_blocks * 16; }
+
+static const NormEntry &entry(const PlenRegNorm &a) {
+    if (a.dtype == PLENREG_F32) return plenreg_norm_f32_f32();
+    if (a.dtype == PLENREG_BF16) return a.w_dtype == PLENREG_F32 ? plenreg_norm_bf16_f32() : plenreg_norm_bf16_bf16();
+    return a.w_dtype == PLENREG_F32 ? plenreg_norm_f16_f32() : plenreg_norm_f16_f16();
+}
+static NormArgs kernel_args(const PlenRegNorm &a) {
+    NormArgs k;
+    k.x = a.x; k.dy = a.dy; k.w = a.w; k.b = a.b; k.out = a.out; k.stats = (double2 *)a.stats; k.rng = a.rng; k.used = a.used;
+    k.N = a.N; k.x_stride = a.x_stride; k.dy_stride = a.dy_stride; k.size = a.L * a.C;
+    k.C = a.C; k.G = a.G; k.D = a.C / a.G; k.act = a.act; k.site = a.site; k.cut = a.cut;
+    k.inv_count = 1.0 / ((double)a.L * k.D); k.scale = drop_scale(a.cut); k.eps = (double)a.eps;
+    k.inv_D = 1.f / (float)k.D; k.inv_C = 1.f / (float)a.C;
+    return k;
 }
 
 extern "C" {
 
 int plenreg_dropout(const PlenRegDropout *a, void *stream) {
-    if (!a || !a->x || !a->y || !a->rng || a->rows < 1 || a->cols < 1 || a->rows > ((int64_t)1 << 35) / a->cols || a->x_stride < 0 || bad_type(a->dtype)
-        || bad_draw(a->rng, a->cut, a->site, a->rows * a->cols)) return PLENREG_REFUSE;
-    const int64_t chunks = (a->rows * a->cols + 7) / 8;
+    if (!a || !a->x || !a->y || !a->rng || a->rows < 1 || a->cols < 1 || a->rows > ((int64_t)1 << 35) / a->cols || a->x_stride < 0 || bad_type(a->dtype) || bad_draw(a->cut, a->site, a->rows * a->cols))
+        return PLENREG_REFUSE;
+    const DropArgs k = {a->x, a->y, a->rng, a->used, a->rows, a->cols, a->x_stride, a->cut, a->site, (float)drop_scale(a->cut)};
+    const hipStream_t s = (hipStream_t)stream;
+    // few chunks: one per thread, so that every compute unit gets some; many: four, whose loads are in flight together
+    const int64_t chunks = div_up(a->rows * a->cols, 8);
     const bool rows = a->rows > 1 && a->x_stride != a->cols, small = chunks <= DROPOUT_SMALL;
-    const dim3 grid((unsigned)((chunks + (small ? 255 : 1023)) / (small ? 256 : 1024)));
-#define CALL(DT)                                                                                                                              \
-    small ? (rows ? k_dropout<DT, 1, true><<<grid, 256, 0, (hipStream_t)stream>>>(*a) : k_dropout<DT, 1, false><<<grid, 256, 0, (hipStream_t)stream>>>(*a)) \
-          : (rows ? k_dropout<DT, 4, true><<<grid, 256, 0, (hipStream_t)stream>>>(*a) : k_dropout<DT, 4, false><<<grid, 256, 0, (hipStream_t)stream>>>(*a))
-    PLENREG_BY_TYPE(a->dtype, CALL)
+    const unsigned grid = (unsigned)div_up(chunks, small ? 256 : 1024);
+#define CALL(DT)                                                                                          \
+    if (small) { if (rows) k_dropout<DT, 1, true><<<grid, 256, 0, s>>>(k); else k_dropout<DT, 1, false><<<grid, 256, 0, s>>>(k); } \
+    else if (rows) k_dropout<DT, 4, true><<<grid, 256, 0, s>>>(k);                                        \
+    else k_dropout<DT, 4, false><<<grid, 256, 0, s>>>(k)
+    if (a->dtype == PLENREG_F32) { CALL(PLENREG_F32); }
+    else if (a->dtype == PLENREG_BF16) { CALL(PLENREG_BF16); }
+    else { CALL(PLENREG_F16); }
 #undef CALL
     return launched();
 }
 
 int64_t plenreg_norm_workspace(const PlenRegNorm *a, int backward) {
-    (void)backward;
-    return bad_norm(a) ? PLENREG_REFUSE : 0;
+    if (bad_norm(a)) return PLENREG_REFUSE;
+    if (by_rows(*a, backward)) return backward ? (int64_t)row_plan(*a, true).grid.x * 2 * a->C * 4 : 0;
+    const MapLaunch m = map_plan(*a);
+    return part_bytes(*a, m) + (backward ? a->N * a->G * 8 + (int64_t)m.sums.x * 2 * a->C * 4 : a->N * a->G * 16);
 }
 
 int plenreg_norm_forward(const PlenRegNorm *a, void *stream) {
     if (bad_norm(a) || !a->x || !a->out || a->x_stride < 0 || (a->cut && !a->rng)) return PLENREG_REFUSE;
-    const dim3 grid((unsigned)(a->N * a->G));
-#define CALL(DT) k_norm_forward<DT><<<grid, 256, 0, (hipStream_t)stream>>>(*a)
-    PLENREG_BY_TYPE(a->dtype, CALL)
-#undef CALL
+    NormArgs k = kernel_args(*a);
+    if (by_rows(*a, false)) {
+        entry(*a).row_forward(k, row_plan(*a, false), (hipStream_t)stream);
+        return launched();
+    }
+    if (!a->ws) return PLENREG_REFUSE;
+    const MapLaunch m = map_plan(*a);
+    if (!k.stats) k.stats = (double2 *)((char *)a->ws + part_bytes(*a, m));
+    entry(*a).map_forward(k, m, (double2 *)a->ws, (hipStream_t)stream);
     return launched();
 }
 
 int plenreg_norm_backward(const PlenRegNorm *a, void *stream) {
     if (bad_norm(a) || !a->x || !a->dy || !a->out || !a->stats || a->x_stride < 0 || a->dy_stride < 0 || (a->cut && !a->rng)) return PLENREG_REFUSE;
-    const dim3 grid((unsigned)(a->N * a->G));
-#define CALL(DT) k_norm_backward<DT><<<grid, 256, 0, (hipStream_t)stream>>>(*a)
-    PLENREG_BY_TYPE(a->dtype, CALL)
-#undef CALL
-    if (a->dw || a->db) {
-        const dim3 cols((unsigned)a->C);
-#define CALL(DT) k_norm_params<DT><<<cols, 256, 0, (hipStream_t)stream>>>(*a)
-        PLENREG_BY_TYPE(a->dtype, CALL)
-#undef CALL
+    const bool params = a->dw || a->db, rows = by_rows(*a, true);
+    if ((params || !rows) && !a->ws) return PLENREG_REFUSE;
+    const NormArgs k = kernel_args(*a);
+    const NormEntry &e = entry(*a);
+    if (rows) {
+        const RowLaunch r = row_plan(*a, true);
+        e.row_backward(k, r, params ? (float *)a->ws : nullptr, (hipStream_t)stream);
+        if (params) e.params(k, (const float *)a->ws, (int)r.grid.x, a->dw, a->db, (hipStream_t)stream);
+        return launched();
     }
+    const MapLaunch m = map_plan(*a);
+    char *ws = (char *)a->ws;
+    float2 *means = (float2 *)(ws + part_bytes(*a, m));
+    e.map_backward(k, m, (double2 *)ws, means, params ? (float *)(means + a->N * a->G) : nullptr, a->dw, a->db, (hipStream_t)stream);
     return launched();
 }
 

@@ -1,0 +1,755 @@
+// regularise_norm.hip -- group norm with an activation, with dropout before it or without, for one pair of element types: REG_DT of x and of the results, REG_WT of
+// the parameters; REG_ENTRY names the table of launches.
+//
+// Statistics are sums of (x - s) and (x - s)^2 in 64 bits, s = an element of the input: a 64-bit addition costs a vector slot like a 32-bit one on this chip, one
+// pass over the data is enough, the sums of different workgroups join by addition, a constant input has exactly no variance, and the variance survives a
+// mean of any size.  (It is also what the gate of ReLU's gradient is decided with.)  The rest is in 32 bits, with the mean as a sum of two floats, so that x - mean is
+// exact to a rounding of its own.
+//
+// Code size counts: the instruction cache is cold at each launch, and a kernel that runs its text once is bound by fetching it.  So: quotients come from the
+// host, the form without partial chunks (V > 0) is a variant of its own, parameter types are compiled in.
+//
+// No variant may spill to scratch memory (tests/test_regularise_cpu.py): a spilling one has lost values of lanes that a divergent branch left out.
+#include "regularise.h"
+
+#define DT REG_DT
+#define WT REG_WT
+typedef Elem<DT>::T T;
+typedef Elem<WT>::T W;
+// variants: 0 = chunks may be partial, 1 = all chunks are whole, 2 = and belong to one group each
+namespace {
+
+__device__ __forceinline__ float logistic(float z) {
+    // 16-bit results: exponential and reciprocal from the hardware's approximations, off by (|z| + 4) 2^-24 of the value, a 2^8th of the result's own rounding and less
+    if (DT != PLENREG_F32) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
+    return 1.f / (1.f + expf(-z));
+}
+__device__ __forceinline__ void activate(float (&z)[8], int act) {
+    if (act == PLENREG_ACT_RELU) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) z[e] = z[e] <= 0.f ? 0.f : z[e];             // (a NaN stays one)
+    } else if (act == PLENREG_ACT_SILU) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) z[e] *= logistic(z[e]);
+    }
+}
+// 1 / sqrt(v) in 64 bits: the hardware's approximation and two Newton steps
+__device__ __forceinline__ double inverse_sqrt(double v) {
+    double r = __builtin_amdgcn_rsq(v);
+    r = fma(0.5 * r, fma(-v * r, r, 1.0), r);
+    return fma(0.5 * r, fma(-v * r, r, 1.0), r);
+}
+// sums of (x - s), (x - s)^2 -> the pair that NormArgs.stats holds
+__device__ __forceinline__ double2 finish_stats(const NormArgs &A, double s, double sum, double squares) {
+    const double m = sum * A.inv_count;
+    double var = fma(-m, m, squares * A.inv_count);
+    if (var < 0.0) var = 0.0;
+    return double2{s + m, A.scale * inverse_sqrt(fma(var, A.scale * A.scale, A.eps))};
+}
+__device__ __forceinline__ void write_used(const NormArgs &A) {
+    if (A.used && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) { A.used[0] = A.rng[0]; A.used[1] = A.rng[1]; }
+}
+// a chunk's elements as floats; masked ones as zeros
+template <bool DROP, int E> __device__ __forceinline__ void unpack(const Chunk<E> &c, uint32_t kept_bits, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = !DROP || kept_bits >> e & 1u ? (float)c.v[e] : 0.f;
+}
+
+// ---- sums over 2^log neighbouring lanes, left in each of them: exchanges within 16 lanes by DPP, beyond by the row swaps
+template <int CTRL> __device__ __forceinline__ float from_lane(float v) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)); }
+template <int CTRL> __device__ __forceinline__ double from_lane(double v) {
+    const int lo = __builtin_amdgcn_mov_dpp(__double2loint(v), CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_mov_dpp(__double2hiint(v), CTRL, 0xf, 0xf, true);
+    return __hiloint2double(hi, lo);
+}
+// v of this row of 16 (half of 32) lanes + v of its neighbour
+__device__ __forceinline__ float add_swapped(float v, bool halves) {
+    const uint32_t u = __float_as_uint(v);
+    const auto s = halves ? __builtin_amdgcn_permlane32_swap(u, u, false, false) : __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+__device__ __forceinline__ double add_swapped(double v, bool halves) {
+    const uint32_t lo = (uint32_t)__double2loint(v), hi = (uint32_t)__double2hiint(v);
+    const auto a = halves ? __builtin_amdgcn_permlane32_swap(lo, lo, false, false) : __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+    const auto b = halves ? __builtin_amdgcn_permlane32_swap(hi, hi, false, false) : __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+    return __hiloint2double((int)b[0], (int)a[0]) + __hiloint2double((int)b[1], (int)a[1]);
+}
+template <typename F> __device__ __forceinline__ void lanes_sum2(F &a, F &b, int log) {
+    if (log < 1) return;
+    a += from_lane<0xB1>(a); b += from_lane<0xB1>(b);            // lane ^ 1
+    if (log < 2) return;
+    a += from_lane<0x4E>(a); b += from_lane<0x4E>(b);            // lane ^ 2
+    if (log < 3) return;
+    a += from_lane<0x141>(a); b += from_lane<0x141>(b);          // mirrored in 8 lanes (all four lanes of each half hold the same by now)
+    if (log < 4) return;
+    a += from_lane<0x140>(a); b += from_lane<0x140>(b);          // mirrored in 16 lanes
+    if (log < 5) return;
+    a = add_swapped(a, false); b = add_swapped(b, false);
+    if (log < 6) return;
+    a = add_swapped(a, true); b = add_swapped(b, true);
+}
+// ... over a team of up to NT lanes; `turn` counts the calls.  Two buffers in turn: whoever writes one again has passed the barrier of the turn between, after which
+// nobody still reads it.
+template <int NT, typename F> __device__ __forceinline__ void team_sum2(F &a, F &b, int log, int turn, double2 (&lds)[2][NT / 64]) {
+    lanes_sum2(a, b, log);
+    if (log > 6) {
+        double2 *p = lds[turn & 1];
+        if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = double2{(double)a, (double)b};
+        __syncthreads();
+        const int waves = 1 << (log - 6), w0 = (threadIdx.x >> log) << (log - 6);
+        double s = 0.0, q = 0.0;
+        for (int k = 0; k < waves; k++) { s += p[w0 + k].x; q += p[w0 + k].y; }
+        a = (F)s; b = (F)q;
+    }
+}
+
+// ---- the pass back through the activation for one chunk: xh and dy -> dz (zeros beyond `valid`).  ReLU's gate: where 32 bits leave the sign of z open it is decided in
+// 64, from the inputs in memory (x of the chunk at px, statistics and parameters of channel (c0 + e) % C): the gradient jumps there.  xh is off by at most 4 roundings.
+template <bool DROP, int V> __device__ __forceinline__ void back_activation(const NormArgs &A, const T *px, int64_t n, int c0, int valid, uint32_t kept_bits, const float (&xh)[8], const float (&dy)[8],
+                                                                             const float (&w)[8], const float (&b)[8], float (&dz)[8]) {
+    if (A.act == PLENREG_ACT_RELU) {
+        uint32_t open = 0, doubt = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float t = xh[e] * w[e], z = t + b[e];
+            open |= z > 0.f ? 1u << e : 0u;
+            doubt |= fabsf(z) <= 6e-7f * (fabsf(t) + fabsf(b[e])) ? 1u << e : 0u;
+        }
+        if (V == 0) doubt &= (1u << valid) - 1u;
+#pragma unroll 1
+        while (doubt) {
+            const int e = __ffs(doubt) - 1, c = (c0 + e) % A.C;
+            doubt &= doubt - 1u;
+            const double2 st = A.stats[n * A.G + c / A.D];
+            const double v = DROP && !(kept_bits >> e & 1u) ? 0.0 : (double)(float)px[e], wd = A.w ? (double)(float)((const W *)A.w)[c] : 1.0, bd = A.b ? (double)(float)((const W *)A.b)[c] : 0.0;
+            open = (v - st.x) * st.y * wd + bd > 0.0 ? open | 1u << e : open & ~(1u << e);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) dz[e] = open >> e & 1u ? dy[e] : 0.f;
+    } else if (A.act == PLENREG_ACT_SILU) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float z = xh[e] * w[e] + b[e], s = logistic(z);
+            dz[e] = dy[e] * (s * (1.f + z * (1.f - s)));
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) dz[e] = dy[e];
+    }
+    if (V == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) dz[e] = e < valid ? dz[e] : 0.f;
+    }
+}
+
+// ---- rows of one position (L = 1): a team of lanes per (row, group), K chunks per lane held in registers, one pass.  Teams of one wave join their sums by lane exchange,
+//      wider ones through LDS.  A workgroup walks down the rows with its groups fixed, so that a lane keeps its channels: their parameters (and in the backward
+//      pass their gradients) stay in registers.
+struct RowPlace { int lane, gl, g, row; bool mine; };
+template <int NT> __device__ __forceinline__ RowPlace row_place(const NormArgs &A, const RowPlan &P) {
+    RowPlace p;
+    const int team = threadIdx.x >> P.team_log;
+    p.lane = threadIdx.x & ((1 << P.team_log) - 1);
+    p.row = small_quotient(team, P.inv_gb);
+    p.gl = team - p.row * P.gb;
+    p.g = blockIdx.y * P.gb + p.gl;
+    p.mine = p.row < P.rb && p.g < A.G;
+    return p;
+}
+template <int K> __device__ __forceinline__ void row_valid(const NormArgs &A, const RowPlan &P, const RowPlace &p, int (&valid)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int left = A.D - 8 * (p.lane + (k << P.team_log));
+        valid[k] = !p.mine || left < 0 ? 0 : left > 8 ? 8 : left;
+    }
+}
+template <int V, int E> __device__ __forceinline__ Chunk<E> row_load(const typename Elem<E>::T *p, int valid) {
+    Chunk<E> c = {};
+    if (valid) c = V ? load_whole<E>(p) : load_chunk<E>(p, valid);
+    return c;
+}
+template <int V> __device__ __forceinline__ void row_store(T *p, int valid, const float (&v)[8]) {
+    if (V) store_whole<DT>(p, v);
+    else store_chunk<DT>(p, valid, v);
+}
+// parameters of a lane's chunk, 1 / 0 where there are none
+template <int V> __device__ __forceinline__ void row_params(const void *p, int c0, int valid, float otherwise, float (&out)[8]) {
+    if (p) {
+        const Chunk<WT> c = row_load<V, WT>((const W *)p + c0, valid);
+#pragma unroll
+        for (int e = 0; e < 8; e++) out[e] = (float)c.v[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) out[e] = otherwise;
+    }
+}
+
+template <int V, int K, int NT, bool DROP> __global__ __launch_bounds__(NT) void k_row_forward(NormArgs A, RowPlan P) {
+    __shared__ double2 lds[2][NT / 64];
+    const RowPlace p = row_place<NT>(A, P);
+    const int step = 8 << P.team_log, c0 = p.g * A.D + 8 * p.lane;
+    int valid[K];
+    row_valid<K>(A, P, p, valid);
+    int64_t n = (int64_t)blockIdx.x * P.rb + p.row;
+    Chunk<DT> x[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) x[k] = row_load<V, DT>((const T *)A.x + n * A.x_stride + c0 + k * step, n < A.N ? valid[k] : 0);
+    float w[K][8], b[K][8];
+#pragma unroll
+    for (int k = 0; k < K; k++) { row_params<V>(A.w, c0 + k * step, valid[k], 1.f, w[k]); row_params<V>(A.b, c0 + k * step, valid[k], 0.f, b[k]); }
+    Draw d = {};
+    if (DROP) { d = make_draw(A.rng, A.site, A.cut); write_used(A); }
+#pragma unroll 1
+    for (int turn = 0; turn < P.trips; turn++) {
+        const bool on = p.mine && n < A.N;
+        const int64_t next = n + (int64_t)gridDim.x * P.rb;
+        float v[K][8];
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            unpack<DROP>(x[k], DROP && on && valid[k] ? chunk_mask(d, n * A.C + c0 + k * step) : 255u, v[k]);
+            x[k] = row_load<V, DT>((const T *)A.x + next * A.x_stride + c0 + k * step, turn + 1 < P.trips && next < A.N ? valid[k] : 0);      // the next row's, while this one is worked on
+        }
+        // s: the group's first element, after the mask
+        float first;
+        if (P.team_log <= 6) first = __shfl(v[0][0], (threadIdx.x & 63) >> P.team_log << P.team_log);
+        else {
+            first = on ? (float)((const T *)A.x)[n * A.x_stride + p.g * A.D] : 0.f;
+            if (DROP && on && !kept(d, n * A.C + p.g * A.D)) first = 0.f;
+        }
+        const double shift = (double)first;
+        double s = 0.0, q = 0.0;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                if ((V ? valid[k] : valid[k] - e) <= 0) v[k][e] = first;                     // what is not there adds nothing
+                const double t = (double)v[k][e] - shift;
+                s += t; q = fma(t, t, q);
+            }
+        }
+        team_sum2<NT>(s, q, P.team_log, turn, lds);
+        const double2 st = finish_stats(A, shift, s, q);
+        if (on) {
+            if (A.stats && p.lane == 0) A.stats[n * A.G + p.g] = st;
+            const float mean = (float)st.x, rest = (float)(st.x - (double)mean), rstd = (float)st.y;
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                if (!valid[k]) continue;
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[k][e] = ((v[k][e] - mean) - rest) * rstd * w[k][e] + b[k][e];
+                activate(v[k], A.act);
+                row_store<V>((T *)A.out + n * A.C + c0 + k * step, valid[k], v[k]);
+            }
+        }
+        n = next;
+    }
+}
+
+// backward of the rows.  Each workgroup leaves one row of partial parameter gradients: part[blockIdx.x][0 / 1][C] = dw, db of its rows, summed over its teams in LDS.
+template <int V, int NT, bool DROP> __global__ __launch_bounds__(NT) void k_row_backward(NormArgs A, RowPlan P, float *part) {
+    __shared__ double2 lds[2][NT / 64];
+    __shared__ float joined[NT * 8];
+    const RowPlace p = row_place<NT>(A, P);
+    const int c0 = p.g * A.D + 8 * p.lane;
+    int valid[1];
+    row_valid<1>(A, P, p, valid);
+    int64_t n = (int64_t)blockIdx.x * P.rb + p.row;
+    float w[8], b[8], dw[8] = {}, db[8] = {};
+    row_params<V>(A.w, c0, valid[0], 1.f, w);
+    row_params<V>(A.b, c0, valid[0], 0.f, b);
+    Draw d = {};
+    if (DROP) d = make_draw(A.rng, A.site, A.cut);
+#pragma unroll 1
+    for (int turn = 0; turn < P.trips; turn++, n += (int64_t)gridDim.x * P.rb) {
+        const bool on = p.mine && n < A.N && valid[0];
+        const T *px = (const T *)A.x + n * A.x_stride + c0;
+        float xh[8] = {}, gw[8] = {}, s = 0.f, q = 0.f, rstd = 0.f;
+        uint32_t m = 255u;
+        if (on) {
+            const Chunk<DT> x = row_load<V, DT>(px, valid[0]), g = row_load<V, DT>((const T *)A.dy + n * A.dy_stride + c0, valid[0]);
+            const double2 st = A.stats[n * A.G + p.g];
+            if (DROP) m = chunk_mask(d, n * A.C + c0);
+            const float mean = (float)st.x, rest = (float)(st.x - (double)mean);
+            rstd = (float)st.y;
+            float dy[8], dz[8];
+            unpack<DROP>(x, m, xh);
+            unpack<false>(g, 255u, dy);
+#pragma unroll
+            for (int e = 0; e < 8; e++) xh[e] = ((xh[e] - mean) - rest) * rstd;
+            back_activation<DROP, V>(A, px, n, c0, valid[0], m, xh, dy, w, b, dz);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                gw[e] = dz[e] * w[e];
+                s += gw[e]; q = fmaf(gw[e], xh[e], q);
+                db[e] += dz[e]; dw[e] = fmaf(dz[e], xh[e], dw[e]);
+            }
+        }
+        team_sum2<NT>(s, q, P.team_log, turn, lds);
+        if (on) {
+            const float m1 = s * (float)A.inv_count, m2 = q * (float)A.inv_count;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float t = rstd * (gw[e] - m1 - xh[e] * m2);
+                gw[e] = !DROP || m >> e & 1u ? t : 0.f;
+            }
+            row_store<V>((T *)A.out + n * A.C + c0, valid[0], gw);
+        }
+    }
+    if (!part) return;
+    const int width = 8 << P.team_log, columns = P.gb * width;                  // joined[row][group of the workgroup][channel of the group, padded to whole chunks]
+#pragma unroll 1
+    for (int pass = 0; pass < 2; pass++) {
+        __syncthreads();
+        if (p.row < P.rb)
+#pragma unroll
+            for (int e = 0; e < 8; e++) joined[p.row * columns + p.gl * width + 8 * p.lane + e] = pass ? db[e] : dw[e];
+        __syncthreads();
+        for (int j = threadIdx.x; j < columns; j += NT) {
+            const int gj = j >> (P.team_log + 3), c = j & (width - 1), g = blockIdx.y * P.gb + gj;
+            if (g >= A.G || c >= A.D) continue;
+            float t = 0.f;
+            for (int r = 0; r < P.rb; r++) t += joined[r * columns + j];
+            part[((int64_t)blockIdx.x * 2 + pass) * A.C + g * A.D + c] = t;
+        }
+    }
+}
+
+// dw, db = column sums of part[rows][2][C] in 64 bits: 16 columns per workgroup of 1024 threads, 64 rows at a time
+__device__ __forceinline__ void param_columns(const NormArgs &A, const float *part, int rows, int block, void *dw, void *db, double (&lds)[64][17]) {
+    const int64_t width = 2 * (int64_t)A.C, column = (int64_t)block * 16 + (threadIdx.x & 15);
+    const int r0 = threadIdx.x >> 4;
+    double s = 0.0;
+    if (column < width) {
+        int r = r0;
+        for (; r + 7 * 64 < rows; r += 8 * 64) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = part[(r + k * 64) * width + column];
+#pragma unroll
+            for (int k = 0; k < 8; k++) s += (double)v[k];
+        }
+        for (; r < rows; r += 64) s += (double)part[r * width + column];
+    }
+    lds[r0][threadIdx.x & 15] = s;
+    __syncthreads();
+    if (threadIdx.x < 256) {
+        // column t / 16, rows t % 16 + 16 k: then over 16 lanes
+        const int col = threadIdx.x >> 4, r = threadIdx.x & 15;
+        double t = (lds[r][col] + lds[r + 16][col]) + (lds[r + 32][col] + lds[r + 48][col]), unused = 0.0;
+        lanes_sum2(t, unused, 4);
+        const int64_t c = (int64_t)block * 16 + col;
+        if (r == 0 && c < width) {
+            void *to = c < A.C ? dw : db;
+            if (to) ((W *)to)[c < A.C ? c : c - A.C] = (W)(float)t;
+        }
+    }
+}
+__global__ __launch_bounds__(1024) void k_row_params(NormArgs A, const float *part, int rows, void *dw, void *db) {
+    __shared__ double lds[64][17];
+    param_columns(A, part, rows, blockIdx.x, dw, db, lds);
+}
+
+// ---- many positions (or rows too wide for a workgroup's lanes): a slab is L C contiguous elements, seen as rows of q C (q = the smallest number of positions that fill
+//      whole chunks, so that odd channel counts load whole chunks too; 1 where that would be too wide).  A thread owns one chunk column (8 fixed virtual channels v,
+//      channel v % C) and walks down the rows; workgroups split the rows and, where they are wide, the columns.  Statistics, their join, and the result are launches of their
+//      own: the second reading of x comes out of the caches while it fits.
+struct Column { int first, col, r, tail; bool mine; };
+__device__ __forceinline__ Column my_column(const NormArgs &A, const MapPlan &P, int col_block) {
+    Column c;
+    c.first = col_block * P.bcol;
+    c.r = small_quotient(threadIdx.x, P.inv_bcol);
+    c.col = c.first + (int)threadIdx.x - c.r * P.bcol;
+    c.mine = c.r < P.R && c.col < P.ncol;
+    const int left = P.q * A.C - 8 * c.col;
+    c.tail = left > 8 ? 8 : left;
+    return c;
+}
+// U chunks at rows row, row + R, ...: how much of each there is, and its elements.  V > 0: whole or beyond the end.
+template <int V, int U> __device__ __forceinline__ void map_valid(const NormArgs &A, const MapPlan &P, const Column &c, int64_t row, int64_t end, int64_t width, int (&valid)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int64_t at = row + u * P.R, left = A.size - (at * width + 8 * c.col);
+        valid[u] = at >= end ? 0 : V ? 8 : left < c.tail ? (int)left : c.tail;
+        if (!V && valid[u] < 0) valid[u] = 0;
+    }
+}
+template <int V, int U> __device__ __forceinline__ void map_load(const T *p, int64_t step, const int (&valid)[U], Chunk<DT> (&v)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if (valid[u]) v[u] = V ? load_whole<DT>(p + u * step) : load_chunk<DT>(p + u * step, valid[u]);
+}
+// channel and group of the first of a thread's virtual channels; `next` steps to the one after
+struct Channel {
+    int c, g, d;
+    __device__ __forceinline__ Channel(const NormArgs &A, int v) {
+        c = v - small_quotient(v, A.inv_C) * A.C;
+        g = small_quotient(c, A.inv_D);
+        d = c - g * A.D;
+    }
+    __device__ __forceinline__ void next(const NormArgs &A) {
+        c++; d++;
+        if (d == A.D) { d = 0; g++; }
+        if (c == A.C) { c = 0; g = 0; }
+    }
+};
+// sums over the workgroup's threads of a[8], b[8] per virtual channel, joined per group: out[g stride] (zeros for a group with no channel in this workgroup's columns).
+// `lds`: blockDim.x (8 blockDim.x, V < 2) pairs.
+template <int V> __device__ __forceinline__ void join_groups(const double (&a)[8], const double (&b)[8], const NormArgs &A, const MapPlan &P, const Column &c, double2 *lds, double2 *out, int64_t stride) {
+    const int NT = blockDim.x, at = c.r * P.bcol + c.col - c.first;
+    __syncthreads();
+    if (c.mine) {
+        if (V == 2) lds[at] = double2{((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7])), ((b[0] + b[1]) + (b[2] + b[3])) + ((b[4] + b[5]) + (b[6] + b[7]))};
+        else
+#pragma unroll
+            for (int e = 0; e < 8; e++) lds[e * NT + at] = double2{a[e], b[e]};
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & ((1 << P.lanes_log) - 1), teams = NT >> P.lanes_log;
+    const int D = V == 2 ? A.D >> 3 : A.D;                                                           // channels, or whole chunks of them
+    const int from = P.col_blocks == 1 ? 0 : V == 2 ? c.first : 8 * c.first, to = P.col_blocks == 1 ? A.G * D : from + (V == 2 ? P.bcol : 8 * P.bcol);
+#pragma unroll 1
+    for (int g0 = 0; g0 < A.G; g0 += teams) {                        // (every lane takes every turn: the exchange needs them all)
+        const int g = g0 + (threadIdx.x >> P.lanes_log);
+        const int lo = g * D > from ? g * D : from, hi = (g + 1) * D < to ? (g + 1) * D : to, per = hi - lo;
+        double s = 0.0, q = 0.0;
+        if (g < A.G && per > 0) {
+            const float inv_per = 1.f / (float)per;
+            for (int i = lane, entries = P.R * P.q * per; i < entries; i += 1 << P.lanes_log) {
+                const int t = small_quotient(i, inv_per), j = i - t * per;
+                double2 v;
+                if (V == 2) v = lds[t * P.bcol + lo + j - c.first];
+                else {
+                    const int r = t / P.q, vc = (t - r * P.q) * A.C + lo + j;
+                    v = lds[(vc & 7) * NT + r * P.bcol + (vc >> 3) - c.first];
+                }
+                s += v.x; q += v.y;
+            }
+        }
+        lanes_sum2(s, q, P.lanes_log);
+        if (g < A.G && lane == 0) out[(int64_t)g * stride] = double2{s, q};
+    }
+}
+// sums over the `splits` partial pairs of one (n, g), by one wave
+__device__ __forceinline__ double2 join_splits(const double2 *part, int splits) {
+    double s = 0.0, q = 0.0;
+    for (int k = threadIdx.x & 63; k < splits; k += 64) { const double2 t = part[k]; s += t.x; q += t.y; }
+    lanes_sum2(s, q, 6);
+    return double2{s, q};
+}
+// s of a slab: its first element, after the mask
+template <bool DROP> __device__ __forceinline__ double slab_shift(const NormArgs &A, const Draw &d, int64_t n) {
+    const float v = (float)((const T *)A.x)[n * A.x_stride];
+    return DROP && !kept(d, n * A.size) ? 0.0 : (double)v;
+}
+
+// part[n][g][split][column block] = sums of (x - s), (x - s)^2
+template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_sums(NormArgs A, MapPlan P, double2 *part) {
+    extern __shared__ double2 lds[];
+    const int64_t width = (int64_t)P.q * A.C, items = A.N * P.splits;
+    const Column c = my_column(A, P, blockIdx.y);
+    Draw d = {};
+    if (DROP) { d = make_draw(A.rng, A.site, A.cut); write_used(A); }
+#pragma unroll 1
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t n = item / P.splits, split = item - n * P.splits;
+        const T *x = (const T *)A.x + n * A.x_stride;
+        const double shift = slab_shift<DROP>(A, d, n);
+        double s[8] = {}, q[8] = {};
+        const int64_t end = (split + 1) * P.rows_per < P.rows ? (split + 1) * P.rows_per : P.rows;
+        if (c.mine)
+#pragma unroll 1
+            for (int64_t row = split * P.rows_per + c.r; row < end; row += 4 * P.R) {
+                const int64_t off = row * width + 8 * c.col;
+                int valid[4];
+                Chunk<DT> v[4];
+                map_valid<V, 4>(A, P, c, row, end, width, valid);
+                map_load<V, 4>(x + off, P.R * width, valid, v);
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    if (!valid[u]) continue;
+                    float f[8];
+                    unpack<DROP>(v[u], DROP ? chunk_mask(d, n * A.size + off + u * P.R * width) : 255u, f);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        double t = (double)f[e] - shift;
+                        if (!V && e >= valid[u]) t = 0.0;
+                        s[e] += t; q[e] = fma(t, t, q[e]);
+                    }
+                }
+            }
+        const int64_t parts = (int64_t)P.splits * P.col_blocks;
+        join_groups<V>(s, q, A, P, c, lds, part + n * A.G * parts + split * P.col_blocks + blockIdx.y, parts);
+    }
+}
+template <bool DROP> __global__ __launch_bounds__(256) void k_map_stats(NormArgs A, int splits, const double2 *part) {
+    Draw d = {};
+    if (DROP) d = make_draw(A.rng, A.site, A.cut);
+    for (int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); item < A.N * A.G; item += (int64_t)gridDim.x * 4) {
+        const double shift = slab_shift<DROP>(A, d, item / A.G);
+        const double2 t = join_splits(part + item * splits, splits);
+        if ((threadIdx.x & 63) == 0) A.stats[item] = finish_stats(A, shift, t.x, t.y);
+    }
+}
+// statistics and parameters of a thread's 8 virtual channels (V = 2: one group, statistics in element 0).
+// (The column is hidden from the compiler: it would keep every address of a loop over slabs in registers, and spill.)
+template <int V> struct Constants { float mean[V == 2 ? 1 : 8], rest[V == 2 ? 1 : 8], rstd[V == 2 ? 1 : 8], w[8], b[8]; };
+template <int V> __device__ __forceinline__ void load_constants(const NormArgs &A, int64_t n, int col, Constants<V> &k) {
+    asm volatile("" : "+v"(col));
+    Channel ch(A, 8 * col);
+    const double2 *stats = A.stats + n * A.G;
+    if (V == 2) {
+        const double2 st = stats[ch.g];
+        k.mean[0] = (float)st.x; k.rest[0] = (float)(st.x - (double)k.mean[0]); k.rstd[0] = (float)st.y;
+        row_params<1>(A.w, ch.c, 8, 1.f, k.w);
+        row_params<1>(A.b, ch.c, 8, 0.f, k.b);
+    } else
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const double2 st = stats[ch.g];
+            const int i = V == 2 ? 0 : e;
+            k.mean[i] = (float)st.x; k.rest[i] = (float)(st.x - (double)k.mean[i]); k.rstd[i] = (float)st.y;
+            k.w[e] = A.w ? (float)((const W *)A.w)[ch.c] : 1.f;
+            k.b[e] = A.b ? (float)((const W *)A.b)[ch.c] : 0.f;
+            ch.next(A);
+        }
+}
+template <int V> __device__ __forceinline__ void normalise(const Constants<V> &k, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) { const int i = V == 2 ? 0 : e; v[e] = ((v[e] - k.mean[i]) - k.rest[i]) * k.rstd[i]; }
+}
+// item number `item` of the result's launch -> slab, column block and rows
+struct ApplyItem { int64_t n, row, end; int col_block; };
+__device__ __forceinline__ ApplyItem apply_item(const MapPlan &P, int64_t item) {
+    ApplyItem t;
+    const int per = P.col_blocks * P.row_blocks;
+    t.n = item / per;
+    const int left = (int)(item - t.n * per);
+    t.col_block = P.col_blocks == 1 ? 0 : left / P.row_blocks;
+    t.row = (int64_t)(left - t.col_block * P.row_blocks) * P.apply_rows;
+    t.end = t.row + P.apply_rows < P.rows ? t.row + P.apply_rows : P.rows;
+    return t;
+}
+template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_apply(NormArgs A, MapPlan P) {
+    const int64_t width = (int64_t)P.q * A.C, items = A.N * P.col_blocks * P.row_blocks;
+    Draw d = {};
+    if (DROP) d = make_draw(A.rng, A.site, A.cut);
+#pragma unroll 1
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const ApplyItem t = apply_item(P, item);
+        const Column c = my_column(A, P, t.col_block);
+        if (!c.mine) continue;
+        Constants<V> k;
+        load_constants<V>(A, t.n, c.col, k);
+        const T *x = (const T *)A.x + t.n * A.x_stride;
+        T *y = (T *)A.out + t.n * A.size;
+#pragma unroll 1
+        for (int64_t row = t.row + c.r; row < t.end; row += 4 * P.R) {
+            const int64_t off = row * width + 8 * c.col;
+            int valid[4];
+            Chunk<DT> v[4];
+            map_valid<V, 4>(A, P, c, row, t.end, width, valid);
+            map_load<V, 4>(x + off, P.R * width, valid, v);
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                if (!valid[u]) continue;
+                const int64_t at = off + u * P.R * width;
+                float f[8];
+                unpack<DROP>(v[u], DROP ? chunk_mask(d, t.n * A.size + at) : 255u, f);
+                normalise<V>(k, f);
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[e] = f[e] * k.w[e] + k.b[e];
+                activate(f, A.act);
+                row_store<V>(y + at, valid[u], f);
+            }
+        }
+    }
+}
+
+// backward, first launch: per workgroup the channel sums of dz xh and dz (params[workgroup][2][C]), per split their w-weighted group sums (part[n][g][split][column block]
+// = sum w dz, sum w dz xh), in 64 bits.
+template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_sums(NormArgs A, MapPlan P, double2 *part, float *params) {
+    extern __shared__ double2 lds[];
+    const int64_t width = (int64_t)P.q * A.C, items = A.N * P.splits;
+    const Column c = my_column(A, P, blockIdx.y);
+    const int NT = blockDim.x;
+    Draw d = {};
+    if (DROP) d = make_draw(A.rng, A.site, A.cut);
+#pragma unroll 1
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t n = item / P.splits, split = item - n * P.splits;
+        const T *x = (const T *)A.x + n * A.x_stride, *dy = (const T *)A.dy + n * A.dy_stride;
+        double s1[8] = {}, s2[8] = {};
+        Constants<V> k;
+        if (c.mine) {
+            load_constants<V>(A, n, c.col, k);
+            const int64_t end = (split + 1) * P.rows_per < P.rows ? (split + 1) * P.rows_per : P.rows;
+#pragma unroll 1
+            for (int64_t row = split * P.rows_per + c.r; row < end; row += 2 * P.R) {
+                const int64_t off = row * width + 8 * c.col;
+                int valid[2];
+                Chunk<DT> v[2], g[2];
+                map_valid<V, 2>(A, P, c, row, end, width, valid);
+                map_load<V, 2>(x + off, P.R * width, valid, v);
+                map_load<V, 2>(dy + off, P.R * width, valid, g);
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    if (!valid[u]) continue;
+                    const int64_t at = off + u * P.R * width;
+                    const uint32_t m = DROP ? chunk_mask(d, n * A.size + at) : 255u;
+                    float xh[8], dv[8], dz[8];
+                    unpack<DROP>(v[u], m, xh);
+                    unpack<false>(g[u], 255u, dv);
+                    normalise<V>(k, xh);
+                    back_activation<DROP, V>(A, x + at, n, 8 * c.col, valid[u], m, xh, dv, k.w, k.b, dz);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) { s1[e] += (double)dz[e]; s2[e] += (double)(dz[e] * xh[e]); }
+                }
+            }
+        }
+        if (params) {
+            // channel by channel over the workgroup's threads: a few lanes per channel where channels are few
+            __syncthreads();
+            if (c.mine)
+#pragma unroll
+                for (int e = 0; e < 8; e++) lds[e * NT + c.r * P.bcol + c.col - c.first] = double2{s2[e], s1[e]};
+            __syncthreads();
+            float *to = params + blockIdx.x * 2 * (int64_t)A.C;
+            const int from = P.col_blocks == 1 ? 0 : 8 * c.first, last = P.col_blocks == 1 || 8 * (c.first + P.bcol) > A.C ? A.C : 8 * (c.first + P.bcol);
+            const int lane = threadIdx.x & 7;
+#pragma unroll 1
+            for (int c8 = from; c8 < last; c8 += NT >> 3) {
+                const int ch = c8 + (threadIdx.x >> 3);
+                double s = 0.0, q = 0.0;
+                if (ch < last)
+                    for (int i = lane; i < P.q * P.R; i += 8) {
+                        const int r = i / P.q, vc = (i - r * P.q) * A.C + ch;
+                        const double2 v = lds[(vc & 7) * NT + r * P.bcol + (vc >> 3) - c.first];
+                        s += v.x; q += v.y;
+                    }
+                lanes_sum2(s, q, 3);
+                if (ch < last && lane < 2) {
+                    float *word = to + lane * (int64_t)A.C + ch;              // (this thread's own word: later items of the workgroup add to it)
+                    const float v = (float)(lane ? q : s);
+                    *word = item == blockIdx.x ? v : *word + v;
+                }
+            }
+        }
+        if (c.mine)
+#pragma unroll
+            for (int e = 0; e < 8; e++) { s1[e] *= (double)k.w[e]; s2[e] *= (double)k.w[e]; }
+        const int64_t parts = (int64_t)P.splits * P.col_blocks;
+        join_groups<V>(s1, s2, A, P, c, lds, part + n * A.G * parts + split * P.col_blocks + blockIdx.y, parts);
+    }
+}
+// second launch: the first workgroups join the splits of each (n, g) into {mean of w dz, mean of w dz xh}, the others the parameter gradients
+__global__ __launch_bounds__(1024) void k_map_back_join(NormArgs A, int splits, const double2 *part, const float *params, int param_rows, int join_blocks, float2 *means, void *dw, void *db) {
+    __shared__ double lds[64][17];
+    if ((int)blockIdx.x >= join_blocks) { param_columns(A, params, param_rows, blockIdx.x - join_blocks, dw, db, lds); return; }
+    for (int64_t item = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 6); item < A.N * A.G; item += (int64_t)join_blocks * 16) {
+        const double2 t = join_splits(part + item * splits, splits);
+        if ((threadIdx.x & 63) == 0) means[item] = float2{(float)(t.x * A.inv_count), (float)(t.y * A.inv_count)};
+    }
+}
+template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_apply(NormArgs A, MapPlan P, const float2 *means) {
+    const int64_t width = (int64_t)P.q * A.C, items = A.N * P.col_blocks * P.row_blocks;
+    Draw d = {};
+    if (DROP) d = make_draw(A.rng, A.site, A.cut);
+#pragma unroll 1
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const ApplyItem t = apply_item(P, item);
+        const Column c = my_column(A, P, t.col_block);
+        if (!c.mine) continue;
+        Constants<V> k;
+        load_constants<V>(A, t.n, c.col, k);
+        float m1[V == 2 ? 1 : 8], m2[V == 2 ? 1 : 8];
+        {
+            Channel ch(A, 8 * c.col);
+#pragma unroll
+            for (int e = 0; e < (V == 2 ? 1 : 8); e++) { const float2 m = means[t.n * A.G + ch.g]; m1[e] = m.x; m2[e] = m.y; ch.next(A); }
+        }
+        const T *x = (const T *)A.x + t.n * A.x_stride, *dy = (const T *)A.dy + t.n * A.dy_stride;
+        T *dx = (T *)A.out + t.n * A.size;
+#pragma unroll 1
+        for (int64_t row = t.row + c.r; row < t.end; row += 2 * P.R) {
+            const int64_t off = row * width + 8 * c.col;
+            int valid[2];
+            Chunk<DT> v[2], g[2];
+            map_valid<V, 2>(A, P, c, row, t.end, width, valid);
+            map_load<V, 2>(x + off, P.R * width, valid, v);
+            map_load<V, 2>(dy + off, P.R * width, valid, g);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                if (!valid[u]) continue;
+                const int64_t at = off + u * P.R * width;
+                const uint32_t m = DROP ? chunk_mask(d, t.n * A.size + at) : 255u;
+                float xh[8], dv[8], dz[8];
+                unpack<DROP>(v[u], m, xh);
+                unpack<false>(g[u], 255u, dv);
+                normalise<V>(k, xh);
+                back_activation<DROP, V>(A, x + at, t.n, 8 * c.col, valid[u], m, xh, dv, k.w, k.b, dz);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int i = V == 2 ? 0 : e;
+                    const float r = k.rstd[i] * (dz[e] * k.w[e] - m1[i] - xh[e] * m2[i]);
+                    dz[e] = !DROP || m >> e & 1u ? r : 0.f;
+                }
+                row_store<V>(dx + at, valid[u], dz);
+            }
+        }
+    }
+}
+
+// ---- launches
+template <int V, bool DROP> void row_forward_v(const NormArgs &a, const RowLaunch &r, hipStream_t s) {
+    if (r.K == 1) k_row_forward<V, 1, 256, DROP><<<r.grid, 256, 0, s>>>(a, r.P);
+    else if (r.K == 2) k_row_forward<V, 2, 256, DROP><<<r.grid, 256, 0, s>>>(a, r.P);
+    else k_row_forward<V, 4, 256, DROP><<<r.grid, 256, 0, s>>>(a, r.P);
+}
+void row_forward(const NormArgs &a, const RowLaunch &r, hipStream_t s) {
+    if (a.D % 8) a.cut ? row_forward_v<0, true>(a, r, s) : row_forward_v<0, false>(a, r, s);
+    else a.cut ? row_forward_v<1, true>(a, r, s) : row_forward_v<1, false>(a, r, s);
+}
+template <int V, bool DROP> void row_backward_v(const NormArgs &a, const RowLaunch &r, float *part, hipStream_t s) { k_row_backward<V, 512, DROP><<<r.grid, 512, 0, s>>>(a, r.P, part); }
+void row_backward(const NormArgs &a, const RowLaunch &r, float *part, hipStream_t s) {
+    if (a.D % 8) a.cut ? row_backward_v<0, true>(a, r, part, s) : row_backward_v<0, false>(a, r, part, s);
+    else a.cut ? row_backward_v<1, true>(a, r, part, s) : row_backward_v<1, false>(a, r, part, s);
+}
+unsigned column_blocks(const NormArgs &a) { return (unsigned)((2 * (int64_t)a.C + 15) / 16); }
+void params(const NormArgs &a, const float *part, int rows, void *dw, void *db, hipStream_t s) { k_row_params<<<column_blocks(a), 1024, 0, s>>>(a, part, rows, dw, db); }
+
+int variant(const NormArgs &a, const MapLaunch &m) {
+    const int64_t width = (int64_t)m.P.q * a.C;
+    return width % 8 || a.size % width ? 0 : a.C % 8 || a.D % 8 ? 1 : 2;
+}
+template <int V, bool DROP> void map_forward_v(const NormArgs &a, const MapLaunch &m, double2 *part, hipStream_t s) {
+    k_map_sums<V, DROP><<<m.sums, m.NT, (size_t)m.NT * (V == 2 ? 16 : 128), s>>>(a, m.P, part);
+    k_map_stats<DROP><<<m.stat_blocks, 256, 0, s>>>(a, m.P.splits * m.P.col_blocks, part);
+    k_map_apply<V, DROP><<<m.apply_blocks, m.NT, 0, s>>>(a, m.P);
+}
+void map_forward(const NormArgs &a, const MapLaunch &m, double2 *part, hipStream_t s) {
+    switch (variant(a, m)) {
+    case 0: a.cut ? map_forward_v<0, true>(a, m, part, s) : map_forward_v<0, false>(a, m, part, s); break;
+    case 1: a.cut ? map_forward_v<1, true>(a, m, part, s) : map_forward_v<1, false>(a, m, part, s); break;
+    default: a.cut ? map_forward_v<2, true>(a, m, part, s) : map_forward_v<2, false>(a, m, part, s); break;
+    }
+}
+template <int V, bool DROP> void map_backward_v(const NormArgs &a, const MapLaunch &m, double2 *part, float2 *means, float *sums, void *dw, void *db, hipStream_t s) {
+    k_map_back_sums<V, DROP><<<m.sums, m.NT, (size_t)m.NT * 128, s>>>(a, m.P, part, sums);
+    const int64_t items = a.N * a.G;
+    const int join = (int)(items < 16 * 4096 ? (items + 15) / 16 : 4096);
+    k_map_back_join<<<join + (sums ? column_blocks(a) : 0), 1024, 0, s>>>(a, m.P.splits * m.P.col_blocks, part, sums, (int)m.sums.x, join, means, dw, db);
+    k_map_back_apply<V, DROP><<<m.apply_blocks, m.NT, 0, s>>>(a, m.P, means);
+}
+void map_backward(const NormArgs &a, const MapLaunch &m, double2 *part, float2 *means, float *sums, void *dw, void *db, hipStream_t s) {
+    switch (variant(a, m)) {
+    case 0: a.cut ? map_backward_v<0, true>(a, m, part, means, sums, dw, db, s) : map_backward_v<0, false>(a, m, part, means, sums, dw, db, s); break;
+    case 1: a.cut ? map_backward_v<1, true>(a, m, part, means, sums, dw, db, s) : map_backward_v<1, false>(a, m, part, means, sums, dw, db, s); break;
+    default: a.cut ? map_backward_v<2, true>(a, m, part, means, sums, dw, db, s) : map_backward_v<2, false>(a, m, part, means, sums, dw, db, s); break;
+    }
+}
+
+}  // namespace
+
+const NormEntry &REG_ENTRY() {
+    static const NormEntry e = {row_forward, row_backward, map_forward, map_backward, params};
+    return e;
+}

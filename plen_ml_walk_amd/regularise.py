@@ -224,9 +224,14 @@ def dropout(x, p, rng, site=0):
 # ---- group norm with an activation, with dropout before it or without ------------------------------------------------------------------------------
 def _slabs(x):
     """x with the elements of each x[n] contiguous, and the distance of x[n] from x[n + 1]."""
-    if not x[0].is_contiguous():
+    if not x.is_contiguous() and not x[0].is_contiguous():
         x = x.contiguous()
     return x, x.stride(0)
+
+
+def _param(t, x):
+    """A parameter in a type the kernels read beside x's: float32 or x's own."""
+    return t if t is None or t.dtype == torch.float32 or t.dtype == x.dtype else t.float()
 
 
 def _norm_args(x, groups, weight, bias, eps, act, cut, site):
@@ -252,7 +257,7 @@ def _workspace(a, backward, device):
 def _norm_forward(x, groups, weight, bias, eps, act, cut, rng, site, stats=None, used=None):
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if x.numel():
-        x, stride = _slabs(x)
+        (x, stride), weight, bias = _slabs(x), _param(weight, x), _param(bias, x)
         a = _norm_args(x, groups, weight, bias, eps, act, cut, site)
         a.x, a.x_stride, a.out = x.data_ptr(), stride, y.data_ptr()
         a.stats = stats.data_ptr() if stats is not None else None
@@ -279,8 +284,10 @@ class _NormAct(torch.autograd.Function):
         x, weight, bias, stats, used = ctx.saved_tensors
         groups, eps, act, cut, site = ctx.rest
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dw = torch.empty(weight.shape, dtype=weight.dtype, device=x.device) if ctx.needs_input_grad[1] else None
-        db = torch.empty(bias.shape, dtype=bias.dtype, device=x.device) if ctx.needs_input_grad[2] else None
+        types = [t.dtype if t is not None else None for t in (weight, bias)]
+        weight, bias = _param(weight, x), _param(bias, x)
+        dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
+        db = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
         if x.numel():
             (x, xs), (dy, dys) = _slabs(x), _slabs(dy)
             a = _norm_args(x, groups, weight, bias, eps, act, cut, site)
@@ -293,6 +300,7 @@ class _NormAct(torch.autograd.Function):
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
+        dw, db = (t if t is None or t.dtype == dt else t.to(dt) for t, dt in zip((dw, db), types))
         return dx, dw, db, None, None, None, None, None, None
 
 

@@ -28,6 +28,16 @@ def test_library_exports_its_header(lib):
     assert b"gfx950" in lib.plenreg_version()
 
 
+def test_no_kernel_uses_scratch_memory(lib):
+    """The compiler's report of the build: a spilling variant of the wide backward pass has given wrong results on lanes that a divergent branch leaves out."""
+    import json
+    from plen_ml_walk_amd.build import REG_RESOURCES
+    report = json.load(open(REG_RESOURCES))
+    assert len(report) > 30
+    for name, r in report.items():
+        assert r["ScratchSize"] == 0 and r.get("VGPRs Spill", 0) == 0 and r["LDS Size"] <= 65536, (name, r)
+
+
 def test_struct_layouts_match_the_header(tmp_path):
     """Sizes and offsets of the ctypes mirrors against the C compiler's."""
     src = tmp_path / "s.c"
