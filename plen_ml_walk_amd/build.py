@@ -115,6 +115,30 @@ def build_regularise(force=False, flags=(), out=None):
     return out or REG_OUT
 
 
+REG_TORCH_SRC = os.path.join(CSRC, "regularise_torch.cpp")
+REG_TORCH_OUT = os.path.join(CSRC, "plenreg_torch.so")
+
+
+def build_regularise_nodes(force=False):
+    """Compile regularise_torch.cpp -> csrc/plenreg_torch.so (host code): the autograd nodes of regularise.py around libplenreg.so's C ABI."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    deps = [REG_TORCH_SRC, os.path.join(os.path.dirname(_HERE), "include", "plenreg.h")]
+    if not force and os.path.exists(REG_TORCH_OUT) and all(os.path.getmtime(REG_TORCH_OUT) >= os.path.getmtime(d) for d in deps):
+        return REG_TORCH_OUT
+    rocm = os.path.dirname(os.path.dirname(hipcc_path()))
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=plenreg_torch", "-DUSE_ROCM=1", "-D__HIP_PLATFORM_AMD__=1",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+    for inc in cpp_extension.include_paths() + [os.path.join(rocm, "include"), sysconfig.get_paths()["include"]]:
+        cmd += ["-isystem", inc]
+    cmd += [REG_TORCH_SRC, "-o", REG_TORCH_OUT]
+    for lib in cpp_extension.library_paths():
+        cmd += ["-L" + lib, "-Wl,-rpath," + lib]
+    subprocess.check_call(cmd + ["-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python"], cwd=CSRC)
+    return REG_TORCH_OUT
+
+
 # The A/B partner of the shipped env library (csrc/variants/nospec.so; tests/test_env_gpu.py holds the two to bitwise equality): every round-4/5 restructuring switched off --
 # run-time point tests instead of the count-specialised solver loops (with their hoisted commits), the Delassus matrix as vector multiply-adds from broadcast LDS reads instead of
 # matrix-core tiles.  (Not the mass matrix: -DPLENVEC_MFMA_MASS=0 changes how the compiler contracts the rest of that phase -- even the bias force, which the switch does not

@@ -383,3 +383,27 @@ def test_saved_inputs_are_watched():
     x.add_(1)
     with pytest.raises(RuntimeError):
         y.sum().backward()
+
+
+def test_a_second_derivative_is_refused():
+    x, dy, w, b = _case((8, 64), 2, torch.float32)
+    for y in (R.group_norm_act(x, 2, w, b), R.dropout(x, 0.3, _rng())):
+        (dx,) = torch.autograd.grad(y, x, dy, create_graph=True)
+        with pytest.raises(RuntimeError):
+            dx.sum().backward()
+
+
+def test_gradients_reach_only_what_asks_for_them():
+    x, dy, w, b = _case((40, 64), 2, torch.float32)
+    full = torch.autograd.grad(R.group_norm_act(x, 2, w, b), (x, w, b), dy)
+    fixed = [t.detach() for t in (x, w, b)]
+    for k, leaf in enumerate((x, w, b)):
+        args = [leaf if i == k else fixed[i] for i in range(3)]
+        (got,) = torch.autograd.grad(R.group_norm_act(args[0], 2, args[1], args[2]), leaf, dy)
+        assert torch.equal(got, full[k])
+    # the same tensor as weight and bias: its gradient is the sum of both
+    both = w.detach().clone().requires_grad_()
+    (got,) = torch.autograd.grad(R.group_norm_act(x, 2, both, both, act="none"), both, dy)
+    dx, dw, db = torch.autograd.grad(R.group_norm_act(x, 2, w, w.detach(), act="none"), (x, w), dy) + torch.autograd.grad(
+        R.group_norm_act(x, 2, w.detach(), w, act="none"), w, dy)
+    assert torch.equal(got, dw + db)
