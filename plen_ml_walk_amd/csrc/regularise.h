@@ -23,37 +23,59 @@ template <int DT> static __device__ __forceinline__ Chunk<DT> load_whole(const t
     __builtin_memcpy(&c, p, sizeof c);
     return c;
 }
-// the first `valid` elements (the rest: zeros).  A part of a chunk goes as four, two and one elements.
-template <int DT> static __device__ __forceinline__ Chunk<DT> load_chunk(const typename Elem<DT>::T *p, int valid) {
-    typedef typename Elem<DT>::T T;
-    if (valid >= 8) return load_whole<DT>(p);
-    T four[4] = {}, two[2] = {}, one = (T)0.f;
-    if (valid & 4) __builtin_memcpy(four, p, sizeof four);
-    if (valid & 2) __builtin_memcpy(two, p + (valid & 4), sizeof two);
-    if (valid & 1) one = p[valid & 6];
-    const T rest[4] = {valid & 2 ? two[0] : one, two[1], valid & 2 ? one : (T)0.f, (T)0.f};
-    Chunk<DT> c;
-#pragma unroll
-    for (int e = 0; e < 4; e++) { c.v[e] = valid & 4 ? four[e] : rest[e]; c.v[4 + e] = valid & 4 ? rest[e] : (T)0.f; }
-    return c;
-}
 template <int DT> static __device__ __forceinline__ void store_whole(typename Elem<DT>::T *p, const float (&v)[8]) {
     Chunk<DT> c;
 #pragma unroll
     for (int e = 0; e < 8; e++) c.v[e] = (typename Elem<DT>::T)v[e];
     __builtin_memcpy(p, &c, sizeof c);
 }
+// Part of a chunk goes as four, two and one elements.  Quad: four elements in one register value (an array here would be put into memory).
+template <int SIZE> struct Quad;
+template <> struct Quad<2> {
+    typedef uint64_t Four; typedef uint32_t Two; typedef uint16_t One;
+    static __device__ __forceinline__ Four join(Two two, One one, bool has_two) { return has_two ? (Four)two | (Four)one << 32 : (Four)one; }
+    static __device__ __forceinline__ Two first(Four q) { return (Two)q; }
+    static __device__ __forceinline__ One single(Four q, bool after_two) { return (One)(after_two ? q >> 32 : q); }
+};
+template <> struct Quad<4> {
+    typedef uint32_t Four __attribute__((ext_vector_type(4)));
+    typedef uint32_t Two __attribute__((ext_vector_type(2)));
+    typedef uint32_t One;
+    static __device__ __forceinline__ Four join(Two two, One one, bool has_two) { return has_two ? Four{two.x, two.y, one, 0u} : Four{one, 0u, 0u, 0u}; }
+    static __device__ __forceinline__ Two first(Four q) { return q.xy; }
+    static __device__ __forceinline__ One single(Four q, bool after_two) { return after_two ? q.z : q.x; }
+};
+// the first `valid` elements (the rest: zeros)
+template <int DT> static __device__ __forceinline__ Chunk<DT> load_chunk(const typename Elem<DT>::T *p, int valid) {
+    typedef Quad<sizeof(typename Elem<DT>::T)> Q;
+    if (valid >= 8) return load_whole<DT>(p);
+    typename Q::Four four = {};
+    typename Q::Two two = {};
+    typename Q::One one = 0;
+    if (valid & 4) __builtin_memcpy(&four, p, sizeof four);
+    if (valid & 2) __builtin_memcpy(&two, p + (valid & 4), sizeof two);
+    if (valid & 1) __builtin_memcpy(&one, p + (valid & 6), sizeof one);
+    const typename Q::Four rest = Q::join(two, one, valid & 2);
+    struct { typename Q::Four lo, hi; } both = {valid & 4 ? four : rest, valid & 4 ? rest : (typename Q::Four){}};
+    Chunk<DT> c;
+    __builtin_memcpy(&c, &both, sizeof c);
+    return c;
+}
 template <int DT> static __device__ __forceinline__ void store_chunk(typename Elem<DT>::T *p, int valid, const float (&v)[8]) {
     typedef typename Elem<DT>::T T;
+    typedef Quad<sizeof(T)> Q;
     if (valid >= 8) { store_whole<DT>(p, v); return; }
-    T c[8], rest[3];
+    Chunk<DT> c;
 #pragma unroll
-    for (int e = 0; e < 8; e++) c[e] = (T)v[e];
-    if (valid & 4) __builtin_memcpy(p, c, 4 * sizeof(T));
-#pragma unroll
-    for (int e = 0; e < 3; e++) rest[e] = valid & 4 ? c[4 + e] : c[e];
-    if (valid & 2) __builtin_memcpy(p + (valid & 4), rest, 2 * sizeof(T));
-    if (valid & 1) p[valid & 6] = valid & 2 ? rest[2] : rest[0];
+    for (int e = 0; e < 8; e++) c.v[e] = (T)v[e];
+    struct { typename Q::Four lo, hi; } both;
+    __builtin_memcpy(&both, &c, sizeof c);
+    if (valid & 4) __builtin_memcpy(p, &both.lo, sizeof both.lo);
+    const typename Q::Four rest = valid & 4 ? both.hi : both.lo;
+    const typename Q::Two two = Q::first(rest);
+    const typename Q::One one = Q::single(rest, valid & 2);
+    if (valid & 2) __builtin_memcpy(p + (valid & 4), &two, sizeof two);
+    if (valid & 1) __builtin_memcpy(p + (valid & 6), &one, sizeof one);
 }
 
 // ---- the mask (plenreg.h): 16 bits of the stream per element, so one generator call serves a chunk.  Ten rounds of two 32 x 32 -> 64-bit products
@@ -101,9 +123,10 @@ static __device__ __forceinline__ int small_quotient(int i, float inv_n) { retur
 // rows of one position: 2^team_log lanes per (row, group); a workgroup covers gb neighbouring groups of rb rows per turn
 struct RowPlan { int team_log, gb, rb, trips; float inv_gb; };
 struct RowLaunch { RowPlan P; int K, NT; dim3 grid; };
-// many positions.  A slab as `rows` rows of `ncol` chunk columns (q positions to a row); bcol columns in a workgroup, R rows per turn of it
-struct MapPlan { int q, ncol, bcol, col_blocks, R, splits; int64_t rows, rows_per; int lanes_log, row_blocks; int64_t apply_rows; float inv_bcol; };
-struct MapLaunch { MapPlan P; dim3 sums; int NT; unsigned stat_blocks, apply_blocks; size_t lds; };
+// many positions.  A slab as `rows` rows of `ncol` chunk columns (2^q_log positions to a row); bcol columns in a workgroup, R rows per turn of it; rows_per rows in a
+// workgroup of the sums, apply_rows in one of the result; 2^lanes_log lanes join one group
+struct MapPlan { int q_log, ncol, bcol, col_blocks, R, splits, lanes_log; int64_t rows, rows_per, apply_rows; float inv_bcol; };
+struct MapLaunch { MapPlan P; dim3 sums, apply; int NT, param_rows; unsigned stat_blocks; };
 
 // one per pair of element types (x and results, parameters), in regularise_norm.hip
 struct NormEntry {

@@ -3,6 +3,13 @@
 #include "regularise.h"
 
 #define DROPOUT_SMALL (1 << 18)
+#ifndef MAP_BLOCKS
+#define MAP_BLOCKS 512
+#endif
+#ifndef MAP_APPLY_BLOCKS
+#define MAP_APPLY_BLOCKS 512
+#endif
+#define MAP_MAX_SPAN ((int64_t)1 << 28)      // elements of a slab that one workgroup walks over
 #define ROW_MAX_FORWARD 8192            // widest group that the lanes of one workgroup hold: 256 lanes of 4 chunks, or in the backward pass (which holds four times as much) 512 of one
 #define ROW_MAX_BACKWARD 4096
 
@@ -93,7 +100,7 @@ static RowLaunch row_plan(const PlenRegNorm &a, bool backward) {
     r.P.rb = teams / r.P.gb;
     const int64_t gy = div_up(a.G, r.P.gb), need = div_up(a.N, r.P.rb);
     // as many workgroups as are resident at a time, each over several rows; in the backward pass at most 256 rows per lane (its 32-bit sums)
-    int64_t gx = div_up(backward ? 512 : 2048, gy);
+    int64_t gx = div_up(backward ? 512 : r.K == 4 ? 512 : 1024, gy);
     if (backward && gx < div_up(need, 256)) gx = div_up(need, 256);
     if (gx > need) gx = need;
     r.P.trips = (int)div_up(need, gx);
@@ -113,33 +120,35 @@ static int fill_threads(int ncol, int lo, int hi) {
 static MapLaunch map_plan(const PlenRegNorm &a) {
     MapLaunch m;
     const int D = a.C / a.G;
-    int q = 1;
-    while (q < 8 && (int64_t)q * a.C % 8) q *= 2;
-    if ((int64_t)q * a.C / 8 > 512 || q > a.L) q = 1;
-    m.P.q = q;
-    m.P.ncol = (int)div_up((int64_t)q * a.C, 8);
-    m.P.rows = div_up(a.L, q);
+    const int64_t size = a.L * a.C;
+    m.P.q_log = 0;
+    while (((int64_t)a.C << m.P.q_log) % 8) m.P.q_log++;
+    const int64_t columns = ((int64_t)a.C << m.P.q_log) / 8, chunks = div_up(size, 8);
+    m.P.ncol = (int)(columns < chunks ? columns : chunks);
+    m.P.rows = div_up(a.L, (int64_t)1 << m.P.q_log);
     m.P.col_blocks = (int)div_up(m.P.ncol, 512);
     m.P.bcol = (int)div_up(m.P.ncol, m.P.col_blocks);
     m.P.inv_bcol = 1.f / (float)m.P.bcol;
     m.NT = fill_threads(m.P.bcol, 256, 512);
     m.P.R = m.NT / m.P.bcol;
-    // ~4 workgroups per compute unit, at least 4 rows per thread
-    const int64_t turns = div_up(m.P.rows, (int64_t)m.P.R * 4), wanted = div_up(1024, m.P.col_blocks);
-    int64_t splits = a.N >= wanted ? 1 : div_up(wanted, a.N);
-    if (splits > turns) splits = turns;
-    m.P.rows_per = div_up(m.P.rows, splits);
+    // ~2 workgroups per compute unit, each thread in whole turns of 2 rows
+    const int64_t turn = (int64_t)m.P.R * 2, turns = div_up(m.P.rows, turn), groups = a.N * m.P.col_blocks;
+    const int64_t most = MAP_MAX_SPAN / (turn * ((int64_t)a.C << m.P.q_log));              // turns of a workgroup, so that its offsets fit
+    const int64_t sum_turns = div_up(turns, groups >= MAP_BLOCKS ? 1 : div_up(MAP_BLOCKS, groups)), apply_turns = div_up(turns, groups >= MAP_APPLY_BLOCKS ? 1 : div_up(MAP_APPLY_BLOCKS, groups));
+    m.P.rows_per = (sum_turns < most ? sum_turns : most) * turn;
     m.P.splits = (int)div_up(m.P.rows, m.P.rows_per);
-    m.P.lanes_log = log2_up(div_up((int64_t)m.P.R * q * (a.C % 8 || D % 8 ? D : D / 8), 4));
+    m.P.apply_rows = (apply_turns < most ? apply_turns : most) * turn;
+    const int64_t row_blocks = div_up(m.P.rows, m.P.apply_rows);
+    // about four entries of a group for each lane that joins it
+    m.P.lanes_log = log2_up(div_up((int64_t)m.P.R * (a.C % 8 || D % 8 ? D : D / 8), 4));
     if (m.P.lanes_log > 6) m.P.lanes_log = 6;
-    m.sums = dim3((unsigned)(a.N * m.P.splits < 2048 ? a.N * m.P.splits : 2048), (unsigned)m.P.col_blocks);
+    // slabs beyond what fills the chip (and the grid's limit of 65535) are walked by the workgroups
+    int64_t z = div_up(2048, m.P.splits);
+    m.sums = dim3((unsigned)m.P.splits, (unsigned)m.P.col_blocks, (unsigned)(a.N < z ? a.N : z));
+    m.param_rows = (int)(m.sums.x * (m.P.q_log ? m.sums.y : 1) * m.sums.z);
+    z = div_up(8192, row_blocks);
+    m.apply = dim3((unsigned)row_blocks, (unsigned)m.P.col_blocks, (unsigned)(a.N < z ? a.N : z));
     m.stat_blocks = (unsigned)(a.N * a.G < 4 * 65536 ? div_up(a.N * a.G, 4) : 65536);
-    int64_t blocks = div_up(2048, a.N * m.P.col_blocks);
-    if (blocks > turns) blocks = turns;
-    m.P.apply_rows = div_up(m.P.rows, blocks);
-    m.P.row_blocks = (int)div_up(m.P.rows, m.P.apply_rows);
-    const int64_t items = a.N * m.P.col_blocks * m.P.row_blocks;
-    m.apply_blocks = (unsigned)(items < 65536 ? items : 65536);
     return m;
 }
 // bytes of the partial pairs of a map launch
@@ -186,7 +195,7 @@ int64_t plenreg_norm_workspace(const PlenRegNorm *a, int backward) {
     if (bad_norm(a)) return PLENREG_REFUSE;
     if (by_rows(*a, backward)) return backward ? (int64_t)row_plan(*a, true).grid.x * 2 * a->C * 4 : 0;
     const MapLaunch m = map_plan(*a);
-    return part_bytes(*a, m) + (backward ? a->N * a->G * 8 + (int64_t)m.sums.x * 2 * a->C * 4 : a->N * a->G * 16);
+    return part_bytes(*a, m) + (backward ? a->N * a->G * 8 + (int64_t)m.param_rows * 2 * a->C * 4 : a->N * a->G * 16);
 }
 
 int plenreg_norm_forward(const PlenRegNorm *a, void *stream) {

@@ -16,7 +16,7 @@
 #define WT REG_WT
 typedef Elem<DT>::T T;
 typedef Elem<WT>::T W;
-// variants: 0 = chunks may be partial, 1 = all chunks are whole, 2 = and belong to one group each
+// variants V: rows 0 = groups that end within a chunk, 1 = whole chunks; slabs 1 = chunks that span groups, 2 = one group each
 namespace {
 
 __device__ __forceinline__ float logistic(float z) {
@@ -47,12 +47,37 @@ __device__ __forceinline__ double2 finish_stats(const NormArgs &A, double s, dou
     return double2{s + m, A.scale * inverse_sqrt(fma(var, A.scale * A.scale, A.eps))};
 }
 __device__ __forceinline__ void write_used(const NormArgs &A) {
-    if (A.used && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) { A.used[0] = A.rng[0]; A.used[1] = A.rng[1]; }
+    if (A.used && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) { A.used[0] = A.rng[0]; A.used[1] = A.rng[1]; }
 }
 // a chunk's elements as floats; masked ones as zeros
 template <bool DROP, int E> __device__ __forceinline__ void unpack(const Chunk<E> &c, uint32_t kept_bits, float (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; e++) v[e] = !DROP || kept_bits >> e & 1u ? (float)c.v[e] : 0.f;
+}
+
+// ---- loads without branches.  A load under a condition waits for the ones before it, so every lane loads whole chunks from inside its row or slab of `size` elements, and
+//      what is not asked for is left out of the sums and not stored.  V = 0: the last chunk of a row may begin less than 8 elements before its end: then the 8 last elements are
+//      loaded and moved down.
+template <int V, int E> __device__ __forceinline__ Chunk<E> load_inside(const typename Elem<E>::T *p, int64_t off, int64_t size) {
+    if (V) return load_whole<E>(p + off);
+    if (size < 8) return load_chunk<E>(p + off, (int)(size - off));
+    return load_whole<E>(p + (off < size - 8 ? off : size - 8));
+}
+template <int V> __device__ __forceinline__ void move_down(float (&v)[8], int64_t off, int64_t size) {
+    if (V || size < 8 || off <= size - 8) return;
+    const int by = (int)(off - (size - 8));
+    if (by & 4) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = v[e + 4];
+    }
+    if (by & 2) {
+#pragma unroll
+        for (int e = 0; e < 6; e++) v[e] = v[e + 2];
+    }
+    if (by & 1) {
+#pragma unroll
+        for (int e = 0; e < 7; e++) v[e] = v[e + 1];
+    }
 }
 
 // ---- sums over 2^log neighbouring lanes, left in each of them: exchanges within 16 lanes by DPP, beyond by the row swaps
@@ -102,9 +127,9 @@ template <int NT, typename F> __device__ __forceinline__ void team_sum2(F &a, F 
     }
 }
 
-// ---- the pass back through the activation for one chunk: xh and dy -> dz (zeros beyond `valid`).  ReLU's gate: where 32 bits leave the sign of z open it is decided in
+// ---- the pass back through the activation for one chunk of `valid` elements: xh and dy -> dz.  ReLU's gate: where 32 bits leave the sign of z open it is decided in
 // 64, from the inputs in memory (x of the chunk at px, statistics and parameters of channel (c0 + e) % C): the gradient jumps there.  xh is off by at most 4 roundings.
-template <bool DROP, int V> __device__ __forceinline__ void back_activation(const NormArgs &A, const T *px, int64_t n, int c0, int valid, uint32_t kept_bits, const float (&xh)[8], const float (&dy)[8],
+template <bool DROP> __device__ __forceinline__ void back_activation(const NormArgs &A, const T *px, int64_t n, int c0, int valid, uint32_t kept_bits, const float (&xh)[8], const float (&dy)[8],
                                                                              const float (&w)[8], const float (&b)[8], float (&dz)[8]) {
     if (A.act == PLENREG_ACT_RELU) {
         uint32_t open = 0, doubt = 0;
@@ -114,7 +139,7 @@ template <bool DROP, int V> __device__ __forceinline__ void back_activation(cons
             open |= z > 0.f ? 1u << e : 0u;
             doubt |= fabsf(z) <= 6e-7f * (fabsf(t) + fabsf(b[e])) ? 1u << e : 0u;
         }
-        if (V == 0) doubt &= (1u << valid) - 1u;
+        doubt &= (1u << valid) - 1u;
 #pragma unroll 1
         while (doubt) {
             const int e = __ffs(doubt) - 1, c = (c0 + e) % A.C;
@@ -135,10 +160,6 @@ template <bool DROP, int V> __device__ __forceinline__ void back_activation(cons
 #pragma unroll
         for (int e = 0; e < 8; e++) dz[e] = dy[e];
     }
-    if (V == 0) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) dz[e] = e < valid ? dz[e] : 0.f;
-    }
 }
 
 // ---- rows of one position (L = 1): a team of lanes per (row, group), K chunks per lane held in registers, one pass.  Teams of one wave join their sums by lane exchange,
@@ -155,28 +176,27 @@ template <int NT> __device__ __forceinline__ RowPlace row_place(const NormArgs &
     p.mine = p.row < P.rb && p.g < A.G;
     return p;
 }
-template <int K> __device__ __forceinline__ void row_valid(const NormArgs &A, const RowPlan &P, const RowPlace &p, int (&valid)[K]) {
+// first channel of chunk k of a lane within the row, and how much of the chunk belongs to the lane's group; lanes with nothing to do look at the last chunk of the last group
+template <int K> __device__ __forceinline__ void row_chunks(const NormArgs &A, const RowPlan &P, const RowPlace &p, int (&c)[K], int (&valid)[K]) {
+    const int g = p.g < A.G ? p.g : A.G - 1;
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        const int left = A.D - 8 * (p.lane + (k << P.team_log));
+        const int at = 8 * (p.lane + (k << P.team_log)), left = A.D - at;
         valid[k] = !p.mine || left < 0 ? 0 : left > 8 ? 8 : left;
+        c[k] = g * A.D + (left > 0 ? at : (A.D - 1) & ~7);
     }
-}
-template <int V, int E> __device__ __forceinline__ Chunk<E> row_load(const typename Elem<E>::T *p, int valid) {
-    Chunk<E> c = {};
-    if (valid) c = V ? load_whole<E>(p) : load_chunk<E>(p, valid);
-    return c;
 }
 template <int V> __device__ __forceinline__ void row_store(T *p, int valid, const float (&v)[8]) {
     if (V) store_whole<DT>(p, v);
     else store_chunk<DT>(p, valid, v);
 }
 // parameters of a lane's chunk, 1 / 0 where there are none
-template <int V> __device__ __forceinline__ void row_params(const void *p, int c0, int valid, float otherwise, float (&out)[8]) {
+template <int V> __device__ __forceinline__ void row_params(const NormArgs &A, const void *p, int c0, float otherwise, float (&out)[8]) {
     if (p) {
-        const Chunk<WT> c = row_load<V, WT>((const W *)p + c0, valid);
+        const Chunk<WT> c = load_inside<V, WT>((const W *)p, c0, A.C);
 #pragma unroll
         for (int e = 0; e < 8; e++) out[e] = (float)c.v[e];
+        move_down<V>(out, c0, A.C);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; e++) out[e] = otherwise;
@@ -186,16 +206,16 @@ template <int V> __device__ __forceinline__ void row_params(const void *p, int c
 template <int V, int K, int NT, bool DROP> __global__ __launch_bounds__(NT) void k_row_forward(NormArgs A, RowPlan P) {
     __shared__ double2 lds[2][NT / 64];
     const RowPlace p = row_place<NT>(A, P);
-    const int step = 8 << P.team_log, c0 = p.g * A.D + 8 * p.lane;
-    int valid[K];
-    row_valid<K>(A, P, p, valid);
+    int c[K], valid[K];
+    row_chunks<K>(A, P, p, c, valid);
     int64_t n = (int64_t)blockIdx.x * P.rb + p.row;
+    const T *px = (const T *)A.x + (n < A.N ? n : A.N - 1) * A.x_stride;
     Chunk<DT> x[K];
 #pragma unroll
-    for (int k = 0; k < K; k++) x[k] = row_load<V, DT>((const T *)A.x + n * A.x_stride + c0 + k * step, n < A.N ? valid[k] : 0);
+    for (int k = 0; k < K; k++) x[k] = load_inside<V, DT>(px, c[k], A.C);
     float w[K][8], b[K][8];
 #pragma unroll
-    for (int k = 0; k < K; k++) { row_params<V>(A.w, c0 + k * step, valid[k], 1.f, w[k]); row_params<V>(A.b, c0 + k * step, valid[k], 0.f, b[k]); }
+    for (int k = 0; k < K; k++) { row_params<V>(A, A.w, c[k], 1.f, w[k]); row_params<V>(A, A.b, c[k], 0.f, b[k]); }
     Draw d = {};
     if (DROP) { d = make_draw(A.rng, A.site, A.cut); write_used(A); }
 #pragma unroll 1
@@ -205,15 +225,26 @@ template <int V, int K, int NT, bool DROP> __global__ __launch_bounds__(NT) void
         float v[K][8];
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            unpack<DROP>(x[k], DROP && on && valid[k] ? chunk_mask(d, n * A.C + c0 + k * step) : 255u, v[k]);
-            x[k] = row_load<V, DT>((const T *)A.x + next * A.x_stride + c0 + k * step, turn + 1 < P.trips && next < A.N ? valid[k] : 0);      // the next row's, while this one is worked on
+            unpack<false>(x[k], 255u, v[k]);
+            move_down<V>(v[k], c[k], A.C);
+            if (DROP) {
+                const uint32_t m = chunk_mask(d, n * A.C + c[k]);
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[k][e] = m >> e & 1u ? v[k][e] : 0.f;
+            }
+        }
+        if (turn + 1 < P.trips) {                               // the next row's, while this one is worked on
+            px = (const T *)A.x + (next < A.N ? next : A.N - 1) * A.x_stride;
+#pragma unroll
+            for (int k = 0; k < K; k++) x[k] = load_inside<V, DT>(px, c[k], A.C);
         }
         // s: the group's first element, after the mask
         float first;
         if (P.team_log <= 6) first = __shfl(v[0][0], (threadIdx.x & 63) >> P.team_log << P.team_log);
         else {
-            first = on ? (float)((const T *)A.x)[n * A.x_stride + p.g * A.D] : 0.f;
-            if (DROP && on && !kept(d, n * A.C + p.g * A.D)) first = 0.f;
+            const int64_t row = n < A.N ? n : A.N - 1;
+            first = (float)((const T *)A.x)[row * A.x_stride + c[0] - 8 * p.lane];
+            if (DROP && !kept(d, row * A.C + c[0] - 8 * p.lane)) first = 0.f;
         }
         const double shift = (double)first;
         double s = 0.0, q = 0.0;
@@ -237,7 +268,7 @@ template <int V, int K, int NT, bool DROP> __global__ __launch_bounds__(NT) void
 #pragma unroll
                 for (int e = 0; e < 8; e++) v[k][e] = ((v[k][e] - mean) - rest) * rstd * w[k][e] + b[k][e];
                 activate(v[k], A.act);
-                row_store<V>((T *)A.out + n * A.C + c0 + k * step, valid[k], v[k]);
+                row_store<V>((T *)A.out + n * A.C + c[k], valid[k], v[k]);
             }
         }
         n = next;
@@ -249,33 +280,39 @@ template <int V, int NT, bool DROP> __global__ __launch_bounds__(NT) void k_row_
     __shared__ double2 lds[2][NT / 64];
     __shared__ float joined[NT * 8];
     const RowPlace p = row_place<NT>(A, P);
-    const int c0 = p.g * A.D + 8 * p.lane;
-    int valid[1];
-    row_valid<1>(A, P, p, valid);
-    int64_t n = (int64_t)blockIdx.x * P.rb + p.row;
+    int c[1], valid[1];
+    row_chunks<1>(A, P, p, c, valid);
+    const int c0 = c[0], g0 = p.g < A.G ? p.g : A.G - 1;
+    int64_t n = (int64_t)blockIdx.x * P.rb + p.row, row = n < A.N ? n : A.N - 1;
+    const T *px = (const T *)A.x + row * A.x_stride;
+    Chunk<DT> x = load_inside<V, DT>(px, c0, A.C), g = load_inside<V, DT>((const T *)A.dy + row * A.dy_stride, c0, A.C);
+    double2 st = A.stats[row * A.G + g0];
     float w[8], b[8], dw[8] = {}, db[8] = {};
-    row_params<V>(A.w, c0, valid[0], 1.f, w);
-    row_params<V>(A.b, c0, valid[0], 0.f, b);
+    row_params<V>(A, A.w, c0, 1.f, w);
+    row_params<V>(A, A.b, c0, 0.f, b);
     Draw d = {};
     if (DROP) d = make_draw(A.rng, A.site, A.cut);
 #pragma unroll 1
-    for (int turn = 0; turn < P.trips; turn++, n += (int64_t)gridDim.x * P.rb) {
-        const bool on = p.mine && n < A.N && valid[0];
-        const T *px = (const T *)A.x + n * A.x_stride + c0;
+    for (int turn = 0; turn < P.trips; turn++) {
+        const bool on = n < A.N && valid[0];
         float xh[8] = {}, gw[8] = {}, s = 0.f, q = 0.f, rstd = 0.f;
         uint32_t m = 255u;
         if (on) {
-            const Chunk<DT> x = row_load<V, DT>(px, valid[0]), g = row_load<V, DT>((const T *)A.dy + n * A.dy_stride + c0, valid[0]);
-            const double2 st = A.stats[n * A.G + p.g];
             if (DROP) m = chunk_mask(d, n * A.C + c0);
             const float mean = (float)st.x, rest = (float)(st.x - (double)mean);
             rstd = (float)st.y;
             float dy[8], dz[8];
-            unpack<DROP>(x, m, xh);
+            unpack<false>(x, 255u, xh);
             unpack<false>(g, 255u, dy);
+            move_down<V>(xh, c0, A.C);
+            move_down<V>(dy, c0, A.C);
 #pragma unroll
-            for (int e = 0; e < 8; e++) xh[e] = ((xh[e] - mean) - rest) * rstd;
-            back_activation<DROP, V>(A, px, n, c0, valid[0], m, xh, dy, w, b, dz);
+            for (int e = 0; e < 8; e++) xh[e] = (((!DROP || m >> e & 1u ? xh[e] : 0.f) - mean) - rest) * rstd;
+            back_activation<DROP>(A, px + c0, n, c0, valid[0], m, xh, dy, w, b, dz);
+            if (!V) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) dz[e] = e < valid[0] ? dz[e] : 0.f;
+            }
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 gw[e] = dz[e] * w[e];
@@ -292,6 +329,13 @@ template <int V, int NT, bool DROP> __global__ __launch_bounds__(NT) void k_row_
                 gw[e] = !DROP || m >> e & 1u ? t : 0.f;
             }
             row_store<V>((T *)A.out + n * A.C + c0, valid[0], gw);
+        }
+        n += (int64_t)gridDim.x * P.rb;
+        if (turn + 1 < P.trips) {
+            row = n < A.N ? n : A.N - 1;
+            px = (const T *)A.x + row * A.x_stride;
+            x = load_inside<V, DT>(px, c0, A.C); g = load_inside<V, DT>((const T *)A.dy + row * A.dy_stride, c0, A.C);
+            st = A.stats[row * A.G + g0];
         }
     }
     if (!part) return;
@@ -348,35 +392,35 @@ __global__ __launch_bounds__(1024) void k_row_params(NormArgs A, const float *pa
     param_columns(A, part, rows, blockIdx.x, dw, db, lds);
 }
 
-// ---- many positions (or rows too wide for a workgroup's lanes): a slab is L C contiguous elements, seen as rows of q C (q = the smallest number of positions that fill
-//      whole chunks, so that odd channel counts load whole chunks too; 1 where that would be too wide).  A thread owns one chunk column (8 fixed virtual channels v,
-//      channel v % C) and walks down the rows; workgroups split the rows and, where they are wide, the columns.  Statistics, their join, and the result are launches of their
-//      own: the second reading of x comes out of the caches while it fits.
-struct Column { int first, col, r, tail; bool mine; };
-__device__ __forceinline__ Column my_column(const NormArgs &A, const MapPlan &P, int col_block) {
+// ---- many positions (or rows too wide for a workgroup's lanes): a slab is size = L C contiguous elements, seen as rows of q C (q = the smallest number of positions that
+//      fill whole chunks, so that odd channel counts load whole chunks too; the last row may be cut short, and of its last chunk there may be a part).  A thread owns one
+//      chunk column (8 fixed virtual channels v, channel v % C) and walks down the rows; workgroups split the rows and, where they are wide, the columns.  Statistics, their
+//      join, and the result are launches of their own: the second reading of x comes out of the caches while it fits.
+struct Column { int first, col, r; bool mine; };
+__device__ __forceinline__ Column my_column(const MapPlan &P, int col_block) {
     Column c;
     c.first = col_block * P.bcol;
     c.r = small_quotient(threadIdx.x, P.inv_bcol);
     c.col = c.first + (int)threadIdx.x - c.r * P.bcol;
     c.mine = c.r < P.R && c.col < P.ncol;
-    const int left = P.q * A.C - 8 * c.col;
-    c.tail = left > 8 ? 8 : left;
     return c;
 }
-// U chunks at rows row, row + R, ...: how much of each there is, and its elements.  V > 0: whole or beyond the end.
-template <int V, int U> __device__ __forceinline__ void map_valid(const NormArgs &A, const MapPlan &P, const Column &c, int64_t row, int64_t end, int64_t width, int (&valid)[U]) {
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int64_t at = row + u * P.R, left = A.size - (at * width + 8 * c.col);
-        valid[u] = at >= end ? 0 : V ? 8 : left < c.tail ? (int)left : c.tail;
-        if (!V && valid[u] < 0) valid[u] = 0;
-    }
+// a workgroup's rows of slab n: `base` elements into it, `lim` elements; a thread takes the chunks at off, off + step, ... that are whole, and if it then stands at off < lim,
+// the slab's last, partial chunk.  (Spans are below 2^28 elements: offsets in 32 bits, what is the same for the workgroup in scalar registers.)
+struct Span { int64_t base; int lim, off, step; };
+__device__ __forceinline__ Span my_span(const NormArgs &A, const MapPlan &P, const Column &c, int64_t rows_per) {
+    Span t;
+    const int width = A.C << P.q_log;
+    t.base = blockIdx.x * rows_per * width;
+    const int64_t left = A.size - t.base;
+    t.lim = left < rows_per * width ? (int)left : (int)(rows_per * width);
+    t.step = P.R * width;
+    t.off = c.r * width + 8 * c.col;
+    return t;
 }
-template <int V, int U> __device__ __forceinline__ void map_load(const T *p, int64_t step, const int (&valid)[U], Chunk<DT> (&v)[U]) {
-#pragma unroll
-    for (int u = 0; u < U; u++)
-        if (valid[u]) v[u] = V ? load_whole<DT>(p + u * step) : load_chunk<DT>(p + u * step, valid[u]);
-}
+// the chunk at off, or the span's last whole one (a load under a condition would wait for the ones before it); lim >= 8
+__device__ __forceinline__ Chunk<DT> span_load(const T *p, const Span &t, int off) { return load_whole<DT>(p + (off < t.lim - 8 ? off : t.lim - 8)); }
+
 // channel and group of the first of a thread's virtual channels; `next` steps to the one after
 struct Channel {
     int c, g, d;
@@ -392,7 +436,7 @@ struct Channel {
     }
 };
 // sums over the workgroup's threads of a[8], b[8] per virtual channel, joined per group: out[g stride] (zeros for a group with no channel in this workgroup's columns).
-// `lds`: blockDim.x (8 blockDim.x, V < 2) pairs.
+// `lds`: blockDim.x (V = 1: 8 blockDim.x) pairs.
 template <int V> __device__ __forceinline__ void join_groups(const double (&a)[8], const double (&b)[8], const NormArgs &A, const MapPlan &P, const Column &c, double2 *lds, double2 *out, int64_t stride) {
     const int NT = blockDim.x, at = c.r * P.bcol + c.col - c.first;
     __syncthreads();
@@ -404,26 +448,25 @@ template <int V> __device__ __forceinline__ void join_groups(const double (&a)[8
     }
     __syncthreads();
     const int lane = threadIdx.x & ((1 << P.lanes_log) - 1), teams = NT >> P.lanes_log;
-    const int D = V == 2 ? A.D >> 3 : A.D;                                                           // channels, or whole chunks of them
-    const int from = P.col_blocks == 1 ? 0 : V == 2 ? c.first : 8 * c.first, to = P.col_blocks == 1 ? A.G * D : from + (V == 2 ? P.bcol : 8 * P.bcol);
+    // in channels, or (V = 2) in whole chunks of them: the width of a group and of a row's copy, and this workgroup's columns
+    const int D = V == 2 ? A.D >> 3 : A.D, C = V == 2 ? A.C >> 3 : A.C, unit = V == 2 ? 1 : 8;
+    const int from = unit * c.first, to = unit * (c.first + P.bcol < P.ncol ? c.first + P.bcol : P.ncol);
 #pragma unroll 1
     for (int g0 = 0; g0 < A.G; g0 += teams) {                        // (every lane takes every turn: the exchange needs them all)
         const int g = g0 + (threadIdx.x >> P.lanes_log);
-        const int lo = g * D > from ? g * D : from, hi = (g + 1) * D < to ? (g + 1) * D : to, per = hi - lo;
         double s = 0.0, q = 0.0;
-        if (g < A.G && per > 0) {
-            const float inv_per = 1.f / (float)per;
-            for (int i = lane, entries = P.R * P.q * per; i < entries; i += 1 << P.lanes_log) {
-                const int t = small_quotient(i, inv_per), j = i - t * per;
-                double2 v;
-                if (V == 2) v = lds[t * P.bcol + lo + j - c.first];
-                else {
-                    const int r = t / P.q, vc = (t - r * P.q) * A.C + lo + j;
-                    v = lds[(vc & 7) * NT + r * P.bcol + (vc >> 3) - c.first];
+        if (g < A.G)
+#pragma unroll 1
+            for (int k = 0; k < 1 << P.q_log; k++) {
+                const int lo = k * C + g * D > from ? k * C + g * D : from, hi = k * C + (g + 1) * D < to ? k * C + (g + 1) * D : to, per = hi - lo;
+                if (per <= 0) continue;
+                const float inv_per = 1.f / (float)per;
+                for (int i = lane; i < P.R * per; i += 1 << P.lanes_log) {
+                    const int r = small_quotient(i, inv_per), v = lo + i - r * per;
+                    const double2 t = V == 2 ? lds[r * P.bcol + v - c.first] : lds[(v & 7) * NT + r * P.bcol + (v >> 3) - c.first];
+                    s += t.x; q += t.y;
                 }
-                s += v.x; q += v.y;
             }
-        }
         lanes_sum2(s, q, P.lanes_log);
         if (g < A.G && lane == 0) out[(int64_t)g * stride] = double2{s, q};
     }
@@ -441,43 +484,42 @@ template <bool DROP> __device__ __forceinline__ double slab_shift(const NormArgs
     return DROP && !kept(d, n * A.size) ? 0.0 : (double)v;
 }
 
-// part[n][g][split][column block] = sums of (x - s), (x - s)^2
+// part[n][g][split][column block] = sums of (x - s), (x - s)^2.  Grid: splits, column blocks, slabs.
 template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_sums(NormArgs A, MapPlan P, double2 *part) {
     extern __shared__ double2 lds[];
-    const int64_t width = (int64_t)P.q * A.C, items = A.N * P.splits;
-    const Column c = my_column(A, P, blockIdx.y);
+    const Column c = my_column(P, blockIdx.y);
+    const Span t = my_span(A, P, c, P.rows_per);
     Draw d = {};
     if (DROP) { d = make_draw(A.rng, A.site, A.cut); write_used(A); }
 #pragma unroll 1
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t n = item / P.splits, split = item - n * P.splits;
-        const T *x = (const T *)A.x + n * A.x_stride;
+    for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) {
+        const T *x = (const T *)A.x + n * A.x_stride + t.base;
+        int off = t.off;
+        Chunk<DT> v;
+        if (t.lim >= 8) v = span_load(x, t, off);
         const double shift = slab_shift<DROP>(A, d, n);
         double s[8] = {}, q[8] = {};
-        const int64_t end = (split + 1) * P.rows_per < P.rows ? (split + 1) * P.rows_per : P.rows;
-        if (c.mine)
-#pragma unroll 1
-            for (int64_t row = split * P.rows_per + c.r; row < end; row += 4 * P.R) {
-                const int64_t off = row * width + 8 * c.col;
-                int valid[4];
-                Chunk<DT> v[4];
-                map_valid<V, 4>(A, P, c, row, end, width, valid);
-                map_load<V, 4>(x + off, P.R * width, valid, v);
+        const auto add = [&](const Chunk<DT> &chunk, int valid) {
+            float f[8];
+            unpack<DROP>(chunk, DROP ? chunk_mask(d, n * A.size + t.base + off) : 255u, f);
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    if (!valid[u]) continue;
-                    float f[8];
-                    unpack<DROP>(v[u], DROP ? chunk_mask(d, n * A.size + off + u * P.R * width) : 255u, f);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        double t = (double)f[e] - shift;
-                        if (!V && e >= valid[u]) t = 0.0;
-                        s[e] += t; q[e] = fma(t, t, q[e]);
-                    }
-                }
+            for (int e = 0; e < 8; e++) {
+                const double u = e < valid ? (double)f[e] - shift : 0.0;
+                s[e] += u; q[e] = fma(u, u, q[e]);
             }
+        };
+        if (c.mine) {
+#pragma unroll 1
+            while (off + 8 <= t.lim) {
+                const Chunk<DT> now = v;
+                v = span_load(x, t, off + t.step);             // the next chunk is on its way while this one is added
+                add(now, 8);
+                off += t.step;
+            }
+            if (V == 1 && off < t.lim) add(load_chunk<DT>(x + off, t.lim - off), t.lim - off);
+        }
         const int64_t parts = (int64_t)P.splits * P.col_blocks;
-        join_groups<V>(s, q, A, P, c, lds, part + n * A.G * parts + split * P.col_blocks + blockIdx.y, parts);
+        join_groups<V>(s, q, A, P, c, lds, part + n * A.G * parts + blockIdx.x * P.col_blocks + blockIdx.y, parts);
     }
 }
 template <bool DROP> __global__ __launch_bounds__(256) void k_map_stats(NormArgs A, int splits, const double2 *part) {
@@ -492,23 +534,36 @@ template <bool DROP> __global__ __launch_bounds__(256) void k_map_stats(NormArgs
 // statistics and parameters of a thread's 8 virtual channels (V = 2: one group, statistics in element 0).
 // (The column is hidden from the compiler: it would keep every address of a loop over slabs in registers, and spill.)
 template <int V> struct Constants { float mean[V == 2 ? 1 : 8], rest[V == 2 ? 1 : 8], rstd[V == 2 ? 1 : 8], w[8], b[8]; };
-template <int V> __device__ __forceinline__ void load_constants(const NormArgs &A, int64_t n, int col, Constants<V> &k) {
+template <int V> __device__ __forceinline__ void load_constants(const NormArgs &A, const MapPlan &P, int64_t n, int col, Constants<V> &k) {
     asm volatile("" : "+v"(col));
     Channel ch(A, 8 * col);
     const double2 *stats = A.stats + n * A.G;
-    if (V == 2) {
-        const double2 st = stats[ch.g];
-        k.mean[0] = (float)st.x; k.rest[0] = (float)(st.x - (double)k.mean[0]); k.rstd[0] = (float)st.y;
-        row_params<1>(A.w, ch.c, 8, 1.f, k.w);
-        row_params<1>(A.b, ch.c, 8, 0.f, k.b);
-    } else
+    if (P.q_log == 0) {                         // (columns do not wrap: the parameters as whole chunks)
+        row_params<1>(A, A.w, 8 * col, 1.f, k.w);
+        row_params<1>(A, A.b, 8 * col, 0.f, k.b);
+    } else {
+        Channel c = ch;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const double2 st = stats[ch.g];
-            const int i = V == 2 ? 0 : e;
-            k.mean[i] = (float)st.x; k.rest[i] = (float)(st.x - (double)k.mean[i]); k.rstd[i] = (float)st.y;
-            k.w[e] = A.w ? (float)((const W *)A.w)[ch.c] : 1.f;
-            k.b[e] = A.b ? (float)((const W *)A.b)[ch.c] : 0.f;
+            k.w[e] = A.w ? (float)((const W *)A.w)[c.c] : 1.f;
+            k.b[e] = A.b ? (float)((const W *)A.b)[c.c] : 0.f;
+            c.next(A);
+        }
+    }
+    const double2 st = stats[ch.g];
+    const float mean = (float)st.x, rest = (float)(st.x - (double)mean), rstd = (float)st.y;
+    if (V == 2) { k.mean[0] = mean; k.rest[0] = rest; k.rstd[0] = rstd; return; }
+    if (A.D >= 8) {                                         // the chunk reaches into one more group at most
+        const int split = A.D - ch.d;
+        const double2 st1 = stats[ch.g + 1 < A.G ? ch.g + 1 : 0];
+        const float mean1 = (float)st1.x, rest1 = (float)(st1.x - (double)mean1), rstd1 = (float)st1.y;
+#pragma unroll
+        for (int i = 0; i < (V == 2 ? 1 : 8); i++) { k.mean[i] = i < split ? mean : mean1; k.rest[i] = i < split ? rest : rest1; k.rstd[i] = i < split ? rstd : rstd1; }
+    } else
+#pragma unroll
+        for (int i = 0; i < (V == 2 ? 1 : 8); i++) {
+            const double2 t = stats[ch.g];
+            k.mean[i] = (float)t.x; k.rest[i] = (float)(t.x - (double)k.mean[i]); k.rstd[i] = (float)t.y;
             ch.next(A);
         }
 }
@@ -516,51 +571,39 @@ template <int V> __device__ __forceinline__ void normalise(const Constants<V> &k
 #pragma unroll
     for (int e = 0; e < 8; e++) { const int i = V == 2 ? 0 : e; v[e] = ((v[e] - k.mean[i]) - k.rest[i]) * k.rstd[i]; }
 }
-// item number `item` of the result's launch -> slab, column block and rows
-struct ApplyItem { int64_t n, row, end; int col_block; };
-__device__ __forceinline__ ApplyItem apply_item(const MapPlan &P, int64_t item) {
-    ApplyItem t;
-    const int per = P.col_blocks * P.row_blocks;
-    t.n = item / per;
-    const int left = (int)(item - t.n * per);
-    t.col_block = P.col_blocks == 1 ? 0 : left / P.row_blocks;
-    t.row = (int64_t)(left - t.col_block * P.row_blocks) * P.apply_rows;
-    t.end = t.row + P.apply_rows < P.rows ? t.row + P.apply_rows : P.rows;
-    return t;
-}
 template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_apply(NormArgs A, MapPlan P) {
-    const int64_t width = (int64_t)P.q * A.C, items = A.N * P.col_blocks * P.row_blocks;
+    const Column c = my_column(P, blockIdx.y);
+    if (!c.mine) return;
+    const Span t = my_span(A, P, c, P.apply_rows);
     Draw d = {};
     if (DROP) d = make_draw(A.rng, A.site, A.cut);
 #pragma unroll 1
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const ApplyItem t = apply_item(P, item);
-        const Column c = my_column(A, P, t.col_block);
-        if (!c.mine) continue;
+    for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) {
+        const T *x = (const T *)A.x + n * A.x_stride + t.base;
+        T *y = (T *)A.out + n * A.size + t.base;
+        int off = t.off;
+        Chunk<DT> v;
+        if (t.lim >= 8) v = span_load(x, t, off);
         Constants<V> k;
-        load_constants<V>(A, t.n, c.col, k);
-        const T *x = (const T *)A.x + t.n * A.x_stride;
-        T *y = (T *)A.out + t.n * A.size;
+        load_constants<V>(A, P, n, c.col, k);
+#pragma unroll
+        for (int e = 0; e < 8; e++) k.w[e] *= k.rstd[V == 2 ? 0 : e];
+        const auto result = [&](const Chunk<DT> &chunk, float (&f)[8]) {
+            unpack<DROP>(chunk, DROP ? chunk_mask(d, n * A.size + t.base + off) : 255u, f);
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] = ((f[e] - k.mean[V == 2 ? 0 : e]) - k.rest[V == 2 ? 0 : e]) * k.w[e] + k.b[e];
+            activate(f, A.act);
+        };
+        float f[8];
 #pragma unroll 1
-        for (int64_t row = t.row + c.r; row < t.end; row += 4 * P.R) {
-            const int64_t off = row * width + 8 * c.col;
-            int valid[4];
-            Chunk<DT> v[4];
-            map_valid<V, 4>(A, P, c, row, t.end, width, valid);
-            map_load<V, 4>(x + off, P.R * width, valid, v);
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                if (!valid[u]) continue;
-                const int64_t at = off + u * P.R * width;
-                float f[8];
-                unpack<DROP>(v[u], DROP ? chunk_mask(d, t.n * A.size + at) : 255u, f);
-                normalise<V>(k, f);
-#pragma unroll
-                for (int e = 0; e < 8; e++) f[e] = f[e] * k.w[e] + k.b[e];
-                activate(f, A.act);
-                row_store<V>(y + at, valid[u], f);
-            }
+        while (off + 8 <= t.lim) {
+            const Chunk<DT> now = v;
+            v = span_load(x, t, off + t.step);
+            result(now, f);
+            store_whole<DT>(y + off, f);
+            off += t.step;
         }
+        if (V == 1 && off < t.lim) { result(load_chunk<DT>(x + off, t.lim - off), f); store_chunk<DT>(y + off, t.lim - off, f); }
     }
 }
 
@@ -568,42 +611,40 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_apply(N
 // = sum w dz, sum w dz xh), in 64 bits.
 template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_sums(NormArgs A, MapPlan P, double2 *part, float *params) {
     extern __shared__ double2 lds[];
-    const int64_t width = (int64_t)P.q * A.C, items = A.N * P.splits;
-    const Column c = my_column(A, P, blockIdx.y);
+    const Column c = my_column(P, blockIdx.y);
+    const Span t = my_span(A, P, c, P.rows_per);
     const int NT = blockDim.x;
     Draw d = {};
     if (DROP) d = make_draw(A.rng, A.site, A.cut);
 #pragma unroll 1
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t n = item / P.splits, split = item - n * P.splits;
-        const T *x = (const T *)A.x + n * A.x_stride, *dy = (const T *)A.dy + n * A.dy_stride;
+    for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) {
+        const T *x = (const T *)A.x + n * A.x_stride + t.base, *dy = (const T *)A.dy + n * A.dy_stride + t.base;
+        int off = t.off;
+        Chunk<DT> v, g;
+        if (t.lim >= 8) { v = span_load(x, t, off); g = span_load(dy, t, off); }
         double s1[8] = {}, s2[8] = {};
         Constants<V> k;
+        load_constants<V>(A, P, n, c.col, k);
+        const auto add = [&](const Chunk<DT> &cx, const Chunk<DT> &cg, int valid) {
+            const uint32_t m = DROP ? chunk_mask(d, n * A.size + t.base + off) : 255u;
+            float xh[8], dv[8], dz[8];
+            unpack<DROP>(cx, m, xh);
+            unpack<false>(cg, 255u, dv);
+            normalise<V>(k, xh);
+            back_activation<DROP>(A, x + off, n, 8 * c.col, valid, m, xh, dv, k.w, k.b, dz);
+#pragma unroll
+            for (int e = 0; e < 8; e++) { s1[e] += (double)dz[e]; s2[e] += (double)(dz[e] * xh[e]); }
+        };
         if (c.mine) {
-            load_constants<V>(A, n, c.col, k);
-            const int64_t end = (split + 1) * P.rows_per < P.rows ? (split + 1) * P.rows_per : P.rows;
 #pragma unroll 1
-            for (int64_t row = split * P.rows_per + c.r; row < end; row += 2 * P.R) {
-                const int64_t off = row * width + 8 * c.col;
-                int valid[2];
-                Chunk<DT> v[2], g[2];
-                map_valid<V, 2>(A, P, c, row, end, width, valid);
-                map_load<V, 2>(x + off, P.R * width, valid, v);
-                map_load<V, 2>(dy + off, P.R * width, valid, g);
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    if (!valid[u]) continue;
-                    const int64_t at = off + u * P.R * width;
-                    const uint32_t m = DROP ? chunk_mask(d, n * A.size + at) : 255u;
-                    float xh[8], dv[8], dz[8];
-                    unpack<DROP>(v[u], m, xh);
-                    unpack<false>(g[u], 255u, dv);
-                    normalise<V>(k, xh);
-                    back_activation<DROP, V>(A, x + at, n, 8 * c.col, valid[u], m, xh, dv, k.w, k.b, dz);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) { s1[e] += (double)dz[e]; s2[e] += (double)(dz[e] * xh[e]); }
-                }
+            while (off + 8 <= t.lim) {
+                const Chunk<DT> now = v, gnow = g;
+                v = span_load(x, t, off + t.step); g = span_load(dy, t, off + t.step);
+                add(now, gnow, 8);
+                off += t.step;
             }
+            // (of the part's other elements dy is zero)
+            if (V == 1 && off < t.lim) add(load_chunk<DT>(x + off, t.lim - off), load_chunk<DT>(dy + off, t.lim - off), t.lim - off);
         }
         if (params) {
             // channel by channel over the workgroup's threads: a few lanes per channel where channels are few
@@ -612,24 +653,27 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_su
 #pragma unroll
                 for (int e = 0; e < 8; e++) lds[e * NT + c.r * P.bcol + c.col - c.first] = double2{s2[e], s1[e]};
             __syncthreads();
-            float *to = params + blockIdx.x * 2 * (int64_t)A.C;
-            const int from = P.col_blocks == 1 ? 0 : 8 * c.first, last = P.col_blocks == 1 || 8 * (c.first + P.bcol) > A.C ? A.C : 8 * (c.first + P.bcol);
+            // (column blocks of one position each have channels of their own, of several positions they share them)
+            const int64_t row = P.q_log ? (int64_t)blockIdx.z * gridDim.y + blockIdx.y : blockIdx.z;
+            float *to = params + (row * gridDim.x + blockIdx.x) * 2 * A.C;
             const int lane = threadIdx.x & 7;
+            const int from = P.q_log ? 0 : 8 * c.first, last = P.q_log || 8 * (c.first + P.bcol) > A.C ? A.C : 8 * (c.first + P.bcol);
 #pragma unroll 1
             for (int c8 = from; c8 < last; c8 += NT >> 3) {
                 const int ch = c8 + (threadIdx.x >> 3);
                 double s = 0.0, q = 0.0;
                 if (ch < last)
-                    for (int i = lane; i < P.q * P.R; i += 8) {
-                        const int r = i / P.q, vc = (i - r * P.q) * A.C + ch;
-                        const double2 v = lds[(vc & 7) * NT + r * P.bcol + (vc >> 3) - c.first];
+                    for (int i = lane; i < P.R << P.q_log; i += 8) {
+                        const int r = i >> P.q_log, vc = (i - (r << P.q_log)) * A.C + ch, col = (vc >> 3) - c.first;
+                        if (col < 0 || col >= P.bcol || col + c.first >= P.ncol) continue;
+                        const double2 v = lds[(vc & 7) * NT + r * P.bcol + col];
                         s += v.x; q += v.y;
                     }
                 lanes_sum2(s, q, 3);
                 if (ch < last && lane < 2) {
-                    float *word = to + lane * (int64_t)A.C + ch;              // (this thread's own word: later items of the workgroup add to it)
+                    float *word = to + lane * (int64_t)A.C + ch;              // (this thread's own word: later slabs of the workgroup add to it)
                     const float v = (float)(lane ? q : s);
-                    *word = item == blockIdx.x ? v : *word + v;
+                    *word = n == blockIdx.z ? v : *word + v;
                 }
             }
         }
@@ -637,7 +681,7 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_su
 #pragma unroll
             for (int e = 0; e < 8; e++) { s1[e] *= (double)k.w[e]; s2[e] *= (double)k.w[e]; }
         const int64_t parts = (int64_t)P.splits * P.col_blocks;
-        join_groups<V>(s1, s2, A, P, c, lds, part + n * A.G * parts + split * P.col_blocks + blockIdx.y, parts);
+        join_groups<V>(s1, s2, A, P, c, lds, part + n * A.G * parts + blockIdx.x * P.col_blocks + blockIdx.y, parts);
     }
 }
 // second launch: the first workgroups join the splits of each (n, g) into {mean of w dz, mean of w dz xh}, the others the parameter gradients
@@ -650,50 +694,52 @@ __global__ __launch_bounds__(1024) void k_map_back_join(NormArgs A, int splits, 
     }
 }
 template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_apply(NormArgs A, MapPlan P, const float2 *means) {
-    const int64_t width = (int64_t)P.q * A.C, items = A.N * P.col_blocks * P.row_blocks;
+    const Column c = my_column(P, blockIdx.y);
+    if (!c.mine) return;
+    const Span t = my_span(A, P, c, P.apply_rows);
     Draw d = {};
     if (DROP) d = make_draw(A.rng, A.site, A.cut);
 #pragma unroll 1
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const ApplyItem t = apply_item(P, item);
-        const Column c = my_column(A, P, t.col_block);
-        if (!c.mine) continue;
+    for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) {
+        const T *x = (const T *)A.x + n * A.x_stride + t.base, *dy = (const T *)A.dy + n * A.dy_stride + t.base;
+        T *dx = (T *)A.out + n * A.size + t.base;
+        int off = t.off;
+        Chunk<DT> v, g;
+        if (t.lim >= 8) { v = span_load(x, t, off); g = span_load(dy, t, off); }
         Constants<V> k;
-        load_constants<V>(A, t.n, c.col, k);
+        load_constants<V>(A, P, n, c.col, k);
         float m1[V == 2 ? 1 : 8], m2[V == 2 ? 1 : 8];
         {
             Channel ch(A, 8 * c.col);
 #pragma unroll
-            for (int e = 0; e < (V == 2 ? 1 : 8); e++) { const float2 m = means[t.n * A.G + ch.g]; m1[e] = m.x; m2[e] = m.y; ch.next(A); }
+            for (int e = 0; e < (V == 2 ? 1 : 8); e++) { const float2 m = means[n * A.G + ch.g]; m1[e] = m.x; m2[e] = m.y; ch.next(A); }
         }
-        const T *x = (const T *)A.x + t.n * A.x_stride, *dy = (const T *)A.dy + t.n * A.dy_stride;
-        T *dx = (T *)A.out + t.n * A.size;
-#pragma unroll 1
-        for (int64_t row = t.row + c.r; row < t.end; row += 2 * P.R) {
-            const int64_t off = row * width + 8 * c.col;
-            int valid[2];
-            Chunk<DT> v[2], g[2];
-            map_valid<V, 2>(A, P, c, row, t.end, width, valid);
-            map_load<V, 2>(x + off, P.R * width, valid, v);
-            map_load<V, 2>(dy + off, P.R * width, valid, g);
+        const auto result = [&](const Chunk<DT> &cx, const Chunk<DT> &cg, int valid, float (&dz)[8]) {
+            const uint32_t m = DROP ? chunk_mask(d, n * A.size + t.base + off) : 255u;
+            float xh[8], dv[8];
+            unpack<DROP>(cx, m, xh);
+            unpack<false>(cg, 255u, dv);
+            normalise<V>(k, xh);
+            back_activation<DROP>(A, x + off, n, 8 * c.col, valid, m, xh, dv, k.w, k.b, dz);
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                if (!valid[u]) continue;
-                const int64_t at = off + u * P.R * width;
-                const uint32_t m = DROP ? chunk_mask(d, t.n * A.size + at) : 255u;
-                float xh[8], dv[8], dz[8];
-                unpack<DROP>(v[u], m, xh);
-                unpack<false>(g[u], 255u, dv);
-                normalise<V>(k, xh);
-                back_activation<DROP, V>(A, x + at, t.n, 8 * c.col, valid[u], m, xh, dv, k.w, k.b, dz);
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int i = V == 2 ? 0 : e;
-                    const float r = k.rstd[i] * (dz[e] * k.w[e] - m1[i] - xh[e] * m2[i]);
-                    dz[e] = !DROP || m >> e & 1u ? r : 0.f;
-                }
-                row_store<V>(dx + at, valid[u], dz);
+            for (int e = 0; e < 8; e++) {
+                const int i = V == 2 ? 0 : e;
+                const float r = k.rstd[i] * (dz[e] * k.w[e] - m1[i] - xh[e] * m2[i]);
+                dz[e] = !DROP || m >> e & 1u ? r : 0.f;
             }
+        };
+        float f[8];
+#pragma unroll 1
+        while (off + 8 <= t.lim) {
+            const Chunk<DT> now = v, gnow = g;
+            v = span_load(x, t, off + t.step); g = span_load(dy, t, off + t.step);
+            result(now, gnow, 8, f);
+            store_whole<DT>(dx + off, f);
+            off += t.step;
+        }
+        if (V == 1 && off < t.lim) {
+            result(load_chunk<DT>(x + off, t.lim - off), load_chunk<DT>(dy + off, t.lim - off), t.lim - off, f);
+            store_chunk<DT>(dx + off, t.lim - off, f);
         }
     }
 }
@@ -716,35 +762,26 @@ void row_backward(const NormArgs &a, const RowLaunch &r, float *part, hipStream_
 unsigned column_blocks(const NormArgs &a) { return (unsigned)((2 * (int64_t)a.C + 15) / 16); }
 void params(const NormArgs &a, const float *part, int rows, void *dw, void *db, hipStream_t s) { k_row_params<<<column_blocks(a), 1024, 0, s>>>(a, part, rows, dw, db); }
 
-int variant(const NormArgs &a, const MapLaunch &m) {
-    const int64_t width = (int64_t)m.P.q * a.C;
-    return width % 8 || a.size % width ? 0 : a.C % 8 || a.D % 8 ? 1 : 2;
-}
+bool one_group(const NormArgs &a) { return a.C % 8 == 0 && a.D % 8 == 0; }
 template <int V, bool DROP> void map_forward_v(const NormArgs &a, const MapLaunch &m, double2 *part, hipStream_t s) {
     k_map_sums<V, DROP><<<m.sums, m.NT, (size_t)m.NT * (V == 2 ? 16 : 128), s>>>(a, m.P, part);
     k_map_stats<DROP><<<m.stat_blocks, 256, 0, s>>>(a, m.P.splits * m.P.col_blocks, part);
-    k_map_apply<V, DROP><<<m.apply_blocks, m.NT, 0, s>>>(a, m.P);
+    k_map_apply<V, DROP><<<m.apply, m.NT, 0, s>>>(a, m.P);
 }
 void map_forward(const NormArgs &a, const MapLaunch &m, double2 *part, hipStream_t s) {
-    switch (variant(a, m)) {
-    case 0: a.cut ? map_forward_v<0, true>(a, m, part, s) : map_forward_v<0, false>(a, m, part, s); break;
-    case 1: a.cut ? map_forward_v<1, true>(a, m, part, s) : map_forward_v<1, false>(a, m, part, s); break;
-    default: a.cut ? map_forward_v<2, true>(a, m, part, s) : map_forward_v<2, false>(a, m, part, s); break;
-    }
+    if (one_group(a)) a.cut ? map_forward_v<2, true>(a, m, part, s) : map_forward_v<2, false>(a, m, part, s);
+    else a.cut ? map_forward_v<1, true>(a, m, part, s) : map_forward_v<1, false>(a, m, part, s);
 }
 template <int V, bool DROP> void map_backward_v(const NormArgs &a, const MapLaunch &m, double2 *part, float2 *means, float *sums, void *dw, void *db, hipStream_t s) {
     k_map_back_sums<V, DROP><<<m.sums, m.NT, (size_t)m.NT * 128, s>>>(a, m.P, part, sums);
     const int64_t items = a.N * a.G;
     const int join = (int)(items < 16 * 4096 ? (items + 15) / 16 : 4096);
-    k_map_back_join<<<join + (sums ? column_blocks(a) : 0), 1024, 0, s>>>(a, m.P.splits * m.P.col_blocks, part, sums, (int)m.sums.x, join, means, dw, db);
-    k_map_back_apply<V, DROP><<<m.apply_blocks, m.NT, 0, s>>>(a, m.P, means);
+    k_map_back_join<<<join + (sums ? column_blocks(a) : 0), 1024, 0, s>>>(a, m.P.splits * m.P.col_blocks, part, sums, m.param_rows, join, means, dw, db);
+    k_map_back_apply<V, DROP><<<m.apply, m.NT, 0, s>>>(a, m.P, means);
 }
 void map_backward(const NormArgs &a, const MapLaunch &m, double2 *part, float2 *means, float *sums, void *dw, void *db, hipStream_t s) {
-    switch (variant(a, m)) {
-    case 0: a.cut ? map_backward_v<0, true>(a, m, part, means, sums, dw, db, s) : map_backward_v<0, false>(a, m, part, means, sums, dw, db, s); break;
-    case 1: a.cut ? map_backward_v<1, true>(a, m, part, means, sums, dw, db, s) : map_backward_v<1, false>(a, m, part, means, sums, dw, db, s); break;
-    default: a.cut ? map_backward_v<2, true>(a, m, part, means, sums, dw, db, s) : map_backward_v<2, false>(a, m, part, means, sums, dw, db, s); break;
-    }
+    if (one_group(a)) a.cut ? map_backward_v<2, true>(a, m, part, means, sums, dw, db, s) : map_backward_v<2, false>(a, m, part, means, sums, dw, db, s);
+    else a.cut ? map_backward_v<1, true>(a, m, part, means, sums, dw, db, s) : map_backward_v<1, false>(a, m, part, means, sums, dw, db, s);
 }
 
 }  // namespace
