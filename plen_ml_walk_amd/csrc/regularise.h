@@ -17,17 +17,51 @@ template <> struct Elem<PLENREG_F16> { typedef _Float16 T; };
 
 // ---- 8 neighbouring elements, the unit of every kernel: 16 bytes of a 16-bit type, 32 of float32; aligned like one element only (rows of odd
 //      widths begin anywhere; the wide loads take any address)
-template <int DT> struct Chunk { typename Elem<DT>::T v[8]; };
+//      (Held as 32-bit words: 16-bit elements would be taken apart, and waited for, at the end of every block that a load is carried out of.)
+template <int DT> struct Chunk {
+    uint32_t w[DT == PLENREG_F32 ? 8 : 4];
+    __device__ __forceinline__ float get(int e) const {          // (e is a constant where this is inlined)
+        if constexpr (DT == PLENREG_F32) return __uint_as_float(w[e]);
+        else if constexpr (DT == PLENREG_BF16) return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+        else return (float)__builtin_bit_cast(_Float16, (uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1]));
+    }
+};
+template <int DT> static __device__ __forceinline__ Chunk<DT> pack(const float (&v)[8]) {
+    typedef typename Elem<DT>::T Two __attribute__((ext_vector_type(2)));
+    Chunk<DT> c;
+    if constexpr (DT == PLENREG_F32) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) c.w[e] = __float_as_uint(v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) c.w[e] = __builtin_bit_cast(uint32_t, Two{(typename Elem<DT>::T)v[2 * e], (typename Elem<DT>::T)v[2 * e + 1]});
+    }
+    return c;
+}
 template <int DT> static __device__ __forceinline__ Chunk<DT> load_whole(const typename Elem<DT>::T *p) {
     Chunk<DT> c;
     __builtin_memcpy(&c, p, sizeof c);
     return c;
 }
 template <int DT> static __device__ __forceinline__ void store_whole(typename Elem<DT>::T *p, const float (&v)[8]) {
+    const Chunk<DT> c = pack<DT>(v);
+    __builtin_memcpy(p, &c, sizeof c);
+}
+// the same past the caches (non-temporal): for tensors beyond what these hold, where keeping this one throws out others
+typedef uint32_t Word4 __attribute__((ext_vector_type(4), aligned(2)));
+template <int DT> static __device__ __forceinline__ Chunk<DT> stream_whole(const typename Elem<DT>::T *p) {
     Chunk<DT> c;
 #pragma unroll
-    for (int e = 0; e < 8; e++) c.v[e] = (typename Elem<DT>::T)v[e];
-    __builtin_memcpy(p, &c, sizeof c);
+    for (int i = 0; i < (int)(sizeof c / 16); i++) {
+        const Word4 t = __builtin_nontemporal_load((const Word4 *)p + i);
+        c.w[4 * i] = t.x; c.w[4 * i + 1] = t.y; c.w[4 * i + 2] = t.z; c.w[4 * i + 3] = t.w;
+    }
+    return c;
+}
+template <int DT> static __device__ __forceinline__ void stream_store_whole(typename Elem<DT>::T *p, const float (&v)[8]) {
+    const Chunk<DT> c = pack<DT>(v);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof c / 16); i++) __builtin_nontemporal_store(Word4{c.w[4 * i], c.w[4 * i + 1], c.w[4 * i + 2], c.w[4 * i + 3]}, (Word4 *)p + i);
 }
 // Part of a chunk goes as four, two and one elements.  Quad: four elements in one register value (an array here would be put into memory).
 template <int SIZE> struct Quad;
@@ -65,9 +99,7 @@ template <int DT> static __device__ __forceinline__ void store_chunk(typename El
     typedef typename Elem<DT>::T T;
     typedef Quad<sizeof(T)> Q;
     if (valid >= 8) { store_whole<DT>(p, v); return; }
-    Chunk<DT> c;
-#pragma unroll
-    for (int e = 0; e < 8; e++) c.v[e] = (T)v[e];
+    const Chunk<DT> c = pack<DT>(v);
     struct { typename Q::Four lo, hi; } both;
     __builtin_memcpy(&both, &c, sizeof c);
     if (valid & 4) __builtin_memcpy(p, &both.lo, sizeof both.lo);
@@ -95,13 +127,39 @@ static __device__ __forceinline__ uint32_t block_mask(const Draw &d, uint32_t bl
     for (int k = 0; k < 4; k++) m |= ((words[k] & 0xffffu) >= d.cut ? 1u << (2 * k) : 0u) | ((words[k] >> 16) >= d.cut ? 2u << (2 * k) : 0u);
     return m;
 }
-// ... of the 8 elements from element i on
-static __device__ __forceinline__ uint32_t chunk_mask(const Draw &d, int64_t i) {
-    const uint32_t block = (uint32_t)(i >> 3), shift = (uint32_t)i & 7u;
-    uint32_t m = block_mask(d, block);
-    if (shift) m = (m | block_mask(d, block + 1) << 8) >> shift;
-    return m;
-}
+// the mask of the 8 elements from element i on.  M = 2: i is a multiple of 8, the block's words are kept and compared where the mask is used (two instructions an element);
+// M = 1: any i, one bit per element; M = 0: nothing is dropped
+template <int M> struct Mask;
+template <> struct Mask<2> {
+    u4 w;
+    uint32_t cut;
+    __device__ __forceinline__ Mask(const Draw &d, int64_t i) : w(block_words(d, (uint32_t)(i >> 3))), cut(d.cut) {}
+    __device__ __forceinline__ float keep(int e, float v) const {          // (e is a constant where this is inlined)
+        const uint32_t word = e < 2 ? w.x : e < 4 ? w.y : e < 6 ? w.z : w.w;
+        return (e & 1 ? word >> 16 : word & 0xffffu) >= cut ? v : 0.f;
+    }
+    __device__ __forceinline__ uint32_t bits() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) m |= keep(e, 1.f) != 0.f ? 1u << e : 0u;
+        return m;
+    }
+};
+template <> struct Mask<1> {
+    uint32_t m;
+    __device__ __forceinline__ Mask(const Draw &d, int64_t i) {
+        const uint32_t block = (uint32_t)(i >> 3), shift = (uint32_t)i & 7u;
+        m = block_mask(d, block);
+        if (shift) m = (m | block_mask(d, block + 1) << 8) >> shift;
+    }
+    __device__ __forceinline__ float keep(int e, float v) const { return m >> e & 1u ? v : 0.f; }
+    __device__ __forceinline__ uint32_t bits() const { return m; }
+};
+template <> struct Mask<0> {
+    __device__ __forceinline__ Mask(const Draw &, int64_t) {}
+    __device__ __forceinline__ float keep(int, float v) const { return v; }
+    __device__ __forceinline__ uint32_t bits() const { return 255u; }
+};
 static __device__ __forceinline__ bool kept(const Draw &d, int64_t i) { return block_mask(d, (uint32_t)(i >> 3)) >> (i & 7) & 1u; }
 
 // ---- group norm: arguments and plans as the host hands them to the kernels (quotients and scales worked out once)
@@ -122,11 +180,11 @@ static __device__ __forceinline__ int small_quotient(int i, float inv_n) { retur
 
 // rows of one position: 2^team_log lanes per (row, group); a workgroup covers gb neighbouring groups of rb rows per turn
 struct RowPlan { int team_log, gb, rb, trips; float inv_gb; };
-struct RowLaunch { RowPlan P; int K, NT; dim3 grid; };
+struct RowLaunch { RowPlan P; int K, NT; dim3 grid; bool stream; };
 // many positions.  A slab as `rows` rows of `ncol` chunk columns (2^q_log positions to a row); bcol columns in a workgroup, R rows per turn of it; rows_per rows in a
 // workgroup of the sums, apply_rows in one of the result; 2^lanes_log lanes join one group
 struct MapPlan { int q_log, ncol, bcol, col_blocks, R, splits, lanes_log; int64_t rows, rows_per, apply_rows; float inv_bcol; };
-struct MapLaunch { MapPlan P; dim3 sums, apply; int NT, param_rows; unsigned stat_blocks; };
+struct MapLaunch { MapPlan P; dim3 sums, apply; int NT, param_rows; unsigned stat_blocks; bool stream; };
 
 // one per pair of element types (x and results, parameters), in regularise_norm.hip
 struct NormEntry {

@@ -3,11 +3,8 @@
 #include "regularise.h"
 
 #define DROPOUT_SMALL (1 << 18)
-#ifndef MAP_BLOCKS
-#define MAP_BLOCKS 512
-#endif
-#ifndef MAP_APPLY_BLOCKS
-#define MAP_APPLY_BLOCKS 512
+#ifndef STREAM_BYTES
+#define STREAM_BYTES ((int64_t)64 << 20)
 #endif
 #define MAP_MAX_SPAN ((int64_t)1 << 28)      // elements of a slab that one workgroup walks over
 #define ROW_MAX_FORWARD 8192            // widest group that the lanes of one workgroup hold: 256 lanes of 4 chunks, or in the backward pass (which holds four times as much) 512 of one
@@ -16,16 +13,6 @@
 // ---- dropout.  U chunks per thread: all loads are issued before the first mask is drawn.  In rows that are not contiguous (ROWS) a chunk that crosses
 //      the end of a row is loaded element by element.
 struct DropArgs { const void *x; void *y; const uint64_t *rng; uint64_t *used; int64_t rows, cols, x_stride; uint32_t cut; int site; float scale; };
-// v[e] = kept ? v[e] scale : 0 for a whole block of 8 elements
-static __device__ __forceinline__ void drop_block(const Draw &d, uint32_t block, float scale, float (&v)[8]) {
-    const u4 w = block_words(d, block);
-    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const float s = v[e] * scale;
-        v[e] = ((e & 1 ? words[e >> 1] >> 16 : words[e >> 1] & 0xffffu) >= d.cut) ? s : 0.f;
-    }
-}
 template <int DT, int U, bool ROWS> __global__ __launch_bounds__(256) void k_dropout(DropArgs A) {
     typedef typename Elem<DT>::T T;
     const T *x = (const T *)A.x;
@@ -36,13 +23,13 @@ template <int DT, int U, bool ROWS> __global__ __launch_bounds__(256) void k_dro
     if (!ROWS && (first + 256 * U) * 8 <= n) {                     // every chunk of the workgroup is whole
         Chunk<DT> c[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) c[u] = load_whole<DT>(x + (first + u * 256 + threadIdx.x) * 8);
+        for (int u = 0; u < U; u++) c[u] = U > 1 ? stream_whole<DT>(x + (first + u * 256 + threadIdx.x) * 8) : load_whole<DT>(x + (first + u * 256 + threadIdx.x) * 8);
 #pragma unroll
         for (int u = 0; u < U; u++) {
+            const Mask<2> m(d, (first + u * 256 + threadIdx.x) * 8);
             float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = (float)c[u].v[e];
-            drop_block(d, (uint32_t)(first + u * 256 + threadIdx.x), A.scale, v);
+            for (int e = 0; e < 8; e++) v[e] = m.keep(e, c[u].get(e) * A.scale);
             store_whole<DT>(y + (first + u * 256 + threadIdx.x) * 8, v);
         }
         return;
@@ -51,20 +38,26 @@ template <int DT, int U, bool ROWS> __global__ __launch_bounds__(256) void k_dro
         const int64_t j = first + u * 256 + threadIdx.x, i = j << 3;
         if (i >= n) return;
         const int valid = n - i < 8 ? (int)(n - i) : 8;
-        Chunk<DT> c;
-        if (ROWS) {
-            int64_t row = n >> 32 ? i / A.cols : (int64_t)((uint32_t)i / (uint32_t)A.cols), col = i - row * A.cols;
-            if (col + valid <= A.cols) c = load_chunk<DT>(x + row * A.x_stride + col, valid);
-            else
-                for (int e = 0; e < 8; e++) {
-                    c.v[e] = e < valid ? x[row * A.x_stride + col] : (T)0.f;
-                    if (++col == A.cols) { col = 0; row++; }
-                }
-        } else c = load_chunk<DT>(x + i, valid);
         float v[8];
+        int64_t row = 0, col = i;
+        if (ROWS) {
+            row = n >> 32 ? i / A.cols : (int64_t)((uint32_t)i / (uint32_t)A.cols);
+            col = i - row * A.cols;
+        }
+        if (!ROWS || col + valid <= A.cols) {
+            const Chunk<DT> c = load_chunk<DT>(x + row * A.x_stride + col, valid);
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = (float)c.v[e];
-        drop_block(d, (uint32_t)j, A.scale, v);
+            for (int e = 0; e < 8; e++) v[e] = c.get(e);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                v[e] = e < valid ? (float)x[row * A.x_stride + col] : 0.f;
+                if (++col == A.cols) { col = 0; row++; }
+            }
+        }
+        const Mask<2> m(d, i);
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = m.keep(e, v[e] * A.scale);
         store_chunk<DT>(y + i, valid, v);
     }
 }
@@ -87,6 +80,8 @@ static int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static int log2_up(int64_t v) { int k = 0; while (((int64_t)1 << k) < v) k++; return k; }
 
 static bool by_rows(const PlenRegNorm &a, bool backward) { return a.L == 1 && a.C / a.G <= (backward ? ROW_MAX_BACKWARD : ROW_MAX_FORWARD); }
+// is a tensor of x's shape beyond what the caches keep for whoever reads it next?
+static bool streams(const PlenRegNorm &a) { return a.N * a.L * a.C * (a.dtype == PLENREG_F32 ? 4 : 2) >= STREAM_BYTES; }
 static RowLaunch row_plan(const PlenRegNorm &a, bool backward) {
     const int64_t chunks = div_up(a.C / a.G, 8);
     RowLaunch r;
@@ -105,6 +100,7 @@ static RowLaunch row_plan(const PlenRegNorm &a, bool backward) {
     if (gx > need) gx = need;
     r.P.trips = (int)div_up(need, gx);
     r.grid = dim3((unsigned)gx, (unsigned)gy);
+    r.stream = streams(a);
     return r;
 }
 // threads (a multiple of 64) of which the fewest idle when `ncol` of them make a row
@@ -131,10 +127,12 @@ static MapLaunch map_plan(const PlenRegNorm &a) {
     m.P.inv_bcol = 1.f / (float)m.P.bcol;
     m.NT = fill_threads(m.P.bcol, 256, 512);
     m.P.R = m.NT / m.P.bcol;
-    // ~2 workgroups per compute unit, each thread in whole turns of 2 rows
+    // 2 workgroups per compute unit, or 4 where their threads then still have 16 chunks each; each thread in whole turns of 2 rows.  (8 x 4096 x 320: 512 workgroups 9.2 + 9.5 us,
+    // 1024: 10.8 + 9.8; 2 x 262144 x 128: 47 + 42 and 40 + 43)
+    const int64_t blocks = a.N * chunks >= (int64_t)1 << 22 ? 1024 : 512;
     const int64_t turn = (int64_t)m.P.R * 2, turns = div_up(m.P.rows, turn), groups = a.N * m.P.col_blocks;
     const int64_t most = MAP_MAX_SPAN / (turn * ((int64_t)a.C << m.P.q_log));              // turns of a workgroup, so that its offsets fit
-    const int64_t sum_turns = div_up(turns, groups >= MAP_BLOCKS ? 1 : div_up(MAP_BLOCKS, groups)), apply_turns = div_up(turns, groups >= MAP_APPLY_BLOCKS ? 1 : div_up(MAP_APPLY_BLOCKS, groups));
+    const int64_t sum_turns = div_up(turns, groups >= blocks ? 1 : div_up(blocks, groups)), apply_turns = div_up(turns, groups >= blocks ? 1 : div_up(blocks, groups));
     m.P.rows_per = (sum_turns < most ? sum_turns : most) * turn;
     m.P.splits = (int)div_up(m.P.rows, m.P.rows_per);
     m.P.apply_rows = (apply_turns < most ? apply_turns : most) * turn;
@@ -148,6 +146,7 @@ static MapLaunch map_plan(const PlenRegNorm &a) {
     m.param_rows = (int)(m.sums.x * (m.P.q_log ? m.sums.y : 1) * m.sums.z);
     z = div_up(8192, row_blocks);
     m.apply = dim3((unsigned)row_blocks, (unsigned)m.P.col_blocks, (unsigned)(a.N < z ? a.N : z));
+    m.stream = streams(a);
     m.stat_blocks = (unsigned)(a.N * a.G < 4 * 65536 ? div_up(a.N * a.G, 4) : 65536);
     return m;
 }

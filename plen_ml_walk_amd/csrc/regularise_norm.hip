@@ -49,17 +49,22 @@ __device__ __forceinline__ double2 finish_stats(const NormArgs &A, double s, dou
 __device__ __forceinline__ void write_used(const NormArgs &A) {
     if (A.used && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) { A.used[0] = A.rng[0]; A.used[1] = A.rng[1]; }
 }
-// a chunk's elements as floats; masked ones as zeros
-template <bool DROP, int E> __device__ __forceinline__ void unpack(const Chunk<E> &c, uint32_t kept_bits, float (&v)[8]) {
+// a chunk's elements as floats
+template <int E> __device__ __forceinline__ void unpack(const Chunk<E> &c, float (&v)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = !DROP || kept_bits >> e & 1u ? (float)c.v[e] : 0.f;
+    for (int e = 0; e < 8; e++) v[e] = c.get(e);
+}
+// ... masked ones as zeros
+template <int E, int M> __device__ __forceinline__ void unpack(const Chunk<E> &c, const Mask<M> &m, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = m.keep(e, c.get(e));
 }
 
 // ---- loads without branches.  A load under a condition waits for the ones before it, so every lane loads whole chunks from inside its row or slab of `size` elements, and
 //      what is not asked for is left out of the sums and not stored.  V = 0: the last chunk of a row may begin less than 8 elements before its end: then the 8 last elements are
 //      loaded and moved down.
-template <int V, int E> __device__ __forceinline__ Chunk<E> load_inside(const typename Elem<E>::T *p, int64_t off, int64_t size) {
-    if (V) return load_whole<E>(p + off);
+template <int V, int E, bool STREAM = false> __device__ __forceinline__ Chunk<E> load_inside(const typename Elem<E>::T *p, int64_t off, int64_t size) {
+    if (V) return STREAM ? stream_whole<E>(p + off) : load_whole<E>(p + off);
     if (size < 8) return load_chunk<E>(p + off, (int)(size - off));
     return load_whole<E>(p + (off < size - 8 ? off : size - 8));
 }
@@ -129,7 +134,7 @@ template <int NT, typename F> __device__ __forceinline__ void team_sum2(F &a, F 
 
 // ---- the pass back through the activation for one chunk of `valid` elements: xh and dy -> dz.  ReLU's gate: where 32 bits leave the sign of z open it is decided in
 // 64, from the inputs in memory (x of the chunk at px, statistics and parameters of channel (c0 + e) % C): the gradient jumps there.  xh is off by at most 4 roundings.
-template <bool DROP> __device__ __forceinline__ void back_activation(const NormArgs &A, const T *px, int64_t n, int c0, int valid, uint32_t kept_bits, const float (&xh)[8], const float (&dy)[8],
+template <int M> __device__ __forceinline__ void back_activation(const NormArgs &A, const T *px, int64_t n, int c0, int valid, const Mask<M> &mask, const float (&xh)[8], const float (&dy)[8],
                                                                              const float (&w)[8], const float (&b)[8], float (&dz)[8]) {
     if (A.act == PLENREG_ACT_RELU) {
         uint32_t open = 0, doubt = 0;
@@ -140,12 +145,13 @@ template <bool DROP> __device__ __forceinline__ void back_activation(const NormA
             doubt |= fabsf(z) <= 6e-7f * (fabsf(t) + fabsf(b[e])) ? 1u << e : 0u;
         }
         doubt &= (1u << valid) - 1u;
+        const uint32_t kept_bits = doubt ? mask.bits() : 0u;
 #pragma unroll 1
         while (doubt) {
             const int e = __ffs(doubt) - 1, c = (c0 + e) % A.C;
             doubt &= doubt - 1u;
             const double2 st = A.stats[n * A.G + c / A.D];
-            const double v = DROP && !(kept_bits >> e & 1u) ? 0.0 : (double)(float)px[e], wd = A.w ? (double)(float)((const W *)A.w)[c] : 1.0, bd = A.b ? (double)(float)((const W *)A.b)[c] : 0.0;
+            const double v = kept_bits >> e & 1u ? (double)(float)px[e] : 0.0, wd = A.w ? (double)(float)((const W *)A.w)[c] : 1.0, bd = A.b ? (double)(float)((const W *)A.b)[c] : 0.0;
             open = (v - st.x) * st.y * wd + bd > 0.0 ? open | 1u << e : open & ~(1u << e);
         }
 #pragma unroll
@@ -186,8 +192,9 @@ template <int K> __device__ __forceinline__ void row_chunks(const NormArgs &A, c
         c[k] = g * A.D + (left > 0 ? at : (A.D - 1) & ~7);
     }
 }
-template <int V> __device__ __forceinline__ void row_store(T *p, int valid, const float (&v)[8]) {
-    if (V) store_whole<DT>(p, v);
+template <int V, bool STREAM> __device__ __forceinline__ void row_store(T *p, int valid, const float (&v)[8]) {
+    if (V && STREAM) stream_store_whole<DT>(p, v);
+    else if (V) store_whole<DT>(p, v);
     else store_chunk<DT>(p, valid, v);
 }
 // parameters of a lane's chunk, 1 / 0 where there are none
@@ -195,7 +202,7 @@ template <int V> __device__ __forceinline__ void row_params(const NormArgs &A, c
     if (p) {
         const Chunk<WT> c = load_inside<V, WT>((const W *)p, c0, A.C);
 #pragma unroll
-        for (int e = 0; e < 8; e++) out[e] = (float)c.v[e];
+        for (int e = 0; e < 8; e++) out[e] = c.get(e);
         move_down<V>(out, c0, A.C);
     } else {
 #pragma unroll
@@ -203,7 +210,7 @@ template <int V> __device__ __forceinline__ void row_params(const NormArgs &A, c
     }
 }
 
-template <int V, int K, int NT, bool DROP> __global__ __launch_bounds__(NT) void k_row_forward(NormArgs A, RowPlan P) {
+template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT) void k_row_forward(NormArgs A, RowPlan P) {
     __shared__ double2 lds[2][NT / 64];
     const RowPlace p = row_place<NT>(A, P);
     int c[K], valid[K];
@@ -212,7 +219,7 @@ template <int V, int K, int NT, bool DROP> __global__ __launch_bounds__(NT) void
     const T *px = (const T *)A.x + (n < A.N ? n : A.N - 1) * A.x_stride;
     Chunk<DT> x[K];
 #pragma unroll
-    for (int k = 0; k < K; k++) x[k] = load_inside<V, DT>(px, c[k], A.C);
+    for (int k = 0; k < K; k++) x[k] = load_inside<V, DT, STREAM>(px, c[k], A.C);
     float w[K][8], b[K][8];
 #pragma unroll
     for (int k = 0; k < K; k++) { row_params<V>(A, A.w, c[k], 1.f, w[k]); row_params<V>(A, A.b, c[k], 0.f, b[k]); }
@@ -225,18 +232,16 @@ template <int V, int K, int NT, bool DROP> __global__ __launch_bounds__(NT) void
         float v[K][8];
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            unpack<false>(x[k], 255u, v[k]);
+            const Mask<DROP ? V + 1 : 0> m(d, n * A.C + c[k]);
+            unpack(x[k], v[k]);
             move_down<V>(v[k], c[k], A.C);
-            if (DROP) {
-                const uint32_t m = chunk_mask(d, n * A.C + c[k]);
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[k][e] = m >> e & 1u ? v[k][e] : 0.f;
-            }
+            for (int e = 0; e < 8; e++) v[k][e] = m.keep(e, v[k][e]);
         }
         if (turn + 1 < P.trips) {                               // the next row's, while this one is worked on
             px = (const T *)A.x + (next < A.N ? next : A.N - 1) * A.x_stride;
 #pragma unroll
-            for (int k = 0; k < K; k++) x[k] = load_inside<V, DT>(px, c[k], A.C);
+            for (int k = 0; k < K; k++) x[k] = load_inside<V, DT, STREAM>(px, c[k], A.C);
         }
         // s: the group's first element, after the mask
         float first;
@@ -268,7 +273,7 @@ template <int V, int K, int NT, bool DROP> __global__ __launch_bounds__(NT) void
 #pragma unroll
                 for (int e = 0; e < 8; e++) v[k][e] = ((v[k][e] - mean) - rest) * rstd * w[k][e] + b[k][e];
                 activate(v[k], A.act);
-                row_store<V>((T *)A.out + n * A.C + c[k], valid[k], v[k]);
+                row_store<V, STREAM>((T *)A.out + n * A.C + c[k], valid[k], v[k]);
             }
         }
         n = next;
@@ -276,7 +281,7 @@ template <int V, int K, int NT, bool DROP> __global__ __launch_bounds__(NT) void
 }
 
 // backward of the rows.  Each workgroup leaves one row of partial parameter gradients: part[blockIdx.x][0 / 1][C] = dw, db of its rows, summed over its teams in LDS.
-template <int V, int NT, bool DROP> __global__ __launch_bounds__(NT) void k_row_backward(NormArgs A, RowPlan P, float *part) {
+template <int V, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT) void k_row_backward(NormArgs A, RowPlan P, float *part) {
     __shared__ double2 lds[2][NT / 64];
     __shared__ float joined[NT * 8];
     const RowPlace p = row_place<NT>(A, P);
@@ -285,7 +290,7 @@ template <int V, int NT, bool DROP> __global__ __launch_bounds__(NT) void k_row_
     const int c0 = c[0], g0 = p.g < A.G ? p.g : A.G - 1;
     int64_t n = (int64_t)blockIdx.x * P.rb + p.row, row = n < A.N ? n : A.N - 1;
     const T *px = (const T *)A.x + row * A.x_stride;
-    Chunk<DT> x = load_inside<V, DT>(px, c0, A.C), g = load_inside<V, DT>((const T *)A.dy + row * A.dy_stride, c0, A.C);
+    Chunk<DT> x = load_inside<V, DT, STREAM>(px, c0, A.C), g = load_inside<V, DT, STREAM>((const T *)A.dy + row * A.dy_stride, c0, A.C);
     double2 st = A.stats[row * A.G + g0];
     float w[8], b[8], dw[8] = {}, db[8] = {};
     row_params<V>(A, A.w, c0, 1.f, w);
@@ -296,19 +301,18 @@ template <int V, int NT, bool DROP> __global__ __launch_bounds__(NT) void k_row_
     for (int turn = 0; turn < P.trips; turn++) {
         const bool on = n < A.N && valid[0];
         float xh[8] = {}, gw[8] = {}, s = 0.f, q = 0.f, rstd = 0.f;
-        uint32_t m = 255u;
+        const Mask<DROP ? V + 1 : 0> m(d, n * A.C + c0);
         if (on) {
-            if (DROP) m = chunk_mask(d, n * A.C + c0);
             const float mean = (float)st.x, rest = (float)(st.x - (double)mean);
             rstd = (float)st.y;
             float dy[8], dz[8];
-            unpack<false>(x, 255u, xh);
-            unpack<false>(g, 255u, dy);
+            unpack(x, xh);
+            unpack(g, dy);
             move_down<V>(xh, c0, A.C);
             move_down<V>(dy, c0, A.C);
 #pragma unroll
-            for (int e = 0; e < 8; e++) xh[e] = (((!DROP || m >> e & 1u ? xh[e] : 0.f) - mean) - rest) * rstd;
-            back_activation<DROP>(A, px + c0, n, c0, valid[0], m, xh, dy, w, b, dz);
+            for (int e = 0; e < 8; e++) xh[e] = ((m.keep(e, xh[e]) - mean) - rest) * rstd;
+            back_activation(A, px + c0, n, c0, valid[0], m, xh, dy, w, b, dz);
             if (!V) {
 #pragma unroll
                 for (int e = 0; e < 8; e++) dz[e] = e < valid[0] ? dz[e] : 0.f;
@@ -325,16 +329,15 @@ template <int V, int NT, bool DROP> __global__ __launch_bounds__(NT) void k_row_
             const float m1 = s * (float)A.inv_count, m2 = q * (float)A.inv_count;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float t = rstd * (gw[e] - m1 - xh[e] * m2);
-                gw[e] = !DROP || m >> e & 1u ? t : 0.f;
+                gw[e] = m.keep(e, rstd * (gw[e] - m1 - xh[e] * m2));
             }
-            row_store<V>((T *)A.out + n * A.C + c0, valid[0], gw);
+            row_store<V, STREAM>((T *)A.out + n * A.C + c0, valid[0], gw);
         }
         n += (int64_t)gridDim.x * P.rb;
         if (turn + 1 < P.trips) {
             row = n < A.N ? n : A.N - 1;
             px = (const T *)A.x + row * A.x_stride;
-            x = load_inside<V, DT>(px, c0, A.C); g = load_inside<V, DT>((const T *)A.dy + row * A.dy_stride, c0, A.C);
+            x = load_inside<V, DT, STREAM>(px, c0, A.C); g = load_inside<V, DT, STREAM>((const T *)A.dy + row * A.dy_stride, c0, A.C);
             st = A.stats[row * A.G + g0];
         }
     }
@@ -418,8 +421,11 @@ __device__ __forceinline__ Span my_span(const NormArgs &A, const MapPlan &P, con
     t.off = c.r * width + 8 * c.col;
     return t;
 }
-// the chunk at off, or the span's last whole one (a load under a condition would wait for the ones before it); lim >= 8
-__device__ __forceinline__ Chunk<DT> span_load(const T *p, const Span &t, int off) { return load_whole<DT>(p + (off < t.lim - 8 ? off : t.lim - 8)); }
+// the chunk at off, or the span's last whole one (a load under a condition would wait for the ones before it); lim >= 8.  STREAM: past the caches
+template <bool STREAM = false> __device__ __forceinline__ Chunk<DT> span_load(const T *p, const Span &t, int off) {
+    p += off < t.lim - 8 ? off : t.lim - 8;
+    return STREAM ? stream_whole<DT>(p) : load_whole<DT>(p);
+}
 
 // channel and group of the first of a thread's virtual channels; `next` steps to the one after
 struct Channel {
@@ -501,7 +507,7 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_sums(No
         double s[8] = {}, q[8] = {};
         const auto add = [&](const Chunk<DT> &chunk, int valid) {
             float f[8];
-            unpack<DROP>(chunk, DROP ? chunk_mask(d, n * A.size + t.base + off) : 255u, f);
+            unpack(chunk, Mask<DROP ? V : 0>(d, n * A.size + t.base + off), f);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const double u = e < valid ? (double)f[e] - shift : 0.0;
@@ -542,13 +548,16 @@ template <int V> __device__ __forceinline__ void load_constants(const NormArgs &
         row_params<1>(A, A.w, 8 * col, 1.f, k.w);
         row_params<1>(A, A.b, 8 * col, 0.f, k.b);
     } else {
-        Channel c = ch;
+        // (all loads of one kind under one condition: each would wait for the one before)
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            k.w[e] = A.w ? (float)((const W *)A.w)[c.c] : 1.f;
-            k.b[e] = A.b ? (float)((const W *)A.b)[c.c] : 0.f;
-            c.next(A);
-        }
+        for (int e = 0; e < 8; e++) { k.w[e] = 1.f; k.b[e] = 0.f; }
+        const auto gather = [&](const void *p, float (&out)[8]) {
+            int at = ch.c;
+#pragma unroll
+            for (int e = 0; e < 8; e++) { out[e] = (float)((const W *)p)[at]; at = at + 1 < A.C ? at + 1 : 0; }
+        };
+        if (A.w) gather(A.w, k.w);
+        if (A.b) gather(A.b, k.b);
     }
     const double2 st = stats[ch.g];
     const float mean = (float)st.x, rest = (float)(st.x - (double)mean), rstd = (float)st.y;
@@ -571,7 +580,7 @@ template <int V> __device__ __forceinline__ void normalise(const Constants<V> &k
 #pragma unroll
     for (int e = 0; e < 8; e++) { const int i = V == 2 ? 0 : e; v[e] = ((v[e] - k.mean[i]) - k.rest[i]) * k.rstd[i]; }
 }
-template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_apply(NormArgs A, MapPlan P) {
+template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(512) void k_map_apply(NormArgs A, MapPlan P) {
     const Column c = my_column(P, blockIdx.y);
     if (!c.mine) return;
     const Span t = my_span(A, P, c, P.apply_rows);
@@ -583,13 +592,13 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_apply(N
         T *y = (T *)A.out + n * A.size + t.base;
         int off = t.off;
         Chunk<DT> v;
-        if (t.lim >= 8) v = span_load(x, t, off);
+        if (t.lim >= 8) v = span_load<STREAM>(x, t, off);
         Constants<V> k;
         load_constants<V>(A, P, n, c.col, k);
 #pragma unroll
         for (int e = 0; e < 8; e++) k.w[e] *= k.rstd[V == 2 ? 0 : e];
         const auto result = [&](const Chunk<DT> &chunk, float (&f)[8]) {
-            unpack<DROP>(chunk, DROP ? chunk_mask(d, n * A.size + t.base + off) : 255u, f);
+            unpack(chunk, Mask<DROP ? V : 0>(d, n * A.size + t.base + off), f);
 #pragma unroll
             for (int e = 0; e < 8; e++) f[e] = ((f[e] - k.mean[V == 2 ? 0 : e]) - k.rest[V == 2 ? 0 : e]) * k.w[e] + k.b[e];
             activate(f, A.act);
@@ -598,9 +607,10 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_apply(N
 #pragma unroll 1
         while (off + 8 <= t.lim) {
             const Chunk<DT> now = v;
-            v = span_load(x, t, off + t.step);
+            v = span_load<STREAM>(x, t, off + t.step);
             result(now, f);
-            store_whole<DT>(y + off, f);
+            if (STREAM) stream_store_whole<DT>(y + off, f);
+            else store_whole<DT>(y + off, f);
             off += t.step;
         }
         if (V == 1 && off < t.lim) { result(load_chunk<DT>(x + off, t.lim - off), f); store_chunk<DT>(y + off, t.lim - off, f); }
@@ -626,12 +636,12 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_su
         Constants<V> k;
         load_constants<V>(A, P, n, c.col, k);
         const auto add = [&](const Chunk<DT> &cx, const Chunk<DT> &cg, int valid) {
-            const uint32_t m = DROP ? chunk_mask(d, n * A.size + t.base + off) : 255u;
+            const Mask<DROP ? V : 0> m(d, n * A.size + t.base + off);
             float xh[8], dv[8], dz[8];
-            unpack<DROP>(cx, m, xh);
-            unpack<false>(cg, 255u, dv);
+            unpack(cx, m, xh);
+            unpack(cg, dv);
             normalise<V>(k, xh);
-            back_activation<DROP>(A, x + off, n, 8 * c.col, valid, m, xh, dv, k.w, k.b, dz);
+            back_activation(A, x + off, n, 8 * c.col, valid, m, xh, dv, k.w, k.b, dz);
 #pragma unroll
             for (int e = 0; e < 8; e++) { s1[e] += (double)dz[e]; s2[e] += (double)(dz[e] * xh[e]); }
         };
@@ -693,7 +703,7 @@ __global__ __launch_bounds__(1024) void k_map_back_join(NormArgs A, int splits, 
         if ((threadIdx.x & 63) == 0) means[item] = float2{(float)(t.x * A.inv_count), (float)(t.y * A.inv_count)};
     }
 }
-template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_apply(NormArgs A, MapPlan P, const float2 *means) {
+template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(512) void k_map_back_apply(NormArgs A, MapPlan P, const float2 *means) {
     const Column c = my_column(P, blockIdx.y);
     if (!c.mine) return;
     const Span t = my_span(A, P, c, P.apply_rows);
@@ -705,7 +715,7 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_ap
         T *dx = (T *)A.out + n * A.size + t.base;
         int off = t.off;
         Chunk<DT> v, g;
-        if (t.lim >= 8) { v = span_load(x, t, off); g = span_load(dy, t, off); }
+        if (t.lim >= 8) { v = span_load<STREAM>(x, t, off); g = span_load<STREAM>(dy, t, off); }
         Constants<V> k;
         load_constants<V>(A, P, n, c.col, k);
         float m1[V == 2 ? 1 : 8], m2[V == 2 ? 1 : 8];
@@ -715,26 +725,26 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_ap
             for (int e = 0; e < (V == 2 ? 1 : 8); e++) { const float2 m = means[n * A.G + ch.g]; m1[e] = m.x; m2[e] = m.y; ch.next(A); }
         }
         const auto result = [&](const Chunk<DT> &cx, const Chunk<DT> &cg, int valid, float (&dz)[8]) {
-            const uint32_t m = DROP ? chunk_mask(d, n * A.size + t.base + off) : 255u;
+            const Mask<DROP ? V : 0> m(d, n * A.size + t.base + off);
             float xh[8], dv[8];
-            unpack<DROP>(cx, m, xh);
-            unpack<false>(cg, 255u, dv);
+            unpack(cx, m, xh);
+            unpack(cg, dv);
             normalise<V>(k, xh);
-            back_activation<DROP>(A, x + off, n, 8 * c.col, valid, m, xh, dv, k.w, k.b, dz);
+            back_activation(A, x + off, n, 8 * c.col, valid, m, xh, dv, k.w, k.b, dz);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const int i = V == 2 ? 0 : e;
-                const float r = k.rstd[i] * (dz[e] * k.w[e] - m1[i] - xh[e] * m2[i]);
-                dz[e] = !DROP || m >> e & 1u ? r : 0.f;
+                dz[e] = m.keep(e, k.rstd[i] * (dz[e] * k.w[e] - m1[i] - xh[e] * m2[i]));
             }
         };
         float f[8];
 #pragma unroll 1
         while (off + 8 <= t.lim) {
             const Chunk<DT> now = v, gnow = g;
-            v = span_load(x, t, off + t.step); g = span_load(dy, t, off + t.step);
+            v = span_load<STREAM>(x, t, off + t.step); g = span_load<STREAM>(dy, t, off + t.step);
             result(now, gnow, 8, f);
-            store_whole<DT>(dx + off, f);
+            if (STREAM) stream_store_whole<DT>(dx + off, f);
+            else store_whole<DT>(dx + off, f);
             off += t.step;
         }
         if (V == 1 && off < t.lim) {
@@ -745,19 +755,23 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_ap
 }
 
 // ---- launches
-template <int V, bool DROP> void row_forward_v(const NormArgs &a, const RowLaunch &r, hipStream_t s) {
-    if (r.K == 1) k_row_forward<V, 1, 256, DROP><<<r.grid, 256, 0, s>>>(a, r.P);
-    else if (r.K == 2) k_row_forward<V, 2, 256, DROP><<<r.grid, 256, 0, s>>>(a, r.P);
-    else k_row_forward<V, 4, 256, DROP><<<r.grid, 256, 0, s>>>(a, r.P);
+template <int V, bool DROP, bool STREAM> void row_forward_v(const NormArgs &a, const RowLaunch &r, hipStream_t s) {
+    if (r.K == 1) k_row_forward<V, 1, 256, DROP, STREAM><<<r.grid, 256, 0, s>>>(a, r.P);
+    else if (r.K == 2) k_row_forward<V, 2, 256, DROP, STREAM><<<r.grid, 256, 0, s>>>(a, r.P);
+    else k_row_forward<V, 4, 256, DROP, STREAM><<<r.grid, 256, 0, s>>>(a, r.P);
 }
 void row_forward(const NormArgs &a, const RowLaunch &r, hipStream_t s) {
-    if (a.D % 8) a.cut ? row_forward_v<0, true>(a, r, s) : row_forward_v<0, false>(a, r, s);
-    else a.cut ? row_forward_v<1, true>(a, r, s) : row_forward_v<1, false>(a, r, s);
+    if (a.D % 8) a.cut ? row_forward_v<0, true, false>(a, r, s) : row_forward_v<0, false, false>(a, r, s);
+    else if (r.stream) a.cut ? row_forward_v<1, true, true>(a, r, s) : row_forward_v<1, false, true>(a, r, s);
+    else a.cut ? row_forward_v<1, true, false>(a, r, s) : row_forward_v<1, false, false>(a, r, s);
 }
-template <int V, bool DROP> void row_backward_v(const NormArgs &a, const RowLaunch &r, float *part, hipStream_t s) { k_row_backward<V, 512, DROP><<<r.grid, 512, 0, s>>>(a, r.P, part); }
+template <int V, bool DROP, bool STREAM> void row_backward_v(const NormArgs &a, const RowLaunch &r, float *part, hipStream_t s) {
+    k_row_backward<V, 512, DROP, STREAM><<<r.grid, 512, 0, s>>>(a, r.P, part);
+}
 void row_backward(const NormArgs &a, const RowLaunch &r, float *part, hipStream_t s) {
-    if (a.D % 8) a.cut ? row_backward_v<0, true>(a, r, part, s) : row_backward_v<0, false>(a, r, part, s);
-    else a.cut ? row_backward_v<1, true>(a, r, part, s) : row_backward_v<1, false>(a, r, part, s);
+    if (a.D % 8) a.cut ? row_backward_v<0, true, false>(a, r, part, s) : row_backward_v<0, false, false>(a, r, part, s);
+    else if (r.stream) a.cut ? row_backward_v<1, true, true>(a, r, part, s) : row_backward_v<1, false, true>(a, r, part, s);
+    else a.cut ? row_backward_v<1, true, false>(a, r, part, s) : row_backward_v<1, false, false>(a, r, part, s);
 }
 unsigned column_blocks(const NormArgs &a) { return (unsigned)((2 * (int64_t)a.C + 15) / 16); }
 void params(const NormArgs &a, const float *part, int rows, void *dw, void *db, hipStream_t s) { k_row_params<<<column_blocks(a), 1024, 0, s>>>(a, part, rows, dw, db); }
@@ -766,7 +780,8 @@ bool one_group(const NormArgs &a) { return a.C % 8 == 0 && a.D % 8 == 0; }
 template <int V, bool DROP> void map_forward_v(const NormArgs &a, const MapLaunch &m, double2 *part, hipStream_t s) {
     k_map_sums<V, DROP><<<m.sums, m.NT, (size_t)m.NT * (V == 2 ? 16 : 128), s>>>(a, m.P, part);
     k_map_stats<DROP><<<m.stat_blocks, 256, 0, s>>>(a, m.P.splits * m.P.col_blocks, part);
-    k_map_apply<V, DROP><<<m.apply, m.NT, 0, s>>>(a, m.P);
+    if (m.stream) k_map_apply<V, DROP, true><<<m.apply, m.NT, 0, s>>>(a, m.P);
+    else k_map_apply<V, DROP, false><<<m.apply, m.NT, 0, s>>>(a, m.P);
 }
 void map_forward(const NormArgs &a, const MapLaunch &m, double2 *part, hipStream_t s) {
     if (one_group(a)) a.cut ? map_forward_v<2, true>(a, m, part, s) : map_forward_v<2, false>(a, m, part, s);
@@ -777,7 +792,8 @@ template <int V, bool DROP> void map_backward_v(const NormArgs &a, const MapLaun
     const int64_t items = a.N * a.G;
     const int join = (int)(items < 16 * 4096 ? (items + 15) / 16 : 4096);
     k_map_back_join<<<join + (sums ? column_blocks(a) : 0), 1024, 0, s>>>(a, m.P.splits * m.P.col_blocks, part, sums, m.param_rows, join, means, dw, db);
-    k_map_back_apply<V, DROP><<<m.apply, m.NT, 0, s>>>(a, m.P, means);
+    if (m.stream) k_map_back_apply<V, DROP, true><<<m.apply, m.NT, 0, s>>>(a, m.P, means);
+    else k_map_back_apply<V, DROP, false><<<m.apply, m.NT, 0, s>>>(a, m.P, means);
 }
 void map_backward(const NormArgs &a, const MapLaunch &m, double2 *part, float2 *means, float *sums, void *dw, void *db, hipStream_t s) {
     if (one_group(a)) a.cut ? map_backward_v<2, true>(a, m, part, means, sums, dw, db, s) : map_backward_v<2, false>(a, m, part, means, sums, dw, db, s);
