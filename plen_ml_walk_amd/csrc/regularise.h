@@ -184,14 +184,15 @@ struct RowLaunch { RowPlan P; int K, NT; dim3 grid; bool stream; };
 // many positions.  A slab as `rows` rows of `ncol` chunk columns (2^q_log positions to a row); bcol columns in a workgroup, R rows per turn of it; rows_per rows in a
 // workgroup of the sums, apply_rows in one of the result; 2^lanes_log lanes join one group
 struct MapPlan { int q_log, ncol, bcol, col_blocks, R, splits, lanes_log; int64_t rows, rows_per, apply_rows; float inv_bcol; };
-struct MapLaunch { MapPlan P; dim3 sums, apply; int NT, param_rows; unsigned stat_blocks; bool stream; };
+// slab: one workgroup does a slab by itself (the grid is `sums`, slabs along y)
+struct MapLaunch { MapPlan P; dim3 sums, apply; int NT, param_rows; unsigned stat_blocks; bool stream, slab; };
 
 // one per pair of element types (x and results, parameters), in regularise_norm.hip
 struct NormEntry {
     void (*row_forward)(const NormArgs &, const RowLaunch &, hipStream_t);
     void (*row_backward)(const NormArgs &, const RowLaunch &, float *part, hipStream_t);
     void (*map_forward)(const NormArgs &, const MapLaunch &, double2 *part, hipStream_t);
-    void (*map_backward)(const NormArgs &, const MapLaunch &, double2 *part, float2 *means, float *params, void *dw, void *db, hipStream_t);
+    void (*map_backward)(const NormArgs &, const MapLaunch &, double2 *part, double2 *means, float *params, void *dw, void *db, hipStream_t);
     void (*params)(const NormArgs &, const float *part, int rows, void *dw, void *db, hipStream_t);
 };
 const NormEntry &plenreg_norm_f32_f32();

@@ -6,6 +6,10 @@
 #ifndef STREAM_BYTES
 #define STREAM_BYTES ((int64_t)64 << 20)
 #endif
+#ifndef SLAB_ANY
+#define SLAB_ANY 32768
+#define SLAB_MANY 131072
+#endif
 #define MAP_MAX_SPAN ((int64_t)1 << 28)      // elements of a slab that one workgroup walks over
 #define ROW_MAX_FORWARD 8192            // widest group that the lanes of one workgroup hold: 256 lanes of 4 chunks, or in the backward pass (which holds four times as much) 512 of one
 #define ROW_MAX_BACKWARD 4096
@@ -125,7 +129,10 @@ static MapLaunch map_plan(const PlenRegNorm &a) {
     m.P.col_blocks = (int)div_up(m.P.ncol, 512);
     m.P.bcol = (int)div_up(m.P.ncol, m.P.col_blocks);
     m.P.inv_bcol = 1.f / (float)m.P.bcol;
-    m.NT = fill_threads(m.P.bcol, 256, 512);
+    // one workgroup per slab: no more launches than one, and the slab is read once from memory; but only as many compute units work as there are slabs
+    m.slab = m.P.bcol <= 448 && m.P.col_blocks == 1 && a.G <= 512 && (size <= SLAB_ANY || (size <= SLAB_MANY && a.N >= 128));
+    const int64_t threads = div_up(chunks, 64) * 64;
+    m.NT = m.slab ? fill_threads(m.P.bcol, threads < 448 ? (int)threads : 448, 448) : fill_threads(m.P.bcol, 256, 512);
     m.P.R = m.NT / m.P.bcol;
     // 2 workgroups per compute unit, or 4 where their threads then still have 16 chunks each; each thread in whole turns of 2 rows.  (8 x 4096 x 320: 512 workgroups 9.2 + 9.5 us,
     // 1024: 10.8 + 9.8; 2 x 262144 x 128: 47 + 42 and 40 + 43)
@@ -146,6 +153,11 @@ static MapLaunch map_plan(const PlenRegNorm &a) {
     m.param_rows = (int)(m.sums.x * (m.P.q_log ? m.sums.y : 1) * m.sums.z);
     z = div_up(8192, row_blocks);
     m.apply = dim3((unsigned)row_blocks, (unsigned)m.P.col_blocks, (unsigned)(a.N < z ? a.N : z));
+    if (m.slab) {
+        m.P.rows_per = m.P.rows; m.P.splits = 1;
+        m.sums = dim3(1, (unsigned)(a.N < 2048 ? a.N : 2048), 1);
+        m.param_rows = (int)m.sums.y;
+    }
     m.stream = streams(a);
     m.stat_blocks = (unsigned)(a.N * a.G < 4 * 65536 ? div_up(a.N * a.G, 4) : 65536);
     return m;
@@ -194,7 +206,8 @@ int64_t plenreg_norm_workspace(const PlenRegNorm *a, int backward) {
     if (bad_norm(a)) return PLENREG_REFUSE;
     if (by_rows(*a, backward)) return backward ? (int64_t)row_plan(*a, true).grid.x * 2 * a->C * 4 : 0;
     const MapLaunch m = map_plan(*a);
-    return part_bytes(*a, m) + (backward ? a->N * a->G * 8 + (int64_t)m.param_rows * 2 * a->C * 4 : a->N * a->G * 16);
+    if (m.slab) return backward ? (int64_t)m.param_rows * 2 * a->C * 4 : 0;
+    return part_bytes(*a, m) + a->N * a->G * 16 + (backward ? (int64_t)m.param_rows * 2 * a->C * 4 : 0);
 }
 
 int plenreg_norm_forward(const PlenRegNorm *a, void *stream) {
@@ -204,9 +217,9 @@ int plenreg_norm_forward(const PlenRegNorm *a, void *stream) {
         entry(*a).row_forward(k, row_plan(*a, false), (hipStream_t)stream);
         return launched();
     }
-    if (!a->ws) return PLENREG_REFUSE;
     const MapLaunch m = map_plan(*a);
-    if (!k.stats) k.stats = (double2 *)((char *)a->ws + part_bytes(*a, m));
+    if (!a->ws && !m.slab) return PLENREG_REFUSE;
+    if (!k.stats && !m.slab) k.stats = (double2 *)((char *)a->ws + part_bytes(*a, m));
     entry(*a).map_forward(k, m, (double2 *)a->ws, (hipStream_t)stream);
     return launched();
 }
@@ -214,7 +227,7 @@ int plenreg_norm_forward(const PlenRegNorm *a, void *stream) {
 int plenreg_norm_backward(const PlenRegNorm *a, void *stream) {
     if (bad_norm(a) || !a->x || !a->dy || !a->out || !a->stats || a->x_stride < 0 || a->dy_stride < 0 || (a->cut && !a->rng)) return PLENREG_REFUSE;
     const bool params = a->dw || a->db, rows = by_rows(*a, true);
-    if ((params || !rows) && !a->ws) return PLENREG_REFUSE;
+    if (plenreg_norm_workspace(a, 1) > 0 && (params || !rows) && !a->ws) return PLENREG_REFUSE;
     const NormArgs k = kernel_args(*a);
     const NormEntry &e = entry(*a);
     if (rows) {
@@ -225,8 +238,9 @@ int plenreg_norm_backward(const PlenRegNorm *a, void *stream) {
     }
     const MapLaunch m = map_plan(*a);
     char *ws = (char *)a->ws;
-    float2 *means = (float2 *)(ws + part_bytes(*a, m));
-    e.map_backward(k, m, (double2 *)ws, means, params ? (float *)(means + a->N * a->G) : nullptr, a->dw, a->db, (hipStream_t)stream);
+    double2 *means = (double2 *)(ws + part_bytes(*a, m));
+    float *sums = !params ? nullptr : m.slab ? (float *)ws : (float *)(means + a->N * a->G);
+    e.map_backward(k, m, (double2 *)ws, means, sums, a->dw, a->db, (hipStream_t)stream);
     return launched();
 }
 

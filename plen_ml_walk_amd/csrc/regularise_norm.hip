@@ -490,6 +490,32 @@ template <bool DROP> __device__ __forceinline__ double slab_shift(const NormArgs
     return DROP && !kept(d, n * A.size) ? 0.0 : (double)v;
 }
 
+// s, q += the sums of (x - s), (x - s)^2 of a span of slab n, per virtual channel
+template <int V, bool DROP> __device__ __forceinline__ void span_sums(const NormArgs &A, const Draw &d, const Column &c, const Span &t, int64_t n, double (&s)[8], double (&q)[8]) {
+    const T *x = (const T *)A.x + n * A.x_stride + t.base;
+    int off = t.off;
+    Chunk<DT> v;
+    if (t.lim >= 8) v = span_load(x, t, off);
+    const double shift = slab_shift<DROP>(A, d, n);
+    const auto add = [&](const Chunk<DT> &chunk, int valid) {
+        float f[8];
+        unpack(chunk, Mask<DROP ? V : 0>(d, n * A.size + t.base + off), f);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const double u = e < valid ? (double)f[e] - shift : 0.0;
+            s[e] += u; q[e] = fma(u, u, q[e]);
+        }
+    };
+    if (!c.mine) return;
+#pragma unroll 1
+    while (off + 8 <= t.lim) {
+        const Chunk<DT> now = v;
+        v = span_load(x, t, off + t.step);             // the next chunk is on its way while this one is added
+        add(now, 8);
+        off += t.step;
+    }
+    if (V == 1 && off < t.lim) add(load_chunk<DT>(x + off, t.lim - off), t.lim - off);
+}
 // part[n][g][split][column block] = sums of (x - s), (x - s)^2.  Grid: splits, column blocks, slabs.
 template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_sums(NormArgs A, MapPlan P, double2 *part) {
     extern __shared__ double2 lds[];
@@ -499,31 +525,8 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_sums(No
     if (DROP) { d = make_draw(A.rng, A.site, A.cut); write_used(A); }
 #pragma unroll 1
     for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) {
-        const T *x = (const T *)A.x + n * A.x_stride + t.base;
-        int off = t.off;
-        Chunk<DT> v;
-        if (t.lim >= 8) v = span_load(x, t, off);
-        const double shift = slab_shift<DROP>(A, d, n);
         double s[8] = {}, q[8] = {};
-        const auto add = [&](const Chunk<DT> &chunk, int valid) {
-            float f[8];
-            unpack(chunk, Mask<DROP ? V : 0>(d, n * A.size + t.base + off), f);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const double u = e < valid ? (double)f[e] - shift : 0.0;
-                s[e] += u; q[e] = fma(u, u, q[e]);
-            }
-        };
-        if (c.mine) {
-#pragma unroll 1
-            while (off + 8 <= t.lim) {
-                const Chunk<DT> now = v;
-                v = span_load(x, t, off + t.step);             // the next chunk is on its way while this one is added
-                add(now, 8);
-                off += t.step;
-            }
-            if (V == 1 && off < t.lim) add(load_chunk<DT>(x + off, t.lim - off), t.lim - off);
-        }
+        span_sums<V, DROP>(A, d, c, t, n, s, q);
         const int64_t parts = (int64_t)P.splits * P.col_blocks;
         join_groups<V>(s, q, A, P, c, lds, part + n * A.G * parts + blockIdx.x * P.col_blocks + blockIdx.y, parts);
     }
@@ -540,10 +543,9 @@ template <bool DROP> __global__ __launch_bounds__(256) void k_map_stats(NormArgs
 // statistics and parameters of a thread's 8 virtual channels (V = 2: one group, statistics in element 0).
 // (The column is hidden from the compiler: it would keep every address of a loop over slabs in registers, and spill.)
 template <int V> struct Constants { float mean[V == 2 ? 1 : 8], rest[V == 2 ? 1 : 8], rstd[V == 2 ? 1 : 8], w[8], b[8]; };
-template <int V> __device__ __forceinline__ void load_constants(const NormArgs &A, const MapPlan &P, int64_t n, int col, Constants<V> &k) {
+template <int V> __device__ __forceinline__ void load_constants(const NormArgs &A, const MapPlan &P, const double2 *stats, int col, Constants<V> &k) {
     asm volatile("" : "+v"(col));
     Channel ch(A, 8 * col);
-    const double2 *stats = A.stats + n * A.G;
     if (P.q_log == 0) {                         // (columns do not wrap: the parameters as whole chunks)
         row_params<1>(A, A.w, 8 * col, 1.f, k.w);
         row_params<1>(A, A.b, 8 * col, 0.f, k.b);
@@ -580,113 +582,118 @@ template <int V> __device__ __forceinline__ void normalise(const Constants<V> &k
 #pragma unroll
     for (int e = 0; e < 8; e++) { const int i = V == 2 ? 0 : e; v[e] = ((v[e] - k.mean[i]) - k.rest[i]) * k.rstd[i]; }
 }
+// the results of a span of slab n, with the slab's statistics at `stats`
+template <int V, bool DROP, bool STREAM> __device__ __forceinline__ void span_apply(const NormArgs &A, const MapPlan &P, const Draw &d, const Column &c, const Span &t, int64_t n, const double2 *stats) {
+    const T *x = (const T *)A.x + n * A.x_stride + t.base;
+    T *y = (T *)A.out + n * A.size + t.base;
+    int off = t.off;
+    Chunk<DT> v;
+    if (t.lim >= 8) v = span_load<STREAM>(x, t, off);
+    Constants<V> k;
+    load_constants<V>(A, P, stats, c.col, k);
+#pragma unroll
+    for (int e = 0; e < 8; e++) k.w[e] *= k.rstd[V == 2 ? 0 : e];
+    const auto result = [&](const Chunk<DT> &chunk, float (&f)[8]) {
+        unpack(chunk, Mask<DROP ? V : 0>(d, n * A.size + t.base + off), f);
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[e] = ((f[e] - k.mean[V == 2 ? 0 : e]) - k.rest[V == 2 ? 0 : e]) * k.w[e] + k.b[e];
+        activate(f, A.act);
+    };
+    float f[8];
+    if (!c.mine) return;
+#pragma unroll 1
+    while (off + 8 <= t.lim) {
+        const Chunk<DT> now = v;
+        v = span_load<STREAM>(x, t, off + t.step);
+        result(now, f);
+        if (STREAM) stream_store_whole<DT>(y + off, f);
+        else store_whole<DT>(y + off, f);
+        off += t.step;
+    }
+    if (V == 1 && off < t.lim) { result(load_chunk<DT>(x + off, t.lim - off), f); store_chunk<DT>(y + off, t.lim - off, f); }
+}
 template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(512) void k_map_apply(NormArgs A, MapPlan P) {
     const Column c = my_column(P, blockIdx.y);
-    if (!c.mine) return;
     const Span t = my_span(A, P, c, P.apply_rows);
     Draw d = {};
     if (DROP) d = make_draw(A.rng, A.site, A.cut);
 #pragma unroll 1
-    for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) {
-        const T *x = (const T *)A.x + n * A.x_stride + t.base;
-        T *y = (T *)A.out + n * A.size + t.base;
-        int off = t.off;
-        Chunk<DT> v;
-        if (t.lim >= 8) v = span_load<STREAM>(x, t, off);
-        Constants<V> k;
-        load_constants<V>(A, P, n, c.col, k);
-#pragma unroll
-        for (int e = 0; e < 8; e++) k.w[e] *= k.rstd[V == 2 ? 0 : e];
-        const auto result = [&](const Chunk<DT> &chunk, float (&f)[8]) {
-            unpack(chunk, Mask<DROP ? V : 0>(d, n * A.size + t.base + off), f);
-#pragma unroll
-            for (int e = 0; e < 8; e++) f[e] = ((f[e] - k.mean[V == 2 ? 0 : e]) - k.rest[V == 2 ? 0 : e]) * k.w[e] + k.b[e];
-            activate(f, A.act);
-        };
-        float f[8];
-#pragma unroll 1
-        while (off + 8 <= t.lim) {
-            const Chunk<DT> now = v;
-            v = span_load<STREAM>(x, t, off + t.step);
-            result(now, f);
-            if (STREAM) stream_store_whole<DT>(y + off, f);
-            else store_whole<DT>(y + off, f);
-            off += t.step;
-        }
-        if (V == 1 && off < t.lim) { result(load_chunk<DT>(x + off, t.lim - off), f); store_chunk<DT>(y + off, t.lim - off, f); }
-    }
+    for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) span_apply<V, DROP, STREAM>(A, P, d, c, t, n, A.stats + n * A.G);
 }
 
-// backward, first launch: per workgroup the channel sums of dz xh and dz (params[workgroup][2][C]), per split their w-weighted group sums (part[n][g][split][column block]
-// = sum w dz, sum w dz xh), in 64 bits.
+// backward: s1, s2 += the sums of dz and dz xh of a span of slab n, per virtual channel; k: the thread's constants, left for the caller
+template <int V, bool DROP> __device__ __forceinline__ void span_back_sums(const NormArgs &A, const MapPlan &P, const Draw &d, const Column &c, const Span &t, int64_t n, Constants<V> &k, double (&s1)[8],
+                                                                           double (&s2)[8]) {
+    const T *x = (const T *)A.x + n * A.x_stride + t.base, *dy = (const T *)A.dy + n * A.dy_stride + t.base;
+    int off = t.off;
+    Chunk<DT> v, g;
+    if (t.lim >= 8) { v = span_load(x, t, off); g = span_load(dy, t, off); }
+    load_constants<V>(A, P, A.stats + n * A.G, c.col, k);
+    const auto add = [&](const Chunk<DT> &cx, const Chunk<DT> &cg, int valid) {
+        const Mask<DROP ? V : 0> m(d, n * A.size + t.base + off);
+        float xh[8], dv[8], dz[8];
+        unpack(cx, m, xh);
+        unpack(cg, dv);
+        normalise<V>(k, xh);
+        back_activation(A, x + off, n, 8 * c.col, valid, m, xh, dv, k.w, k.b, dz);
+#pragma unroll
+        for (int e = 0; e < 8; e++) { s1[e] += (double)dz[e]; s2[e] += (double)(dz[e] * xh[e]); }
+    };
+    if (!c.mine) return;
+#pragma unroll 1
+    while (off + 8 <= t.lim) {
+        const Chunk<DT> now = v, gnow = g;
+        v = span_load(x, t, off + t.step); g = span_load(dy, t, off + t.step);
+        add(now, gnow, 8);
+        off += t.step;
+    }
+    // (of the part's other elements dy is zero)
+    if (V == 1 && off < t.lim) add(load_chunk<DT>(x + off, t.lim - off), load_chunk<DT>(dy + off, t.lim - off), t.lim - off);
+}
+// the workgroup's channel sums into `to`[0 / 1][C] = sums of dz xh, dz: written the first time, then added to (each thread to its own words)
+__device__ __forceinline__ void channel_sums(const double (&s1)[8], const double (&s2)[8], const NormArgs &A, const MapPlan &P, const Column &c, double2 *lds, float *to, bool first_time) {
+    const int NT = blockDim.x, lane = threadIdx.x & 7;
+    __syncthreads();
+    if (c.mine)
+#pragma unroll
+        for (int e = 0; e < 8; e++) lds[e * NT + c.r * P.bcol + c.col - c.first] = double2{s2[e], s1[e]};
+    __syncthreads();
+    const int from = P.q_log ? 0 : 8 * c.first, last = P.q_log || 8 * (c.first + P.bcol) > A.C ? A.C : 8 * (c.first + P.bcol);
+#pragma unroll 1
+    for (int c8 = from; c8 < last; c8 += NT >> 3) {
+        const int ch = c8 + (threadIdx.x >> 3);
+        double s = 0.0, q = 0.0;
+        if (ch < last)
+            for (int i = lane; i < P.R << P.q_log; i += 8) {
+                const int r = i >> P.q_log, vc = (i - (r << P.q_log)) * A.C + ch, col = (vc >> 3) - c.first;
+                if (col < 0 || col >= P.bcol || col + c.first >= P.ncol) continue;
+                const double2 v = lds[(vc & 7) * NT + r * P.bcol + col];
+                s += v.x; q += v.y;
+            }
+        lanes_sum2(s, q, 3);
+        if (ch < last && lane < 2) {
+            float *word = to + lane * (int64_t)A.C + ch;
+            const float v = (float)(lane ? q : s);
+            *word = first_time ? v : *word + v;
+        }
+    }
+}
+// first launch: per workgroup the channel sums (params[workgroup][2][C]), per split their w-weighted group sums (part[n][g][split][column block] = sum w dz, sum w dz xh), in 64
+// bits.
 template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_sums(NormArgs A, MapPlan P, double2 *part, float *params) {
     extern __shared__ double2 lds[];
     const Column c = my_column(P, blockIdx.y);
     const Span t = my_span(A, P, c, P.rows_per);
-    const int NT = blockDim.x;
+    // (column blocks of one position each have channels of their own, of several positions they share them)
+    const int64_t row = P.q_log ? (int64_t)blockIdx.z * gridDim.y + blockIdx.y : blockIdx.z;
     Draw d = {};
     if (DROP) d = make_draw(A.rng, A.site, A.cut);
 #pragma unroll 1
     for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) {
-        const T *x = (const T *)A.x + n * A.x_stride + t.base, *dy = (const T *)A.dy + n * A.dy_stride + t.base;
-        int off = t.off;
-        Chunk<DT> v, g;
-        if (t.lim >= 8) { v = span_load(x, t, off); g = span_load(dy, t, off); }
         double s1[8] = {}, s2[8] = {};
         Constants<V> k;
-        load_constants<V>(A, P, n, c.col, k);
-        const auto add = [&](const Chunk<DT> &cx, const Chunk<DT> &cg, int valid) {
-            const Mask<DROP ? V : 0> m(d, n * A.size + t.base + off);
-            float xh[8], dv[8], dz[8];
-            unpack(cx, m, xh);
-            unpack(cg, dv);
-            normalise<V>(k, xh);
-            back_activation(A, x + off, n, 8 * c.col, valid, m, xh, dv, k.w, k.b, dz);
-#pragma unroll
-            for (int e = 0; e < 8; e++) { s1[e] += (double)dz[e]; s2[e] += (double)(dz[e] * xh[e]); }
-        };
-        if (c.mine) {
-#pragma unroll 1
-            while (off + 8 <= t.lim) {
-                const Chunk<DT> now = v, gnow = g;
-                v = span_load(x, t, off + t.step); g = span_load(dy, t, off + t.step);
-                add(now, gnow, 8);
-                off += t.step;
-            }
-            // (of the part's other elements dy is zero)
-            if (V == 1 && off < t.lim) add(load_chunk<DT>(x + off, t.lim - off), load_chunk<DT>(dy + off, t.lim - off), t.lim - off);
-        }
-        if (params) {
-            // channel by channel over the workgroup's threads: a few lanes per channel where channels are few
-            __syncthreads();
-            if (c.mine)
-#pragma unroll
-                for (int e = 0; e < 8; e++) lds[e * NT + c.r * P.bcol + c.col - c.first] = double2{s2[e], s1[e]};
-            __syncthreads();
-            // (column blocks of one position each have channels of their own, of several positions they share them)
-            const int64_t row = P.q_log ? (int64_t)blockIdx.z * gridDim.y + blockIdx.y : blockIdx.z;
-            float *to = params + (row * gridDim.x + blockIdx.x) * 2 * A.C;
-            const int lane = threadIdx.x & 7;
-            const int from = P.q_log ? 0 : 8 * c.first, last = P.q_log || 8 * (c.first + P.bcol) > A.C ? A.C : 8 * (c.first + P.bcol);
-#pragma unroll 1
-            for (int c8 = from; c8 < last; c8 += NT >> 3) {
-                const int ch = c8 + (threadIdx.x >> 3);
-                double s = 0.0, q = 0.0;
-                if (ch < last)
-                    for (int i = lane; i < P.R << P.q_log; i += 8) {
-                        const int r = i >> P.q_log, vc = (i - (r << P.q_log)) * A.C + ch, col = (vc >> 3) - c.first;
-                        if (col < 0 || col >= P.bcol || col + c.first >= P.ncol) continue;
-                        const double2 v = lds[(vc & 7) * NT + r * P.bcol + col];
-                        s += v.x; q += v.y;
-                    }
-                lanes_sum2(s, q, 3);
-                if (ch < last && lane < 2) {
-                    float *word = to + lane * (int64_t)A.C + ch;              // (this thread's own word: later slabs of the workgroup add to it)
-                    const float v = (float)(lane ? q : s);
-                    *word = n == blockIdx.z ? v : *word + v;
-                }
-            }
-        }
+        span_back_sums<V, DROP>(A, P, d, c, t, n, k, s1, s2);
+        if (params) channel_sums(s1, s2, A, P, c, lds, params + (row * gridDim.x + blockIdx.x) * 2 * A.C, n == blockIdx.z);
         if (c.mine)
 #pragma unroll
             for (int e = 0; e < 8; e++) { s1[e] *= (double)k.w[e]; s2[e] *= (double)k.w[e]; }
@@ -695,62 +702,111 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_su
     }
 }
 // second launch: the first workgroups join the splits of each (n, g) into {mean of w dz, mean of w dz xh}, the others the parameter gradients
-__global__ __launch_bounds__(1024) void k_map_back_join(NormArgs A, int splits, const double2 *part, const float *params, int param_rows, int join_blocks, float2 *means, void *dw, void *db) {
+__global__ __launch_bounds__(1024) void k_map_back_join(NormArgs A, int splits, const double2 *part, const float *params, int param_rows, int join_blocks, double2 *means, void *dw, void *db) {
     __shared__ double lds[64][17];
     if ((int)blockIdx.x >= join_blocks) { param_columns(A, params, param_rows, blockIdx.x - join_blocks, dw, db, lds); return; }
     for (int64_t item = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 6); item < A.N * A.G; item += (int64_t)join_blocks * 16) {
         const double2 t = join_splits(part + item * splits, splits);
-        if ((threadIdx.x & 63) == 0) means[item] = float2{(float)(t.x * A.inv_count), (float)(t.y * A.inv_count)};
+        if ((threadIdx.x & 63) == 0) means[item] = double2{t.x * A.inv_count, t.y * A.inv_count};
     }
 }
-template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(512) void k_map_back_apply(NormArgs A, MapPlan P, const float2 *means) {
-    const Column c = my_column(P, blockIdx.y);
+// dx of a span of slab n; means[g] = scale times {sum of w dz, sum of w dz xh}
+template <int V, bool DROP, bool STREAM>
+__device__ __forceinline__ void span_back_apply(const NormArgs &A, const MapPlan &P, const Draw &d, const Column &c, const Span &t, int64_t n, const double2 *means, double scale) {
+    const T *x = (const T *)A.x + n * A.x_stride + t.base, *dy = (const T *)A.dy + n * A.dy_stride + t.base;
+    T *dx = (T *)A.out + n * A.size + t.base;
+    int off = t.off;
+    Chunk<DT> v, g;
+    if (t.lim >= 8) { v = span_load<STREAM>(x, t, off); g = span_load<STREAM>(dy, t, off); }
+    Constants<V> k;
+    load_constants<V>(A, P, A.stats + n * A.G, c.col, k);
+    float m1[V == 2 ? 1 : 8], m2[V == 2 ? 1 : 8];
+    {
+        Channel ch(A, 8 * c.col);
+#pragma unroll
+        for (int e = 0; e < (V == 2 ? 1 : 8); e++) { const double2 m = means[ch.g]; m1[e] = (float)(m.x * scale); m2[e] = (float)(m.y * scale); ch.next(A); }
+    }
+    const auto result = [&](const Chunk<DT> &cx, const Chunk<DT> &cg, int valid, float (&dz)[8]) {
+        const Mask<DROP ? V : 0> m(d, n * A.size + t.base + off);
+        float xh[8], dv[8];
+        unpack(cx, m, xh);
+        unpack(cg, dv);
+        normalise<V>(k, xh);
+        back_activation(A, x + off, n, 8 * c.col, valid, m, xh, dv, k.w, k.b, dz);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int i = V == 2 ? 0 : e;
+            dz[e] = m.keep(e, k.rstd[i] * (dz[e] * k.w[e] - m1[i] - xh[e] * m2[i]));
+        }
+    };
+    float f[8];
     if (!c.mine) return;
+#pragma unroll 1
+    while (off + 8 <= t.lim) {
+        const Chunk<DT> now = v, gnow = g;
+        v = span_load<STREAM>(x, t, off + t.step); g = span_load<STREAM>(dy, t, off + t.step);
+        result(now, gnow, 8, f);
+        if (STREAM) stream_store_whole<DT>(dx + off, f);
+        else store_whole<DT>(dx + off, f);
+        off += t.step;
+    }
+    if (V == 1 && off < t.lim) {
+        result(load_chunk<DT>(x + off, t.lim - off), load_chunk<DT>(dy + off, t.lim - off), t.lim - off, f);
+        store_chunk<DT>(dx + off, t.lim - off, f);
+    }
+}
+template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(512) void k_map_back_apply(NormArgs A, MapPlan P, const double2 *means) {
+    const Column c = my_column(P, blockIdx.y);
     const Span t = my_span(A, P, c, P.apply_rows);
     Draw d = {};
     if (DROP) d = make_draw(A.rng, A.site, A.cut);
 #pragma unroll 1
-    for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) {
-        const T *x = (const T *)A.x + n * A.x_stride + t.base, *dy = (const T *)A.dy + n * A.dy_stride + t.base;
-        T *dx = (T *)A.out + n * A.size + t.base;
-        int off = t.off;
-        Chunk<DT> v, g;
-        if (t.lim >= 8) { v = span_load<STREAM>(x, t, off); g = span_load<STREAM>(dy, t, off); }
-        Constants<V> k;
-        load_constants<V>(A, P, n, c.col, k);
-        float m1[V == 2 ? 1 : 8], m2[V == 2 ? 1 : 8];
-        {
-            Channel ch(A, 8 * c.col);
-#pragma unroll
-            for (int e = 0; e < (V == 2 ? 1 : 8); e++) { const float2 m = means[n * A.G + ch.g]; m1[e] = m.x; m2[e] = m.y; ch.next(A); }
-        }
-        const auto result = [&](const Chunk<DT> &cx, const Chunk<DT> &cg, int valid, float (&dz)[8]) {
-            const Mask<DROP ? V : 0> m(d, n * A.size + t.base + off);
-            float xh[8], dv[8];
-            unpack(cx, m, xh);
-            unpack(cg, dv);
-            normalise<V>(k, xh);
-            back_activation(A, x + off, n, 8 * c.col, valid, m, xh, dv, k.w, k.b, dz);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int i = V == 2 ? 0 : e;
-                dz[e] = m.keep(e, k.rstd[i] * (dz[e] * k.w[e] - m1[i] - xh[e] * m2[i]));
-            }
-        };
-        float f[8];
+    for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) span_back_apply<V, DROP, STREAM>(A, P, d, c, t, n, means + n * A.G, 1.0);
+}
+
+// ---- slabs that one workgroup goes over by itself: the same passes in one launch, the second reading out of the nearer caches.  `lds`: the join's space, then G pairs.
+template <int V, bool DROP> __global__ __launch_bounds__(512) void k_slab_forward(NormArgs A, MapPlan P) {
+    extern __shared__ double2 lds[];
+    double2 *groups = lds + blockDim.x * (V == 2 ? 1 : 8);
+    const Column c = my_column(P, 0);
+    const Span t = my_span(A, P, c, P.rows);
+    Draw d = {};
+    if (DROP) { d = make_draw(A.rng, A.site, A.cut); write_used(A); }
 #pragma unroll 1
-        while (off + 8 <= t.lim) {
-            const Chunk<DT> now = v, gnow = g;
-            v = span_load<STREAM>(x, t, off + t.step); g = span_load<STREAM>(dy, t, off + t.step);
-            result(now, gnow, 8, f);
-            if (STREAM) stream_store_whole<DT>(dx + off, f);
-            else store_whole<DT>(dx + off, f);
-            off += t.step;
+    for (int64_t n = blockIdx.y; n < A.N; n += gridDim.y) {
+        double s[8] = {}, q[8] = {};
+        span_sums<V, DROP>(A, d, c, t, n, s, q);
+        join_groups<V>(s, q, A, P, c, lds, groups, 1);
+        __syncthreads();
+        const double shift = slab_shift<DROP>(A, d, n);
+        for (int g = threadIdx.x; g < A.G; g += blockDim.x) {
+            groups[g] = finish_stats(A, shift, groups[g].x, groups[g].y);
+            if (A.stats) A.stats[n * A.G + g] = groups[g];
         }
-        if (V == 1 && off < t.lim) {
-            result(load_chunk<DT>(x + off, t.lim - off), load_chunk<DT>(dy + off, t.lim - off), t.lim - off, f);
-            store_chunk<DT>(dx + off, t.lim - off, f);
+        __syncthreads();
+        span_apply<V, DROP, false>(A, P, d, c, t, n, groups);
+    }
+}
+template <int V, bool DROP> __global__ __launch_bounds__(512) void k_slab_backward(NormArgs A, MapPlan P, float *params) {
+    extern __shared__ double2 lds[];
+    double2 *groups = lds + blockDim.x * 8;
+    const Column c = my_column(P, 0);
+    const Span t = my_span(A, P, c, P.rows);
+    Draw d = {};
+    if (DROP) d = make_draw(A.rng, A.site, A.cut);
+#pragma unroll 1
+    for (int64_t n = blockIdx.y; n < A.N; n += gridDim.y) {
+        double s1[8] = {}, s2[8] = {};
+        {
+            Constants<V> k;
+            span_back_sums<V, DROP>(A, P, d, c, t, n, k, s1, s2);
+            if (params) channel_sums(s1, s2, A, P, c, lds, params + (int64_t)blockIdx.y * 2 * A.C, n == blockIdx.y);
+#pragma unroll
+            for (int e = 0; e < 8; e++) { s1[e] *= (double)k.w[e]; s2[e] *= (double)k.w[e]; }
         }
+        join_groups<V>(s1, s2, A, P, c, lds, groups, 1);
+        __syncthreads();
+        span_back_apply<V, DROP, false>(A, P, d, c, t, n, groups, A.inv_count);
     }
 }
 
@@ -778,7 +834,9 @@ void params(const NormArgs &a, const float *part, int rows, void *dw, void *db, 
 
 bool one_group(const NormArgs &a) { return a.C % 8 == 0 && a.D % 8 == 0; }
 template <int V, bool DROP> void map_forward_v(const NormArgs &a, const MapLaunch &m, double2 *part, hipStream_t s) {
-    k_map_sums<V, DROP><<<m.sums, m.NT, (size_t)m.NT * (V == 2 ? 16 : 128), s>>>(a, m.P, part);
+    const size_t lds = (size_t)m.NT * (V == 2 ? 16 : 128);
+    if (m.slab) { k_slab_forward<V, DROP><<<m.sums, m.NT, lds + a.G * 16, s>>>(a, m.P); return; }
+    k_map_sums<V, DROP><<<m.sums, m.NT, lds, s>>>(a, m.P, part);
     k_map_stats<DROP><<<m.stat_blocks, 256, 0, s>>>(a, m.P.splits * m.P.col_blocks, part);
     if (m.stream) k_map_apply<V, DROP, true><<<m.apply, m.NT, 0, s>>>(a, m.P);
     else k_map_apply<V, DROP, false><<<m.apply, m.NT, 0, s>>>(a, m.P);
@@ -787,7 +845,12 @@ void map_forward(const NormArgs &a, const MapLaunch &m, double2 *part, hipStream
     if (one_group(a)) a.cut ? map_forward_v<2, true>(a, m, part, s) : map_forward_v<2, false>(a, m, part, s);
     else a.cut ? map_forward_v<1, true>(a, m, part, s) : map_forward_v<1, false>(a, m, part, s);
 }
-template <int V, bool DROP> void map_backward_v(const NormArgs &a, const MapLaunch &m, double2 *part, float2 *means, float *sums, void *dw, void *db, hipStream_t s) {
+template <int V, bool DROP> void map_backward_v(const NormArgs &a, const MapLaunch &m, double2 *part, double2 *means, float *sums, void *dw, void *db, hipStream_t s) {
+    if (m.slab) {
+        k_slab_backward<V, DROP><<<m.sums, m.NT, (size_t)m.NT * 128 + a.G * 16, s>>>(a, m.P, sums);
+        if (sums) params(a, sums, m.param_rows, dw, db, s);
+        return;
+    }
     k_map_back_sums<V, DROP><<<m.sums, m.NT, (size_t)m.NT * 128, s>>>(a, m.P, part, sums);
     const int64_t items = a.N * a.G;
     const int join = (int)(items < 16 * 4096 ? (items + 15) / 16 : 4096);
@@ -795,7 +858,7 @@ template <int V, bool DROP> void map_backward_v(const NormArgs &a, const MapLaun
     if (m.stream) k_map_back_apply<V, DROP, true><<<m.apply, m.NT, 0, s>>>(a, m.P, means);
     else k_map_back_apply<V, DROP, false><<<m.apply, m.NT, 0, s>>>(a, m.P, means);
 }
-void map_backward(const NormArgs &a, const MapLaunch &m, double2 *part, float2 *means, float *sums, void *dw, void *db, hipStream_t s) {
+void map_backward(const NormArgs &a, const MapLaunch &m, double2 *part, double2 *means, float *sums, void *dw, void *db, hipStream_t s) {
     if (one_group(a)) a.cut ? map_backward_v<2, true>(a, m, part, means, sums, dw, db, s) : map_backward_v<2, false>(a, m, part, means, sums, dw, db, s);
     else a.cut ? map_backward_v<1, true>(a, m, part, means, sums, dw, db, s) : map_backward_v<1, false>(a, m, part, means, sums, dw, db, s);
 }
