@@ -6,10 +6,6 @@
 #ifndef STREAM_BYTES
 #define STREAM_BYTES ((int64_t)64 << 20)
 #endif
-#ifndef SLAB_ANY
-#define SLAB_ANY 32768
-#define SLAB_MANY 131072
-#endif
 #define MAP_MAX_SPAN ((int64_t)1 << 28)      // elements of a slab that one workgroup walks over
 #define ROW_MAX_FORWARD 8192            // widest group that the lanes of one workgroup hold: 256 lanes of 4 chunks, or in the backward pass (which holds four times as much) 512 of one
 #define ROW_MAX_BACKWARD 4096
@@ -117,7 +113,7 @@ static int fill_threads(int ncol, int lo, int hi) {
     }
     return best;
 }
-static MapLaunch map_plan(const PlenRegNorm &a) {
+static MapLaunch map_plan(const PlenRegNorm &a, bool backward) {
     MapLaunch m;
     const int D = a.C / a.G;
     const int64_t size = a.L * a.C;
@@ -129,8 +125,11 @@ static MapLaunch map_plan(const PlenRegNorm &a) {
     m.P.col_blocks = (int)div_up(m.P.ncol, 512);
     m.P.bcol = (int)div_up(m.P.ncol, m.P.col_blocks);
     m.P.inv_bcol = 1.f / (float)m.P.bcol;
-    // one workgroup per slab: no more launches than one, and the slab is read once from memory; but only as many compute units work as there are slabs
-    m.slab = m.P.bcol <= 448 && m.P.col_blocks == 1 && a.G <= 512 && (size <= SLAB_ANY || (size <= SLAB_MANY && a.N >= 128));
+    // one workgroup per slab: one launch instead of three, and the slab is read once from memory; but only as many compute units work as there are slabs.
+    // Measured (us, slab / split; N x L x C bf16): forward 8 x 32 x 320 7.9 / 13.7, 8 x 1024 x 32 9.4 / 11.9, 8 x 128 x 320 12.6 / 13.8, 8 x 512 x 195 28 / 17, 256 x 512 x 195 46 / 46;
+    // backward 8 x 512 x 32 15.5 / 14.5, 8 x 128 x 195 28.5 / 24.8, 64 x 128 x 320 29 / 32, 64 x 512 x 320 70 / 48, 256 x 512 x 320 85 / 127.
+    m.slab = m.P.bcol <= 448 && m.P.col_blocks == 1 && a.G <= 512
+             && (backward ? size <= 16384 || (a.N >= 64 && size <= 49152) || (a.N >= 256 && size <= 262144) : size <= 32768 || (a.N >= 256 && size <= 98304));
     const int64_t threads = div_up(chunks, 64) * 64;
     m.NT = m.slab ? fill_threads(m.P.bcol, threads < 448 ? (int)threads : 448, 448) : fill_threads(m.P.bcol, 256, 512);
     m.P.R = m.NT / m.P.bcol;
@@ -205,7 +204,7 @@ int plenreg_dropout(const PlenRegDropout *a, void *stream) {
 int64_t plenreg_norm_workspace(const PlenRegNorm *a, int backward) {
     if (bad_norm(a)) return PLENREG_REFUSE;
     if (by_rows(*a, backward)) return backward ? (int64_t)row_plan(*a, true).grid.x * 2 * a->C * 4 : 0;
-    const MapLaunch m = map_plan(*a);
+    const MapLaunch m = map_plan(*a, backward);
     if (m.slab) return backward ? (int64_t)m.param_rows * 2 * a->C * 4 : 0;
     return part_bytes(*a, m) + a->N * a->G * 16 + (backward ? (int64_t)m.param_rows * 2 * a->C * 4 : 0);
 }
@@ -217,7 +216,7 @@ int plenreg_norm_forward(const PlenRegNorm *a, void *stream) {
         entry(*a).row_forward(k, row_plan(*a, false), (hipStream_t)stream);
         return launched();
     }
-    const MapLaunch m = map_plan(*a);
+    const MapLaunch m = map_plan(*a, false);
     if (!a->ws && !m.slab) return PLENREG_REFUSE;
     if (!k.stats && !m.slab) k.stats = (double2 *)((char *)a->ws + part_bytes(*a, m));
     entry(*a).map_forward(k, m, (double2 *)a->ws, (hipStream_t)stream);
@@ -236,7 +235,7 @@ int plenreg_norm_backward(const PlenRegNorm *a, void *stream) {
         if (params) e.params(k, (const float *)a->ws, (int)r.grid.x, a->dw, a->db, (hipStream_t)stream);
         return launched();
     }
-    const MapLaunch m = map_plan(*a);
+    const MapLaunch m = map_plan(*a, true);
     char *ws = (char *)a->ws;
     double2 *means = (double2 *)(ws + part_bytes(*a, m));
     float *sums = !params ? nullptr : m.slab ? (float *)ws : (float *)(means + a->N * a->G);
