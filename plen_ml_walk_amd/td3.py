@@ -21,12 +21,64 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import regularise as R
+
 
 def default_device():
     """The rank-local accelerator (one process per GPU), or the CPU when there is none."""
     if torch.cuda.is_available():
         return torch.device("cuda", int(os.environ.get("LOCAL_RANK", torch.cuda.current_device())))
     return torch.device("cpu")
+
+
+class _CapturedLinear(torch.autograd.Function):
+    """F.linear whose weight and bias gradients are one launch of csrc/td3_kernels.hip's weight-gradient kernel."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        ctx.save_for_backward(x, weight)
+        return F.linear(x, weight, bias)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        from . import td3_fused as TF
+        x, weight = ctx.saved_tensors
+        dy, x = (t if t.stride(1) == 1 else t.contiguous() for t in (dy, x))
+        (n, k), rows = weight.shape, dy.shape[0]
+        g = torch.zeros(n * k + n, dtype=torch.float32, device=dy.device)
+        TF._chk(TF.load().plentd3_wgrad(TF._p(dy), dy.stride(0), TF._p(x), x.stride(0), TF._p(g), k, TF.C.c_void_p(g.data_ptr() + 4 * n * k), rows, n, k, 0,
+                                        TF.C.c_void_p(torch.cuda.current_stream(dy.device).cuda_stream)))
+        return dy @ weight if ctx.needs_input_grad[0] else None, g[:n * k].view(n, k), g[n * k:]
+
+
+def _capturing(x):
+    return x.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
+def _linear(x, weight, bias):
+    """F.linear.  While a stream is being captured its gradients come from the framework's own kernel: the library's bias gradient, a sum over many blocks, clears
+    its counters with a memset, and such nodes leave wrong values from a graph's second replay on (at batch 4096 biases off by as much as they are large)."""
+    if torch.is_grad_enabled() and weight.requires_grad and x.dim() == 2 and x.dtype == weight.dtype == torch.float32 and _capturing(x):
+        return _CapturedLinear.apply(x, weight, bias)
+    return F.linear(x, weight, bias)
+
+
+def _layer(layer, x):
+    return _linear(x, layer.weight, layer.bias) if _capturing(x) else layer(x)
+
+
+def _mse(q, target):
+    """F.mse_loss; while capturing, in parts that the library sums within one block each (see _linear)."""
+    if q.numel() <= 4096 or not _capturing(q):
+        return F.mse_loss(q, target)
+    return sum(F.mse_loss(a, b, reduction="sum") for a, b in zip(q.split(4096), target.split(4096))) / q.numel()
+
+
+def _mean(q):
+    if q.numel() <= 4096 or not _capturing(q):
+        return q.mean()
+    return sum(a.sum() for a in q.split(4096)) / q.numel()
 
 
 class Actor(nn.Module):
@@ -40,9 +92,9 @@ class Actor(nn.Module):
         self.max_action = max_action
 
     def forward(self, state):
-        a = F.relu(self.fc1(state))
-        a = F.relu(self.fc2(a))
-        return self.max_action * torch.tanh(self.fc3(a))
+        a = F.relu(_layer(self.fc1, state))
+        a = F.relu(_layer(self.fc2, a))
+        return self.max_action * torch.tanh(_layer(self.fc3, a))
 
 
 class Critic(nn.Module):
@@ -59,19 +111,80 @@ class Critic(nn.Module):
 
     def forward(self, state, action):
         sa = torch.cat([state, action], 1)
-        q1 = F.relu(self.fc1(sa))
-        q1 = F.relu(self.fc2(q1))
-        q1 = self.fc3(q1)
-        q2 = F.relu(self.fc4(sa))
-        q2 = F.relu(self.fc5(q2))
-        q2 = self.fc6(q2)
+        q1 = F.relu(_layer(self.fc1, sa))
+        q1 = F.relu(_layer(self.fc2, q1))
+        q1 = _layer(self.fc3, q1)
+        q2 = F.relu(_layer(self.fc4, sa))
+        q2 = F.relu(_layer(self.fc5, q2))
+        q2 = _layer(self.fc6, q2)
         return q1, q2
 
     def Q1(self, state, action):
         sa = torch.cat([state, action], 1)
-        q1 = F.relu(self.fc1(sa))
-        q1 = F.relu(self.fc2(q1))
-        return self.fc3(q1)
+        q1 = F.relu(_layer(self.fc1, sa))
+        q1 = F.relu(_layer(self.fc2, q1))
+        return _layer(self.fc3, q1)
+
+
+class _HiddenNorm(nn.Module):
+    """Weight (ones) and bias (zeros) of a layer norm over hidden rows."""
+
+    def __init__(self, width):
+        super(_HiddenNorm, self).__init__()
+        self.weight, self.bias = nn.Parameter(torch.ones(width)), nn.Parameter(torch.zeros(width))
+
+
+class RegularisedCritic(Critic):
+    """The twin Q networks with dropout and / or layer norm on both hidden layers: linear -> dropout -> layer norm -> ReLU (the two of them together let a
+    Q network take many updates per environment step).  The hidden rows of both networks lie side by side in one [B, 2h] matrix, so that the first layers are
+    one product and each regularisation is one call for both networks (group norm with two groups is the layer norm of each).
+
+    The names fc1..fc6 are Critic's; norm1 / norm2 hold the weight and bias of the first / second hidden layers, [Q1's h | Q2's h].  Every forward in training mode
+    draws new masks from the device state `rng` = {seed, calls} and moves it on by one call, on the device: a captured forward draws new masks at each replay.  eval()
+    leaves the dropout out.  `rng` is no part of the state_dict: ranks and target networks keep streams of their own (`seed_masks`)."""
+
+    def __init__(self, state_dim, action_dim, dropout=0.0, norm=False, seed=0):
+        super(RegularisedCritic, self).__init__(state_dim, action_dim)
+        if not 0.0 <= float(dropout) < 1.0:
+            raise ValueError("dropout has to be in [0, 1), got %r" % (dropout,))
+        self.dropout, self.norm = float(dropout), bool(norm)
+        if self.norm:
+            self.norm1, self.norm2 = _HiddenNorm(2 * self.fc1.out_features), _HiddenNorm(2 * self.fc2.out_features)
+        self.register_buffer("rng", R.new_rng("cpu", seed), persistent=False)
+
+    def seed_masks(self, seed, calls=0):
+        """Start the mask stream at {seed, calls}, in place (a graph that reads it goes on from there)."""
+        self.rng.copy_(torch.tensor([int(seed) & 0x7fffffffffffffff, int(calls)], dtype=torch.long))
+
+    def _hidden(self, x, layer, groups):
+        """dropout -> layer norm -> ReLU of the `groups` networks' rows of hidden layer `layer` (0 or 1)."""
+        drop = self.training and self.dropout > 0
+        if not self.norm:
+            return F.relu(R.dropout(x, self.dropout, self.rng, site=layer) if drop else x)
+        m = self.norm2 if layer else self.norm1
+        w, b = (m.weight, m.bias) if groups == 2 else (m.weight[:x.shape[1]], m.bias[:x.shape[1]])
+        if drop:
+            return R.dropout_norm_act(x, self.dropout, self.rng, groups, w, b, site=layer, act="relu")
+        return R.group_norm_act(x, groups, w, b, act="relu")
+
+    def _drawn(self):
+        if self.training and self.dropout > 0:
+            R.advance(self.rng)
+
+    def forward(self, state, action):
+        sa = torch.cat([state, action], 1)
+        h = self._hidden(_linear(sa, torch.cat((self.fc1.weight, self.fc4.weight)), torch.cat((self.fc1.bias, self.fc4.bias))), 0, 2)
+        h1, h2 = h.split(self.fc2.in_features, 1)
+        h = self._hidden(torch.cat((_layer(self.fc2, h1), _layer(self.fc5, h2)), 1), 1, 2)
+        h1, h2 = h.split(self.fc3.in_features, 1)
+        self._drawn()
+        return _layer(self.fc3, h1), _layer(self.fc6, h2)
+
+    def Q1(self, state, action):
+        h = self._hidden(_layer(self.fc1, torch.cat([state, action], 1)), 0, 1)
+        h = self._hidden(_layer(self.fc2, h), 1, 1)
+        self._drawn()
+        return _layer(self.fc3, h)
 
 
 class _StorageView(object):
@@ -233,8 +346,9 @@ def _flat_order(module):
     GEMM for both networks' first layers, td3_fused.py) and [fc1.bias; fc4.bias] = "b14", [fc2.bias; fc5.bias] = "b25" single vectors."""
     if isinstance(module, Critic):
         m = module
-        return [m.fc1.weight, m.fc4.weight, m.fc1.bias, m.fc4.bias, m.fc2.weight, m.fc5.weight, m.fc2.bias, m.fc5.bias,
-                m.fc3.weight, m.fc6.weight, m.fc3.bias, m.fc6.bias]
+        order = [m.fc1.weight, m.fc4.weight, m.fc1.bias, m.fc4.bias, m.fc2.weight, m.fc5.weight, m.fc2.bias, m.fc5.bias,
+                 m.fc3.weight, m.fc6.weight, m.fc3.bias, m.fc6.bias]
+        return order + [p for n in ("norm1", "norm2") if hasattr(m, n) for p in getattr(m, n).parameters()]       # (RegularisedCritic: behind the layers)
     return [p for p in module.parameters() if p.requires_grad]
 
 
@@ -323,7 +437,7 @@ def td3_critic_backward(agent, batch, noise=None):
         target_Q = torch.min(target_Q1, target_Q2)
         target_Q = reward + not_done * agent.discount * target_Q
     current_Q1, current_Q2 = agent.critic(state, action)
-    critic_loss = F.mse_loss(current_Q1, target_Q) + F.mse_loss(current_Q2, target_Q)
+    critic_loss = _mse(current_Q1, target_Q) + _mse(current_Q2, target_Q)
     agent._critic_grads.zero()
     critic_loss.backward()
     agent._critic_grads.dirty = True
@@ -333,7 +447,7 @@ def td3_critic_backward(agent, batch, noise=None):
 def td3_actor_backward(agent, batch):
     """Delayed policy gradient (reference td3.py:334-341) into the actor's flat bucket."""
     state = batch[0]
-    actor_loss = -agent.critic.Q1(state, agent.actor(state)).mean()
+    actor_loss = -_mean(agent.critic.Q1(state, agent.actor(state)))
     agent._actor_grads.zero()
     actor_loss.backward()                          # also writes critic grads; they are zeroed before their next use
     agent._actor_grads.dirty = agent._critic_grads.dirty = True
@@ -369,17 +483,23 @@ def td3_update(agent, batch, with_policy, noise=None, all_reduce=True):
 
 
 class TD3Agent(object):
-    """Twin Delayed DDPG agent with the reference's constructor and methods (td3.py:196-376)."""
+    """Twin Delayed DDPG agent with the reference's constructor and methods (td3.py:196-376).
+
+    critic_dropout > 0 and / or critic_norm: the critics are RegularisedCritics (dropout / layer norm on their hidden layers, csrc/regularise*.hip).  train() then takes
+    the autograd iteration; the hand-fused one (td3_fused.FusedTD3) is for the plain critics and refuses these."""
 
     def __init__(self, state_dim, action_dim, max_action, discount=0.99, tau=0.005, policy_noise=0.2, noise_clip=0.5,
-                 policy_freq=2, device=None, lr=3e-4, data_parallel=True):
+                 policy_freq=2, device=None, lr=3e-4, data_parallel=True, critic_dropout=0.0, critic_norm=False):
         self.data_parallel = data_parallel
         self.device = _indexed(device) if device is not None else default_device()
         self.actor = Actor(state_dim, action_dim, max_action).to(self.device)
-        self.critic = Critic(state_dim, action_dim).to(self.device)
+        critic = RegularisedCritic(state_dim, action_dim, critic_dropout, critic_norm) if critic_dropout or critic_norm else Critic(state_dim, action_dim)
+        self.critic = critic.to(self.device)
         self._broadcast_parameters()                       # every rank starts from rank 0's initialisation
         self.actor_target = copy.deepcopy(self.actor)
         self.critic_target = copy.deepcopy(self.critic)
+        if self.regularised:
+            self.seed_masks(torch.initial_seed())
         self._actor_flat, self._critic_flat = _FlatParams(self.actor), _FlatParams(self.critic)
         self._actor_target_flat, self._critic_target_flat = _FlatParams(self.actor_target), _FlatParams(self.critic_target)
         self.actor_optimizer = torch.optim.Adam(self.actor.parameters(), lr=lr)
@@ -407,6 +527,17 @@ class TD3Agent(object):
         if self.data_parallel and dist.is_available() and dist.is_initialized() and (dist.get_world_size() > 1 or os.environ.get("PLEN_TD3_FORCE_COLLECTIVES") == "1"):
             for p in list(self.actor.parameters()) + list(self.critic.parameters()):
                 dist.broadcast(p.data, src=0)
+
+    @property
+    def regularised(self):
+        return isinstance(self.critic, RegularisedCritic)
+
+    def seed_masks(self, seed, calls=0):
+        """Streams of the critics' dropout masks (agents with critic_dropout): one for the critic, one for its target, both different on every rank."""
+        import torch.distributed as dist
+        rank = dist.get_rank() if self.data_parallel and dist.is_available() and dist.is_initialized() else 0
+        for k, net in enumerate((self.critic, self.critic_target)):
+            net.seed_masks((int(seed) & 0x7fffffff) + ((2 * rank + k + 1) << 32), calls)
 
     # ---- acting -------------------------------------------------------------------------
     def select_action(self, state):
@@ -459,7 +590,7 @@ class TD3Agent(object):
         arithmetic, with the replay indices and the target-smoothing noise drawn inside the kernels from the agent's counter-based stream instead of
         torch's / NumPy's generators.  The autograd iteration (td3_update: same order of operations and RNG calls as the reference) runs
         wherever that is not possible or not wanted: on the CPU, with `fused_train = False` or PLEN_TD3_FUSED_TRAIN=0, with PLEN_TD3_NUMPY_RNG=1,
-        or when the buffer's `sample` is not this module's own (a subclass or an instance override: the caller's sampling is honoured)."""
+        with regularised critics, or when the buffer's `sample` is not this module's own (a subclass or an instance override: the caller's sampling is honoured)."""
         self.total_it += 1
         with_policy = self.total_it % self.policy_freq == 0
         fz = self._fused_for(replay_buffer)
@@ -474,7 +605,7 @@ class TD3Agent(object):
         """The FusedTD3 behind train() (created on first use), or None where train() has to take the autograd iteration."""
         if self.fused_train is False or (self.fused_train is None and os.environ.get("PLEN_TD3_FUSED_TRAIN", "1") != "1"):
             return None
-        if self.device.type != "cuda" or os.environ.get("PLEN_TD3_NUMPY_RNG") == "1" or not self._plen_shaped():
+        if self.device.type != "cuda" or os.environ.get("PLEN_TD3_NUMPY_RNG") == "1" or not self._plen_shaped() or self.regularised:
             return None
         if not (isinstance(replay_buffer, ReplayBuffer) and type(replay_buffer).sample is ReplayBuffer.sample and "sample" not in vars(replay_buffer)):
             return None

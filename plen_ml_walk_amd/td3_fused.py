@@ -264,6 +264,9 @@ class FusedTD3(object):
     def __init__(self, agent, seed=0, rows=None, team=None, block=None):
         if agent.device.type != "cuda":
             raise PlenTd3Error("FusedTD3 needs the agent on a HIP device")
+        if agent.regularised:
+            raise PlenTd3Error("FusedTD3 updates the plain critics; an agent with critic_dropout or critic_norm takes the autograd iteration (td3.td3_update, "
+                               "GraphedVecTD3Trainer(fused=False))")
         self.agent = agent
         # counter-based RNG state of the update's draws (replay indices, target-smoothing noise): {seed, calls so far} on the device
         self.rng = self.new_rng(agent.device, seed)

@@ -87,6 +87,8 @@ def resume_training(agent, replay, prefix, replay_id=None):
             with open(prefix + "_trainer.json") as fh:
                 counters.update(json.load(fh))
         agent.total_it = counters["total_it"]
+        if agent.regularised:             # masks that the run before has not drawn: an iteration makes at most two passes over a critic
+            agent.seed_masks(torch.initial_seed(), 2 * agent.total_it)
     if replay_id is not None and os.path.exists(replay.buffer_path + "/replay_buffer_" + str(replay_id) + ".data"):
         replay.load(replay_id)
     return counters
@@ -153,7 +155,14 @@ def main(argv=None):
     ap.add_argument("--buffer-path", default=None, help="directory of replay_buffer_<n>.data files (td3.py:128-131)")
     ap.add_argument("--save-replay", type=int, default=None, help="write the rank-local replay buffer as replay_buffer_<n>.data at the end")
     ap.add_argument("--load-replay", type=int, default=None, help="read replay_buffer_<n>.data before training (with --resume)")
+    ap.add_argument("--critic-dropout", type=float, default=0.0, help="dropout on the critics' hidden layers (td3.RegularisedCritic; the autograd update, captured with --graphs 1)")
+    ap.add_argument("--critic-norm", action="store_true", help="layer norm on the critics' hidden layers")
     a = ap.parse_args(argv)
+    regularised = bool(a.critic_dropout or a.critic_norm)
+    if not 0.0 <= a.critic_dropout < 1.0:
+        ap.error("--critic-dropout has to be in [0, 1)")
+    if regularised and a.schedule == "pipelined":
+        ap.error("--schedule pipelined runs the fused update of the plain critics; --critic-dropout and --critic-norm need --schedule sync")
     from . import sharding
     from .vec_env import PlenVecEnv
     from .td3 import ReplayBuffer, TD3Agent
@@ -165,7 +174,7 @@ def main(argv=None):
     pipelined = a.schedule == "pipelined" and a.graphs and a.updates_per_step == 1 and a.envs % 2 == 0
     envs = [PlenVecEnv(a.envs // 2, device=dev) for _ in range(2)] if pipelined else [PlenVecEnv(a.envs, device=dev)]
     env = envs[0]
-    agent = TD3Agent(26, 18, 1.0, device=dev)
+    agent = TD3Agent(26, 18, 1.0, device=dev, critic_dropout=a.critic_dropout, critic_norm=a.critic_norm)
     replay = ReplayBuffer(a.replay, device=dev)
     replay.seed(a.seed + rank)
     if a.buffer_path:
@@ -177,7 +186,7 @@ def main(argv=None):
     if pipelined:
         tr = PipelinedVecTD3Trainer(envs, agent, replay, a.start_timesteps, 0.1, a.batch, seed=1000 + rank)
     elif a.graphs:
-        tr = GraphedVecTD3Trainer(env, agent, replay, a.start_timesteps, 0.1, a.batch, a.updates_per_step, seed=1000 + rank)
+        tr = GraphedVecTD3Trainer(env, agent, replay, a.start_timesteps, 0.1, a.batch, a.updates_per_step, seed=1000 + rank, fused=not regularised)
     else:
         tr = VecTD3Trainer(env, agent, replay, a.start_timesteps, 0.1, a.batch, a.updates_per_step, seed=1000 + rank)
     if resumed:
@@ -203,6 +212,7 @@ def main(argv=None):
                           "grad_steps_per_sec": (tr.grad_steps - g0) / dt, "n_gpus": world, "envs_per_gpu": a.envs, "batch": a.batch,
                           "updates_per_step": a.updates_per_step, "hip_graphs": bool(a.graphs), "allreduce_mode": getattr(tr, "allreduce_mode", None), "steps": a.steps, "ms_per_step": dt / a.steps * 1e3,
                           "critic_loss": float(agent.last_critic_loss) if agent.last_critic_loss is not None else None,
+                          "critic_dropout": a.critic_dropout, "critic_norm": a.critic_norm,
                           "schedule": "pipelined" if pipelined else "sync", "episodes": tr.episode_stats() if pipelined else None}))
         if a.save:
             save_training(agent, tr, a.save)
