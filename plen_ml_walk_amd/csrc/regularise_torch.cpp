@@ -1,15 +1,18 @@
 // regularise_torch.cpp -- the autograd nodes of regularise.py: tensors in, tensors out, around the C ABI of include/plenreg.h.
 //
 // Native because of the small calls: a training pass of a 100 x 512 layer takes 13 us on the GPU; with the nodes written in Python its two passes cost
-// 120-160 us of host time (the engine's thread has to get hold of the interpreter for each node), with these about a third of that.
+// 120-160 us of host time (the engine's thread has to get hold of the interpreter for each node), with these about a third of that.  Nodes with plain
+// members rather than torch::autograd::Function, whose context (a map of values by name, wrapped inputs and outputs) costs several us a pass.
 // Arguments are checked in regularise.py, and once more, as far as memory is concerned, behind the C ABI.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <c10/hip/HIPStream.h>
 #include "../../include/plenreg.h"
 
 using at::Tensor;
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 namespace {
@@ -41,6 +44,12 @@ variable_list once(variable_list out) {
     return (*node)(std::move(out));
 }
 
+// as saved tensors that are used after their release report it
+void check_alive(bool released) {
+    TORCH_CHECK(!released, "Trying to backward through the graph a second time: the saved state of this operator has been released; pass retain_graph=True to the first backward");
+}
+void no_tangent(const Tensor &t) { TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "plen_ml_walk_amd.regularise has no forward-mode derivatives"); }
+
 // ---- dropout
 // x as rows of contiguous elements, a constant stride apart; what is laid out otherwise is copied first
 Tensor as_rows(const Tensor &x, PlenRegDropout &a) {
@@ -68,28 +77,37 @@ Tensor run_dropout(const Tensor &x, int64_t cut, const Tensor &rng, int64_t site
     launch(dropout_entry, a, x);
     return y;
 }
-struct Dropout : torch::autograd::Function<Dropout> {
-    static Tensor forward(AutogradContext *ctx, const Tensor &x, int64_t cut, const Tensor &rng, int64_t site) {
-        const Tensor used = at::empty_like(rng);
-        const Tensor y = run_dropout(x, cut, rng, site, used);
-        ctx->save_for_backward({used});
-        ctx->saved_data["cut"] = cut;
-        ctx->saved_data["site"] = site;
-        return y;
-    }
-    static variable_list backward(AutogradContext *ctx, variable_list dy) {
-        const variable_list saved = ctx->get_saved_variables();
+struct DropoutNode : torch::autograd::Node {
+    Tensor used;
+    int64_t cut, site;
+    bool released = false;
+    variable_list apply(variable_list &&dy) override {
         Tensor dx;
-        if (dy[0].defined()) {
+        {
+            std::lock_guard<std::mutex> lock(mutex_);
+            check_alive(released);
             const at::NoGradGuard off;
-            dx = run_dropout(dy[0], ctx->saved_data["cut"].toInt(), saved[0], ctx->saved_data["site"].toInt(), Tensor());
+            if (dy[0].defined() && task_should_compute_output(0)) dx = run_dropout(dy[0], cut, used, site, Tensor());
         }
-        return once({dx, Tensor(), Tensor(), Tensor()});
+        return once({dx});
     }
+    void release_variables() override { std::lock_guard<std::mutex> lock(mutex_); used.reset(); released = true; }
+    std::string name() const override { return "RegulariseDropout"; }
 };
 Tensor dropout(const Tensor &x, int64_t cut, const Tensor &rng, int64_t site) {
-    if (x.requires_grad() && at::GradMode::is_enabled()) return Dropout::apply(x, cut, rng, site);
-    return run_dropout(x, cut, rng, site, Tensor());
+    no_tangent(x);
+    if (!x.requires_grad() || !at::GradMode::is_enabled()) return run_dropout(x, cut, rng, site, Tensor());
+    const std::shared_ptr<DropoutNode> node(new DropoutNode, torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x));
+    node->cut = cut; node->site = site;
+    Tensor y;
+    {
+        const at::AutoDispatchBelowADInplaceOrView below;
+        node->used = at::empty({2}, rng.options());
+        y = run_dropout(x, cut, rng, site, node->used);
+    }
+    torch::autograd::set_history(y, node);
+    return y;
 }
 
 // ---- group norm with an activation, with dropout (cut > 0) or without
@@ -140,55 +158,69 @@ Tensor run_forward(const Tensor &x_, const Tensor &w_, const Tensor &b_, const F
     launch(forward_entry, a, x);
     return y;
 }
-struct NormAct : torch::autograd::Function<NormAct> {
-    // (what is not there has to be an empty optional: the engine looks at every tensor it is given)
-    static Tensor forward(AutogradContext *ctx, const Tensor &x, const std::optional<Tensor> &w_, const std::optional<Tensor> &b_, int64_t groups, double eps, int64_t act, int64_t cut,
-                          const std::optional<Tensor> &rng_, int64_t site) {
-        const Tensor w = w_.value_or(Tensor()), b = b_.value_or(Tensor()), rng = rng_.value_or(Tensor());
-        const Form f = {groups, act, cut, site, eps};
-        const Tensor stats = at::empty({x.size(0), groups, 2}, x.options().dtype(at::kDouble).memory_format(at::MemoryFormat::Contiguous)), used = cut ? at::empty_like(rng) : Tensor();
-        const Tensor y = run_forward(x, w, b, f, rng, stats, used);
-        ctx->save_for_backward({x, w, b, stats, used});
-        ctx->saved_data["form"] = c10::IValue(std::vector<int64_t>{groups, act, cut, site});
-        ctx->saved_data["eps"] = eps;
-        return y;
-    }
-    static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        const variable_list saved = ctx->get_saved_variables();
-        variable_list out(9);
+struct NormNode : torch::autograd::Node {
+    SavedVariable x_, w_, b_;
+    Tensor stats, used;
+    Form f;
+    bool released = false;
+    variable_list apply(variable_list &&grads) override {
+        variable_list out(3);
+        std::unique_lock<std::mutex> lock(mutex_);
+        check_alive(released);
         if (grads[0].defined()) {
             const at::NoGradGuard off;
-            const std::vector<int64_t> i = ctx->saved_data["form"].toIntVector();
-            const Form f = {i[0], i[1], i[2], i[3], ctx->saved_data["eps"].toDouble()};
-            const Tensor &x_ = saved[0], w = as_param(saved[1], x_), b = as_param(saved[2], x_);
-            // (counted among the tensors that were there)
-            const bool want_w = w.defined() && ctx->needs_input_grad(1), want_b = b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1);
-            Tensor dx = at::empty(x_.sizes(), x_.options().memory_format(at::MemoryFormat::Contiguous)), dw = want_w ? at::empty_like(w) : Tensor(), db = want_b ? at::empty_like(b) : Tensor();
-            if (x_.numel()) {
+            const Tensor x0 = x_.unpack(), w0 = w_.unpack(), b0 = b_.unpack();
+            const Tensor w = as_param(w0, x0), b = as_param(b0, x0);
+            const bool want_w = w.defined() && task_should_compute_output(1), want_b = b.defined() && task_should_compute_output(2);
+            Tensor dx = at::empty(x0.sizes(), x0.options().memory_format(at::MemoryFormat::Contiguous)), dw = want_w ? at::empty_like(w) : Tensor(), db = want_b ? at::empty_like(b) : Tensor();
+            if (x0.numel()) {
                 int64_t xs, dys;
-                const Tensor x = as_slabs(x_, xs), dy = as_slabs(grads[0], dys);
+                const Tensor x = as_slabs(x0, xs), dy = as_slabs(grads[0], dys);
                 PlenRegNorm a = norm_args(x, w, b, f);
-                a.x = x.data_ptr(); a.x_stride = xs; a.dy = dy.data_ptr(); a.dy_stride = dys; a.out = dx.data_ptr(); a.stats = (double *)saved[3].data_ptr();
+                a.x = x.data_ptr(); a.x_stride = xs; a.dy = dy.data_ptr(); a.dy_stride = dys; a.out = dx.data_ptr(); a.stats = (double *)stats.data_ptr();
                 a.dw = want_w ? dw.data_ptr() : nullptr; a.db = want_b ? db.data_ptr() : nullptr;
-                a.rng = f.cut ? (const uint64_t *)saved[4].data_ptr() : nullptr;
+                a.rng = f.cut ? (const uint64_t *)used.data_ptr() : nullptr;
                 const Tensor ws = workspace(a, 1, x);
                 launch(backward_entry, a, x);
             } else {
                 if (want_w) dw.zero_();
                 if (want_b) db.zero_();
             }
-            out[0] = dx;
-            if (want_w) out[1] = dw.to(saved[1].scalar_type());
-            if (want_b) out[2] = db.to(saved[2].scalar_type());
+            if (task_should_compute_output(0)) out[0] = std::move(dx);
+            if (want_w) out[1] = dw.scalar_type() == w0.scalar_type() ? std::move(dw) : dw.to(w0.scalar_type());
+            if (want_b) out[2] = db.scalar_type() == b0.scalar_type() ? std::move(db) : db.to(b0.scalar_type());
         }
+        lock.unlock();
         return once(std::move(out));
     }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        x_.reset_data(); w_.reset_data(); b_.reset_data(); stats.reset(); used.reset();
+        released = true;
+    }
+    std::string name() const override { return "RegulariseNormAct"; }
 };
 Tensor norm(const Tensor &x, const std::optional<Tensor> &weight, const std::optional<Tensor> &bias, int64_t groups, double eps, int64_t act, int64_t cut, const std::optional<Tensor> &rng_, int64_t site) {
     const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor()), rng = rng_.value_or(Tensor());
-    if (at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad())))
-        return NormAct::apply(x, weight, bias, groups, eps, act, cut, rng_, site);
-    return run_forward(x, w, b, Form{groups, act, cut, site, eps}, rng, Tensor(), Tensor());
+    const Form f = {groups, act, cut, site, eps};
+    no_tangent(x); no_tangent(w); no_tangent(b);
+    if (!at::GradMode::is_enabled() || !(x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad())))
+        return run_forward(x, w, b, f, rng, Tensor(), Tensor());
+    const std::shared_ptr<NormNode> node(new NormNode, torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, w, b));
+    node->f = f;
+    node->x_ = SavedVariable(x, false);
+    if (w.defined()) node->w_ = SavedVariable(w, false);
+    if (b.defined()) node->b_ = SavedVariable(b, false);
+    Tensor y;
+    {
+        const at::AutoDispatchBelowADInplaceOrView below;
+        node->stats = at::empty({x.size(0), groups, 2}, x.options().dtype(at::kDouble).memory_format(at::MemoryFormat::Contiguous));
+        if (cut) node->used = at::empty({2}, rng.options());
+        y = run_forward(x, w, b, f, rng, node->stats, node->used);
+    }
+    torch::autograd::set_history(y, node);
+    return y;
 }
 
 }  // namespace

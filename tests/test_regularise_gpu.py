@@ -407,3 +407,46 @@ def test_gradients_reach_only_what_asks_for_them():
     dx, dw, db = torch.autograd.grad(R.group_norm_act(x, 2, w, w.detach(), act="none"), (x, w), dy) + torch.autograd.grad(
         R.group_norm_act(x, 2, w.detach(), w, act="none"), w, dy)
     assert torch.equal(got, dw + db)
+
+
+@pytest.mark.parametrize("kind", ["dropout", "norm", "layer"])
+def test_a_second_backward_needs_the_graph_kept(kind):
+    x, w, b = (t.cuda().requires_grad_() for t in (torch.randn(9, 40, generator=_gen(1)), torch.ones(40), torch.zeros(40)))
+    rng = _rng()
+    call = {"dropout": lambda: R.dropout(x, 0.3, rng), "norm": lambda: R.group_norm_act(x, 2, w, b), "layer": lambda: R.dropout_norm_act(x, 0.3, rng, 2, w, b)}[kind]
+    leaves, dy = [x] if kind == "dropout" else [x, w, b], torch.randn(9, 40, generator=_gen(2)).cuda()
+    y = call()
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    for a, b_ in zip(first, torch.autograd.grad(y, leaves, dy)):
+        assert torch.equal(a, b_)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, leaves, dy)
+    if kind != "dropout":          # (dropout keeps no input)
+        y = call()
+        with torch.no_grad():
+            x.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, leaves, dy)
+
+
+def test_gradients_of_one_leaf_at_a_time():
+    x, w, b = (t.cuda().requires_grad_() for t in (torch.randn(9, 40, generator=_gen(1)), torch.randn(40, generator=_gen(3)), torch.randn(40, generator=_gen(4))))
+    dy = torch.randn(9, 40, generator=_gen(2)).cuda()
+    whole = torch.autograd.grad(R.group_norm_act(x, 2, w, b), (x, w, b), dy)
+    for k, leaf in enumerate((x, w, b)):
+        (got,) = torch.autograd.grad(R.group_norm_act(x, 2, w, b), leaf, dy)
+        assert torch.equal(got, whole[k])
+    for k in ((0, 1), (0, 2), (1, 2)):           # some of the inputs without a gradient, or not there
+        args = [t if i in k else t.detach() for i, t in enumerate((x, w, b))]
+        got = torch.autograd.grad(R.group_norm_act(args[0], 2, args[1], args[2]), [args[i] for i in k], dy)
+        assert all(torch.equal(g, whole[i]) for g, i in zip(got, k))
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwad
+    x = torch.randn(4, 8, generator=_gen(1)).cuda()
+    with fwad.dual_level():
+        dual = fwad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: R.dropout(dual, 0.5, _rng()), lambda: R.group_norm_act(dual, 2)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
