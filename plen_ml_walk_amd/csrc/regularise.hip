@@ -157,6 +157,13 @@ static MapLaunch map_plan(const PlenRegNorm &a, bool backward) {
         m.sums = dim3(1, (unsigned)(a.N < 2048 ? a.N : 2048), 1);
         m.param_rows = (int)m.sums.y;
     }
+    // few partial pairs per slab: every workgroup of the result's launch joins them for itself (32 KB out of the caches at 2048 pairs), and there is no launch between.
+    // Measured (us, so / with a launch of its own; bf16, pairs per slab): forward 8 x 4096 x 320 2048 18.4 / 19.5, 4096 19.1 / 19.4, 10240 22.5 / 19.5, 2 x 16384 x 128 2048 9.9 / 11.4,
+    // 1 x 4096 x 512 16384 13.1 / 11.3; both passes 4 x 1089 x 195 455 36.4 / 38.5, 2275 37.2 / 39.0, 8 x 4096 x 320 2048 65.5 / 66.4, 4096 67.8 / 66.7
+    m.joins = (int64_t)a.G * m.P.splits * m.P.col_blocks <= (backward ? 2560 : 4096);
+    m.P.param_z = 0;
+    m.P.join_log = log2_up(m.NT / a.G + 1) - 1;
+    m.P.join_log = m.P.join_log < 0 ? 0 : m.P.join_log > 6 ? 6 : m.P.join_log;
     m.stream = streams(a);
     m.stat_blocks = (unsigned)(a.N * a.G < 4 * 65536 ? div_up(a.N * a.G, 4) : 65536);
     return m;

@@ -360,38 +360,39 @@ template <int V, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT
     }
 }
 
-// dw, db = column sums of part[rows][2][C] in 64 bits: 16 columns per workgroup of 1024 threads, 64 rows at a time
-__device__ __forceinline__ void param_columns(const NormArgs &A, const float *part, int rows, int block, void *dw, void *db, double (&lds)[64][17]) {
+// dw, db = column sums of part[rows][2][C] in 64 bits: 16 columns per workgroup, blockDim / 16 rows at a time.  lds: [blockDim / 16][17]
+__device__ __forceinline__ void param_columns(const NormArgs &A, const float *part, int rows, int block, void *dw, void *db, double *lds) {
     const int64_t width = 2 * (int64_t)A.C, column = (int64_t)block * 16 + (threadIdx.x & 15);
-    const int r0 = threadIdx.x >> 4;
+    const int r0 = threadIdx.x >> 4, step = blockDim.x >> 4;
     double s = 0.0;
     if (column < width) {
         int r = r0;
-        for (; r + 7 * 64 < rows; r += 8 * 64) {
+        for (; r + 7 * step < rows; r += 8 * step) {
             float v[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = part[(r + k * 64) * width + column];
+            for (int k = 0; k < 8; k++) v[k] = part[(r + k * step) * width + column];
 #pragma unroll
             for (int k = 0; k < 8; k++) s += (double)v[k];
         }
-        for (; r < rows; r += 64) s += (double)part[r * width + column];
+        for (; r < rows; r += step) s += (double)part[r * width + column];
     }
-    lds[r0][threadIdx.x & 15] = s;
+    lds[r0 * 17 + (threadIdx.x & 15)] = s;
     __syncthreads();
     if (threadIdx.x < 256) {
         // column t / 16, rows t % 16 + 16 k: then over 16 lanes
-        const int col = threadIdx.x >> 4, r = threadIdx.x & 15;
-        double t = (lds[r][col] + lds[r + 16][col]) + (lds[r + 32][col] + lds[r + 48][col]), unused = 0.0;
+        const int col = threadIdx.x >> 4;
+        double t = 0.0, unused = 0.0;
+        for (int r = threadIdx.x & 15; r < step; r += 16) t += lds[r * 17 + col];
         lanes_sum2(t, unused, 4);
         const int64_t c = (int64_t)block * 16 + col;
-        if (r == 0 && c < width) {
+        if ((threadIdx.x & 15) == 0 && c < width) {
             void *to = c < A.C ? dw : db;
             if (to) ((W *)to)[c < A.C ? c : c - A.C] = (W)(float)t;
         }
     }
 }
 __global__ __launch_bounds__(1024) void k_row_params(NormArgs A, const float *part, int rows, void *dw, void *db) {
-    __shared__ double lds[64][17];
+    __shared__ double lds[64 * 17];
     param_columns(A, part, rows, blockIdx.x, dw, db, lds);
 }
 
@@ -483,6 +484,27 @@ __device__ __forceinline__ double2 join_splits(const double2 *part, int splits) 
     for (int k = threadIdx.x & 63; k < splits; k += 64) { const double2 t = part[k]; s += t.x; q += t.y; }
     lanes_sum2(s, q, 6);
     return double2{s, q};
+}
+// the sums over the partial pairs of every group of a slab, by a whole workgroup: result(g, sums) from one lane each
+template <class F> __device__ __forceinline__ void join_slab(const NormArgs &A, const MapPlan &P, const double2 *part, F result) {
+    const int parts = P.splits * P.col_blocks, step = 1 << P.join_log, lane = threadIdx.x & (step - 1), teams = blockDim.x >> P.join_log;
+#pragma unroll 1
+    for (int g0 = 0; g0 < A.G; g0 += teams) {                        // (every lane takes every turn: the exchange needs them all)
+        const int g = g0 + (threadIdx.x >> P.join_log);
+        const double2 *p = part + (int64_t)(g < A.G ? g : A.G - 1) * parts;
+        double s = 0.0, q = 0.0;
+#pragma unroll 1
+        for (int k = lane; k < parts; k += 8 * step) {
+            double2 t[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) t[j] = p[k + j * step < parts ? k + j * step : k];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (k + j * step < parts) { s += t[j].x; q += t[j].y; }
+        }
+        lanes_sum2(s, q, P.join_log);
+        if (g < A.G && lane == 0) result(g, s, q);
+    }
 }
 // s of a slab: its first element, after the mask
 template <bool DROP> __device__ __forceinline__ double slab_shift(const NormArgs &A, const Draw &d, int64_t n) {
@@ -582,15 +604,15 @@ template <int V> __device__ __forceinline__ void normalise(const Constants<V> &k
 #pragma unroll
     for (int e = 0; e < 8; e++) { const int i = V == 2 ? 0 : e; v[e] = ((v[e] - k.mean[i]) - k.rest[i]) * k.rstd[i]; }
 }
-// the results of a span of slab n, with the slab's statistics at `stats`
-template <int V, bool DROP, bool STREAM> __device__ __forceinline__ void span_apply(const NormArgs &A, const MapPlan &P, const Draw &d, const Column &c, const Span &t, int64_t n, const double2 *stats) {
+// the results of a span of slab n; ready() -> the slab's statistics
+template <int V, bool DROP, bool STREAM, class F> __device__ __forceinline__ void span_apply(const NormArgs &A, const MapPlan &P, const Draw &d, const Column &c, const Span &t, int64_t n, F ready) {
     const T *x = (const T *)A.x + n * A.x_stride + t.base;
     T *y = (T *)A.out + n * A.size + t.base;
     int off = t.off;
     Chunk<DT> v;
     if (t.lim >= 8) v = span_load<STREAM>(x, t, off);
     Constants<V> k;
-    load_constants<V>(A, P, stats, c.col, k);
+    load_constants<V>(A, P, ready(), c.col, k);
 #pragma unroll
     for (int e = 0; e < 8; e++) k.w[e] *= k.rstd[V == 2 ? 0 : e];
     const auto result = [&](const Chunk<DT> &chunk, float (&f)[8]) {
@@ -612,13 +634,27 @@ template <int V, bool DROP, bool STREAM> __device__ __forceinline__ void span_ap
     }
     if (V == 1 && off < t.lim) { result(load_chunk<DT>(x + off, t.lim - off), f); store_chunk<DT>(y + off, t.lim - off, f); }
 }
-template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(512) void k_map_apply(NormArgs A, MapPlan P) {
+// part: the sums' partial pairs, joined by every workgroup for itself (the first of a slab writes the statistics down), or null: the statistics are there already
+template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(512) void k_map_apply(NormArgs A, MapPlan P, const double2 *part) {
+    extern __shared__ double2 lds[];
     const Column c = my_column(P, blockIdx.y);
     const Span t = my_span(A, P, c, P.apply_rows);
     Draw d = {};
     if (DROP) d = make_draw(A.rng, A.site, A.cut);
 #pragma unroll 1
-    for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) span_apply<V, DROP, STREAM>(A, P, d, c, t, n, A.stats + n * A.G);
+    for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) 
+        span_apply<V, DROP, STREAM>(A, P, d, c, t, n, [&]() -> const double2 * {
+            if (!part) return A.stats + n * A.G;
+            const double shift = slab_shift<DROP>(A, d, n);
+            const bool first = A.stats && blockIdx.x == 0 && blockIdx.y == 0;
+            __syncthreads();
+            join_slab(A, P, part + n * A.G * P.splits * P.col_blocks, [&](int g, double sum, double squares) {
+                lds[g] = finish_stats(A, shift, sum, squares);
+                if (first) A.stats[n * A.G + g] = lds[g];
+            });
+            __syncthreads();
+            return lds;
+        });
 }
 
 // backward: s1, s2 += the sums of dz and dz xh of a span of slab n, per virtual channel; k: the thread's constants, left for the caller
@@ -703,16 +739,16 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_su
 }
 // second launch: the first workgroups join the splits of each (n, g) into {mean of w dz, mean of w dz xh}, the others the parameter gradients
 __global__ __launch_bounds__(1024) void k_map_back_join(NormArgs A, int splits, const double2 *part, const float *params, int param_rows, int join_blocks, double2 *means, void *dw, void *db) {
-    __shared__ double lds[64][17];
+    __shared__ double lds[64 * 17];
     if ((int)blockIdx.x >= join_blocks) { param_columns(A, params, param_rows, blockIdx.x - join_blocks, dw, db, lds); return; }
     for (int64_t item = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 6); item < A.N * A.G; item += (int64_t)join_blocks * 16) {
         const double2 t = join_splits(part + item * splits, splits);
         if ((threadIdx.x & 63) == 0) means[item] = double2{t.x * A.inv_count, t.y * A.inv_count};
     }
 }
-// dx of a span of slab n; means[g] = scale times {sum of w dz, sum of w dz xh}
-template <int V, bool DROP, bool STREAM>
-__device__ __forceinline__ void span_back_apply(const NormArgs &A, const MapPlan &P, const Draw &d, const Column &c, const Span &t, int64_t n, const double2 *means, double scale) {
+// dx of a span of slab n; ready() -> per group {sum of w dz, sum of w dz xh}, which times `scale` are the means
+template <int V, bool DROP, bool STREAM, class F>
+__device__ __forceinline__ void span_back_apply(const NormArgs &A, const MapPlan &P, const Draw &d, const Column &c, const Span &t, int64_t n, double scale, F ready) {
     const T *x = (const T *)A.x + n * A.x_stride + t.base, *dy = (const T *)A.dy + n * A.dy_stride + t.base;
     T *dx = (T *)A.out + n * A.size + t.base;
     int off = t.off;
@@ -722,6 +758,7 @@ __device__ __forceinline__ void span_back_apply(const NormArgs &A, const MapPlan
     load_constants<V>(A, P, A.stats + n * A.G, c.col, k);
     float m1[V == 2 ? 1 : 8], m2[V == 2 ? 1 : 8];
     {
+        const double2 *means = ready();
         Channel ch(A, 8 * c.col);
 #pragma unroll
         for (int e = 0; e < (V == 2 ? 1 : 8); e++) { const double2 m = means[ch.g]; m1[e] = (float)(m.x * scale); m2[e] = (float)(m.y * scale); ch.next(A); }
@@ -755,13 +792,28 @@ __device__ __forceinline__ void span_back_apply(const NormArgs &A, const MapPlan
         store_chunk<DT>(dx + off, t.lim - off, f);
     }
 }
-template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(512) void k_map_back_apply(NormArgs A, MapPlan P, const double2 *means) {
+// part: the sums' partial pairs, joined by every workgroup for itself, and null: the means are there already.  The first P.param_z slices of the grid join the parameter gradients.
+template <int V, bool DROP, bool STREAM>
+__global__ __launch_bounds__(512) void k_map_back_apply(NormArgs A, MapPlan P, const double2 *part, const double2 *means, const float *params, int param_rows, void *dw, void *db) {
+    extern __shared__ double2 lds[];
+    if ((int)blockIdx.z < P.param_z) {
+        const int block = ((int)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+        if (block * 16 < 2 * A.C) param_columns(A, params, param_rows, block, dw, db, (double *)lds);
+        return;
+    }
     const Column c = my_column(P, blockIdx.y);
     const Span t = my_span(A, P, c, P.apply_rows);
     Draw d = {};
     if (DROP) d = make_draw(A.rng, A.site, A.cut);
 #pragma unroll 1
-    for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) span_back_apply<V, DROP, STREAM>(A, P, d, c, t, n, means + n * A.G, 1.0);
+    for (int64_t n = blockIdx.z - P.param_z; n < A.N; n += gridDim.z - P.param_z)
+        span_back_apply<V, DROP, STREAM>(A, P, d, c, t, n, part ? A.inv_count : 1.0, [&]() -> const double2 * {
+            if (!part) return means + n * A.G;
+            __syncthreads();
+            join_slab(A, P, part + n * A.G * P.splits * P.col_blocks, [&](int g, double s1, double s2) { lds[g] = double2{s1, s2}; });
+            __syncthreads();
+            return lds;
+        });
 }
 
 // ---- slabs that one workgroup goes over by itself: the same passes in one launch, the second reading out of the nearer caches.  `lds`: the join's space, then G pairs.
@@ -784,7 +836,7 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_slab_forwar
             if (A.stats) A.stats[n * A.G + g] = groups[g];
         }
         __syncthreads();
-        span_apply<V, DROP, false>(A, P, d, c, t, n, groups);
+        span_apply<V, DROP, false>(A, P, d, c, t, n, [&] { return groups; });
     }
 }
 template <int V, bool DROP> __global__ __launch_bounds__(512) void k_slab_backward(NormArgs A, MapPlan P, float *params) {
@@ -806,7 +858,7 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_slab_backwa
         }
         join_groups<V>(s1, s2, A, P, c, lds, groups, 1);
         __syncthreads();
-        span_back_apply<V, DROP, false>(A, P, d, c, t, n, groups, A.inv_count);
+        span_back_apply<V, DROP, false>(A, P, d, c, t, n, A.inv_count, [&] { return groups; });
     }
 }
 
@@ -837,9 +889,11 @@ template <int V, bool DROP> void map_forward_v(const NormArgs &a, const MapLaunc
     const size_t lds = (size_t)m.NT * (V == 2 ? 16 : 128);
     if (m.slab) { k_slab_forward<V, DROP><<<m.sums, m.NT, lds + a.G * 16, s>>>(a, m.P); return; }
     k_map_sums<V, DROP><<<m.sums, m.NT, lds, s>>>(a, m.P, part);
-    k_map_stats<DROP><<<m.stat_blocks, 256, 0, s>>>(a, m.P.splits * m.P.col_blocks, part);
-    if (m.stream) k_map_apply<V, DROP, true><<<m.apply, m.NT, 0, s>>>(a, m.P);
-    else k_map_apply<V, DROP, false><<<m.apply, m.NT, 0, s>>>(a, m.P);
+    if (!m.joins) k_map_stats<DROP><<<m.stat_blocks, 256, 0, s>>>(a, m.P.splits * m.P.col_blocks, part);
+    const size_t stats = m.joins ? (size_t)a.G * 16 : 0;
+    const double2 *join = m.joins ? part : nullptr;
+    if (m.stream) k_map_apply<V, DROP, true><<<m.apply, m.NT, stats, s>>>(a, m.P, join);
+    else k_map_apply<V, DROP, false><<<m.apply, m.NT, stats, s>>>(a, m.P, join);
 }
 void map_forward(const NormArgs &a, const MapLaunch &m, double2 *part, hipStream_t s) {
     if (one_group(a)) a.cut ? map_forward_v<2, true>(a, m, part, s) : map_forward_v<2, false>(a, m, part, s);
@@ -852,11 +906,24 @@ template <int V, bool DROP> void map_backward_v(const NormArgs &a, const MapLaun
         return;
     }
     k_map_back_sums<V, DROP><<<m.sums, m.NT, (size_t)m.NT * 128, s>>>(a, m.P, part, sums);
-    const int64_t items = a.N * a.G;
-    const int join = (int)(items < 16 * 4096 ? (items + 15) / 16 : 4096);
-    k_map_back_join<<<join + (sums ? column_blocks(a) : 0), 1024, 0, s>>>(a, m.P.splits * m.P.col_blocks, part, sums, m.param_rows, join, means, dw, db);
-    if (m.stream) k_map_back_apply<V, DROP, true><<<m.apply, m.NT, 0, s>>>(a, m.P, means);
-    else k_map_back_apply<V, DROP, false><<<m.apply, m.NT, 0, s>>>(a, m.P, means);
+    MapPlan P = m.P;
+    dim3 grid = m.apply;
+    size_t lds = 0;
+    if (m.joins) {
+        if (sums) {
+            P.param_z = (int)((column_blocks(a) + grid.x * grid.y - 1) / (grid.x * grid.y));
+            grid.z += P.param_z;
+            lds = (size_t)(m.NT / 16) * 17 * 8;
+        }
+        if (lds < (size_t)a.G * 16) lds = (size_t)a.G * 16;
+    } else {
+        const int64_t items = a.N * a.G;
+        const int join = (int)(items < 16 * 4096 ? (items + 15) / 16 : 4096);
+        k_map_back_join<<<join + (sums ? column_blocks(a) : 0), 1024, 0, s>>>(a, m.P.splits * m.P.col_blocks, part, sums, m.param_rows, join, means, dw, db);
+    }
+    const double2 *join = m.joins ? part : nullptr;
+    if (m.stream) k_map_back_apply<V, DROP, true><<<grid, m.NT, lds, s>>>(a, P, join, means, sums, m.param_rows, dw, db);
+    else k_map_back_apply<V, DROP, false><<<grid, m.NT, lds, s>>>(a, P, join, means, sums, m.param_rows, dw, db);
 }
 void map_backward(const NormArgs &a, const MapLaunch &m, double2 *part, double2 *means, float *sums, void *dw, void *db, hipStream_t s) {
     if (one_group(a)) a.cut ? map_backward_v<2, true>(a, m, part, means, sums, dw, db, s) : map_backward_v<2, false>(a, m, part, means, sums, dw, db, s);
