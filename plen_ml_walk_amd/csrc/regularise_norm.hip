@@ -324,6 +324,14 @@ template <int V, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT
                 db[e] += dz[e]; dw[e] = fmaf(dz[e], xh[e], dw[e]);
             }
         }
+        const int64_t here = n;
+        n += (int64_t)gridDim.x * P.rb;
+        if (turn + 1 < P.trips) {                               // the next row's, while this one's sums are joined
+            row = n < A.N ? n : A.N - 1;
+            px = (const T *)A.x + row * A.x_stride;
+            x = load_inside<V, DT, STREAM>(px, c0, A.C); g = load_inside<V, DT, STREAM>((const T *)A.dy + row * A.dy_stride, c0, A.C);
+            st = A.stats[row * A.G + g0];
+        }
         team_sum2<NT>(s, q, P.team_log, turn, lds);
         if (on) {
             const float m1 = s * (float)A.inv_count, m2 = q * (float)A.inv_count;
@@ -331,14 +339,7 @@ template <int V, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT
             for (int e = 0; e < 8; e++) {
                 gw[e] = m.keep(e, rstd * (gw[e] - m1 - xh[e] * m2));
             }
-            row_store<V, STREAM>((T *)A.out + n * A.C + c0, valid[0], gw);
-        }
-        n += (int64_t)gridDim.x * P.rb;
-        if (turn + 1 < P.trips) {
-            row = n < A.N ? n : A.N - 1;
-            px = (const T *)A.x + row * A.x_stride;
-            x = load_inside<V, DT, STREAM>(px, c0, A.C); g = load_inside<V, DT, STREAM>((const T *)A.dy + row * A.dy_stride, c0, A.C);
-            st = A.stats[row * A.G + g0];
+            row_store<V, STREAM>((T *)A.out + here * A.C + c0, valid[0], gw);
         }
     }
     if (!part) return;
