@@ -46,6 +46,9 @@ __device__ __forceinline__ double2 finish_stats(const NormArgs &A, double s, dou
     if (var < 0.0) var = 0.0;
     return double2{s + m, A.scale * inverse_sqrt(fma(var, A.scale * A.scale, A.eps))};
 }
+// v - (mean + rest), the mean in two words, for a result.  What the first leaves out is below 2^-25 of the mean: for 16-bit elements, whose own steps are 2^-11 of theirs or more, it is
+// left out here too (one of about 40 instructions an element).  The backward pass, which has a gate to decide, takes both.
+__device__ __forceinline__ float from_mean(float v, float mean, float rest) { return DT == PLENREG_F32 ? (v - mean) - rest : v - mean; }
 __device__ __forceinline__ void write_used(const NormArgs &A) {
     if (A.used && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) { A.used[0] = A.rng[0]; A.used[1] = A.rng[1]; }
 }
@@ -125,9 +128,9 @@ template <int NT, typename F> __device__ __forceinline__ void team_sum2(F &a, F 
         double2 *p = lds[turn & 1];
         if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = double2{(double)a, (double)b};
         __syncthreads();
-        const int waves = 1 << (log - 6), w0 = (threadIdx.x >> log) << (log - 6);
-        double s = 0.0, q = 0.0;
-        for (int k = 0; k < waves; k++) { s += p[w0 + k].x; q += p[w0 + k].y; }
+        const double2 wave = p[(threadIdx.x >> log << (log - 6)) + (threadIdx.x & ((1 << (log - 6)) - 1))];          // (a wave's lanes look at all of the team's)
+        double s = wave.x, q = wave.y;
+        lanes_sum2(s, q, log - 6);
         a = (F)s; b = (F)q;
     }
 }
@@ -255,12 +258,14 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
         double s = 0.0, q = 0.0;
 #pragma unroll
         for (int k = 0; k < K; k++) {
+            double sk = 0.0, qk = 0.0;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                if ((V ? valid[k] : valid[k] - e) <= 0) v[k][e] = first;                     // what is not there adds nothing
+                if (!V && e >= valid[k]) v[k][e] = first;                                    // what is not there adds nothing
                 const double t = (double)v[k][e] - shift;
-                s += t; q = fma(t, t, q);
+                sk += t; qk = fma(t, t, qk);
             }
+            s += !V || valid[k] ? sk : 0.0; q += !V || valid[k] ? qk : 0.0;
         }
         team_sum2<NT>(s, q, P.team_log, turn, lds);
         const double2 st = finish_stats(A, shift, s, q);
@@ -271,7 +276,7 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
             for (int k = 0; k < K; k++) {
                 if (!valid[k]) continue;
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[k][e] = ((v[k][e] - mean) - rest) * rstd * w[k][e] + b[k][e];
+                for (int e = 0; e < 8; e++) v[k][e] = from_mean(v[k][e], mean, rest) * rstd * w[k][e] + b[k][e];
                 activate(v[k], A.act);
                 row_store<V, STREAM>((T *)A.out + n * A.C + c[k], valid[k], v[k]);
             }
@@ -619,7 +624,7 @@ template <int V, bool DROP, bool STREAM, class F> __device__ __forceinline__ voi
     const auto result = [&](const Chunk<DT> &chunk, float (&f)[8]) {
         unpack(chunk, Mask<DROP ? V : 0>(d, n * A.size + t.base + off), f);
 #pragma unroll
-        for (int e = 0; e < 8; e++) f[e] = ((f[e] - k.mean[V == 2 ? 0 : e]) - k.rest[V == 2 ? 0 : e]) * k.w[e] + k.b[e];
+        for (int e = 0; e < 8; e++) f[e] = from_mean(f[e], k.mean[V == 2 ? 0 : e], k.rest[V == 2 ? 0 : e]) * k.w[e] + k.b[e];
         activate(f, A.act);
     };
     float f[8];
