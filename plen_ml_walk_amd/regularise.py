@@ -65,7 +65,7 @@ def load():
 
 def _load_nodes():
     """The autograd nodes (csrc/regularise_torch.cpp), bound to the HIP library's entry points."""
-    global _nodes
+    global _nodes, _quick_dropout, _quick_norm, _quick_layer
     lib = load()
     path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc", "plenreg_torch.so")
     if not os.path.exists(path):
@@ -75,7 +75,16 @@ def _load_nodes():
     spec.loader.exec_module(nodes)
     nodes.bind(*(C.cast(f, C.c_void_p).value for f in (lib.plenreg_dropout, lib.plenreg_norm_forward, lib.plenreg_norm_backward, lib.plenreg_norm_workspace)))
     _nodes = nodes
+    _quick_dropout, _quick_norm, _quick_layer = nodes.quick_dropout, nodes.quick_norm, nodes.quick_layer
     return nodes
+
+
+def _not_loaded(*args):
+    return None
+
+
+# natively: a call whose arguments pass every check below is launched at once; None where one does not, or before the first call on a device
+_quick_dropout = _quick_norm = _quick_layer = _not_loaded
 
 
 def new_rng(device, seed):
@@ -174,6 +183,9 @@ def dropout(x, p, rng, site=0):
     float16, any shape of up to 2^35 elements; rng: {seed, calls} (`new_rng`), read and not advanced; site: the number of this place in the model.  Returns a
     contiguous tensor of x's type; the gradient with respect to x draws the same mask again.  Rows of contiguous elements a constant stride apart (a column
     slice) are read in place, other layouts are copied first."""
+    y = _quick_dropout(x, p, rng, site)
+    if y is not None:
+        return y
     _check_x(x)
     cut, site = _check_draw(x, p, rng, site), int(site)
     if x.device.type == "cpu":
@@ -188,6 +200,9 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="relu"):
     weight, bias: [C] of one float type (it may differ from x's) or None.  Returns a contiguous tensor of x's type; differentiable (once) in x, weight and
     bias.  At most 8192 channels where there are positions, 32768 for [N, C].  Each x[n] has to be contiguous (the stride between them is free: a column slice of a
     wider matrix is read in place); what is laid out otherwise is copied first."""
+    y = _quick_norm(x, groups, weight, bias, eps, act)
+    if y is not None:
+        return y
     _check_x(x)
     groups, eps = _check_norm(x, groups, weight, bias, eps, act), float(eps)
     if x.device.type == "cpu":
@@ -197,6 +212,9 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="relu"):
 
 def dropout_norm_act(x, p, rng, groups, weight=None, bias=None, site=0, eps=1e-5, act="relu"):
     """act(group_norm(dropout(x)) * weight + bias) in one pass: `group_norm_act` of `dropout(x, p, rng, site)`, which is not rounded in between."""
+    y = _quick_layer(x, p, rng, groups, weight, bias, site, eps, act)
+    if y is not None:
+        return y
     _check_x(x)
     cut, site = _check_draw(x, p, rng, site), int(site)
     groups, eps = _check_norm(x, groups, weight, bias, eps, act), float(eps)

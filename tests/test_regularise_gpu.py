@@ -459,3 +459,14 @@ def test_statistics_joined_in_the_results_launch_or_in_one_of_their_own(shape, g
     x, dy, w, b = _case(shape, groups, torch.bfloat16)
     _check(x, dy, w, b, groups, "relu", 0.1, _rng())
     _check(x, dy, None, None, groups, "silu", None, None)
+
+
+def test_arguments_of_other_number_types_mean_the_same():
+    """What the native checks do not take as it comes (whole numbers, numpy's, a step of p) goes through the checks in Python to the same result."""
+    x, rng = torch.randn(6, 48, generator=_gen(1)).cuda(), _rng()
+    w = torch.randn(48, generator=_gen(2)).cuda()
+    assert torch.equal(R.dropout(x, 1, rng), R.dropout(x, 1.0, rng)) and torch.equal(R.dropout(x, np.float32(0.25), rng, np.int64(2)), R.dropout(x, 0.25, rng, 2))
+    assert torch.equal(R.group_norm_act(x, np.int32(3), w, None, 1, "silu"), R.group_norm_act(x, 3, w, None, 1.0, "silu"))
+    assert torch.equal(R.dropout_norm_act(x, 0, rng, 3.0, w, eps=np.float64(1e-3)), R.dropout_norm_act(x, 0.0, rng, 3, w, eps=1e-3))
+    for p in (2.0 ** -17, 3 * 2.0 ** -17, 5 * 2.0 ** -17):                # half steps: rounded to even by both
+        assert torch.equal(R.dropout(x, p, rng), R.dropout(x, np.float32(p), rng))
