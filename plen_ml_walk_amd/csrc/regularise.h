@@ -183,7 +183,7 @@ struct RowPlan { int team_log, gb, rb, trips; float inv_gb; };
 struct RowLaunch { RowPlan P; int K, NT; dim3 grid; bool stream; };
 // many positions.  A slab as `rows` rows of `ncol` chunk columns (2^q_log positions to a row); bcol columns in a workgroup, R rows per turn of it; rows_per rows in a
 // workgroup of the sums, apply_rows in one of the result; 2^lanes_log lanes join one group
-struct MapPlan { int q_log, ncol, bcol, col_blocks, R, splits, lanes_log, join_log, param_z; int64_t rows, rows_per, apply_rows; float inv_bcol; };
+struct MapPlan { int q_log, ncol, bcol, col_blocks, R, splits, lanes_log, chan_log, join_log, param_z; int64_t rows, rows_per, apply_rows; float inv_bcol; };
 // slab: one workgroup does a slab by itself (the grid is `sums`, slabs along y)
 struct MapLaunch { MapPlan P; dim3 sums, apply; int NT, param_rows; unsigned stat_blocks; bool stream, slab, joins; };
 

@@ -113,6 +113,12 @@ static int fill_threads(int ncol, int lo, int hi) {
     }
     return best;
 }
+// log of a power of two of lanes: at most `there`, one wave's, and no more than there are entries
+static int lanes_for(int there, int entries) {
+    int log = 0;
+    while (log < 6 && 2 << log <= there && 1 << log < entries) log++;
+    return log;
+}
 static MapLaunch map_plan(const PlenRegNorm &a, bool backward) {
     MapLaunch m;
     const int D = a.C / a.G;
@@ -143,9 +149,10 @@ static MapLaunch map_plan(const PlenRegNorm &a, bool backward) {
     m.P.splits = (int)div_up(m.P.rows, m.P.rows_per);
     m.P.apply_rows = (apply_turns < most ? apply_turns : most) * turn;
     const int64_t row_blocks = div_up(m.P.rows, m.P.apply_rows);
-    // about four entries of a group for each lane that joins it
-    m.P.lanes_log = log2_up(div_up((int64_t)m.P.R * (a.C % 8 || D % 8 ? D : D / 8), 4));
-    if (m.P.lanes_log > 6) m.P.lanes_log = 6;
+    // lanes that join a group (a channel) of a workgroup's entries: all of them at a time where there are as many
+    const int units = a.C % 8 == 0 && D % 8 == 0 ? D / 8 : D >= 8 ? (D + 14) / 8 : D, local = (int)(m.P.q_log || m.P.bcol * 8 > a.C ? a.C : m.P.bcol * 8);
+    m.P.lanes_log = lanes_for(m.NT / a.G, (units * m.P.R) << m.P.q_log);
+    m.P.chan_log = lanes_for(m.NT / local, m.P.R << m.P.q_log);
     // slabs beyond what fills the chip (and the grid's limit of 65535) are walked by the workgroups
     int64_t z = div_up(2048, m.P.splits);
     m.sums = dim3((unsigned)m.P.splits, (unsigned)m.P.col_blocks, (unsigned)(a.N < z ? a.N : z));
@@ -162,8 +169,7 @@ static MapLaunch map_plan(const PlenRegNorm &a, bool backward) {
     // 1 x 4096 x 512 16384 13.1 / 11.3; both passes 4 x 1089 x 195 455 36.4 / 38.5, 2275 37.2 / 39.0, 8 x 4096 x 320 2048 65.5 / 66.4, 4096 67.8 / 66.7
     m.joins = (int64_t)a.G * m.P.splits * m.P.col_blocks <= (backward ? 2560 : 4096);
     m.P.param_z = 0;
-    m.P.join_log = log2_up(m.NT / a.G + 1) - 1;
-    m.P.join_log = m.P.join_log < 0 ? 0 : m.P.join_log > 6 ? 6 : m.P.join_log;
+    m.P.join_log = lanes_for(m.NT / a.G, 64);
     m.stream = streams(a);
     m.stat_blocks = (unsigned)(a.N * a.G < 4 * 65536 ? div_up(a.N * a.G, 4) : 65536);
     return m;
