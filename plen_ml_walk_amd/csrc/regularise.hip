@@ -132,10 +132,11 @@ static MapLaunch map_plan(const PlenRegNorm &a, bool backward) {
     m.P.bcol = (int)div_up(m.P.ncol, m.P.col_blocks);
     m.P.inv_bcol = 1.f / (float)m.P.bcol;
     // one workgroup per slab: one launch instead of three, and the slab is read once from memory; but only as many compute units work as there are slabs.
-    // Measured (us, slab / split; N x L x C bf16): forward 8 x 32 x 320 7.9 / 13.7, 8 x 1024 x 32 9.4 / 11.9, 8 x 128 x 320 12.6 / 13.8, 8 x 512 x 195 28 / 17, 256 x 512 x 195 46 / 46;
-    // backward 8 x 512 x 32 15.5 / 14.5, 8 x 128 x 195 28.5 / 24.8, 64 x 128 x 320 29 / 32, 64 x 512 x 320 70 / 48, 256 x 512 x 320 85 / 127.
+    // Measured (us, slab / split; N x L x C bf16): forward 8 x 32 x 320 6.3 / 8.2, 8 x 128 x 195 8.1 / 8.5, 8 x 1024 x 32 7.5 / 6.7, 64 x 128 x 320 10.8 / 11.0, 64 x 512 x 128 12.4 / 9.5,
+    // 256 x 128 x 320 13.6 / 16.5, 256 x 512 x 320 42.9 / 44.2; both passes 8 x 32 x 320 20.3 / 21.9 (1.9 of it forward), 8 x 512 x 32 18.7 / 17.4, 64 x 128 x 195 35.2 / 32.4,
+    // 256 x 32 x 320 23.5 / 38.6, 256 x 512 x 128 56.1 / 56.9, 256 x 512 x 320 120 / 167.
     m.slab = m.P.bcol <= 448 && m.P.col_blocks == 1 && a.G <= 512
-             && (backward ? size <= 16384 || (a.N >= 64 && size <= 49152) || (a.N >= 256 && size <= 262144) : size <= 32768 || (a.N >= 256 && size <= 98304));
+             && ((a.N >= 256 && size <= 262144) || (backward ? size <= 8192 : size <= 25600 || (a.N >= 64 && size <= 40960)));
     const int64_t threads = div_up(chunks, 64) * 64;
     m.NT = m.slab ? fill_threads(m.P.bcol, threads < 448 ? (int)threads : 448, 448) : fill_threads(m.P.bcol, 256, 512);
     m.P.R = m.NT / m.P.bcol;
