@@ -650,6 +650,11 @@ class TD3Agent(object):
                 net.load_state_dict(sd)
 
 
+def has_critic_norm(filename):
+    """Was the checkpoint `filename` saved by an agent with critic_norm?  (Dropout alone leaves no trace in it: such files and a plain agent's are alike.)"""
+    return "norm1.weight" in torch.load(filename + "_critic", map_location="cpu", weights_only=True)
+
+
 def evaluate_policy(policy, env_name, seed, eval_episodes=10, render=False):
     """Average undiscounted return over `eval_episodes` episodes, reference td3.py:381-415."""
     from . import gym_compat

@@ -11,7 +11,7 @@ import os
 import numpy as np
 import torch
 
-from .td3 import TD3Agent
+from .td3 import TD3Agent, has_critic_norm
 from .vec_env import PlenVecEnv
 
 
@@ -51,7 +51,7 @@ def evaluate(policy, num_envs=64, episodes_per_env=1, dtype=torch.float32, devic
 
 
 def load_policy(path, device=None):
-    policy = TD3Agent(26, 18, 1.0, device=device, data_parallel=False)
+    policy = TD3Agent(26, 18, 1.0, device=device, data_parallel=False, critic_norm=not path.endswith(".npz") and has_critic_norm(path))
     if path.endswith(".npz"):
         policy.load_arrays(np.load(path))
     else:

@@ -105,6 +105,15 @@ def test_checkpoint_goes_on_with_masks_not_drawn_before(tmp_path):
     assert torch.isfinite(other.last_critic_loss)
 
 
+@pytest.mark.parametrize("dropout,norm", KINDS + [(0.0, False)])
+def test_the_evaluation_command_loads_every_kind_of_checkpoint(tmp_path, dropout, norm):
+    from plen_ml_walk_amd.walk_eval import load_policy
+    agent = _agent(dropout, norm)
+    agent.save(str(tmp_path / "run"))
+    policy, state = load_policy(str(tmp_path / "run"), device="cpu"), torch.randn(5, 26)
+    assert torch.equal(policy.select_action_batch(state), agent.select_action_batch(state))
+
+
 def test_two_ranks_share_gradients_and_draw_their_own_masks(tmp_path):
     out = str(tmp_path / "reg")
     cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node", "2", "--master-addr", "127.0.0.1", "--master-port", str(_free_port()),
