@@ -41,7 +41,8 @@ __device__ __forceinline__ double inverse_sqrt(double v) {
 }
 // sums of (x - s), (x - s)^2 -> the pair that NormArgs.stats holds
 __device__ __forceinline__ double2 finish_stats(const NormArgs &A, double s, double sum, double squares) {
-    const double m = sum * A.inv_count;
+    double m = sum * A.inv_count;
+    m = fma(fma(-m, A.count, sum), A.inv_count, m);          // the quotient to its last bit: a group that is constant, or wholly dropped, beside a slab's other first element has exactly its mean
     double var = fma(-m, m, squares * A.inv_count);
     if (var < 0.0) var = 0.0;
     return double2{s + m, A.scale * inverse_sqrt(fma(var, A.scale * A.scale, A.eps))};

@@ -471,3 +471,28 @@ def test_arguments_of_other_number_types_mean_the_same():
     assert torch.equal(R.dropout_norm_act(x, 0, rng, 3.0, w, eps=np.float64(1e-3)), R.dropout_norm_act(x, 0.0, rng, 3, w, eps=1e-3))
     for p in (2.0 ** -17, 3 * 2.0 ** -17, 5 * 2.0 ** -17):                # half steps: rounded to even by both
         assert torch.equal(R.dropout(x, p, rng), R.dropout(x, np.float32(p), rng))
+
+
+@pytest.mark.parametrize("shape,groups", [((6, 512), 4), ((3, 50, 24), 3), ((300, 3, 2), 2), ((1, 40000, 16), 4), ((2, 777, 195), 13), ((3, 700, 30), 10)], ids=ids)
+@pytest.mark.parametrize("value", [0.0, 1.7, -123.456])
+def test_constant_groups_beside_others(shape, groups, value):
+    """A group without variance has exactly its value as its mean, whatever the other groups of its slab hold: y = act(b) (to b's product), gates of z = 0 are shut."""
+    x, dy, w, b = _case(shape, groups, torch.float32)
+    with torch.no_grad():
+        v = x.view(shape[0], -1, groups, shape[-1] // groups)
+        v[:, :, 1::2] = value
+    for act in ("none", "relu", "silu"):
+        y, grads = _check(x, dy, w, None, groups, act, None, None)
+        assert not y.detach().view(v.shape)[:, :, 1::2].any() and not grads["dw"].view(groups, -1)[1::2].any()
+        _check(x, dy, w, b, groups, act, None, None)
+        if value == 0.0:
+            _check(x, dy, w, None, groups, act, 0.3, _rng())
+
+
+@pytest.mark.parametrize("shape,groups", [((300, 3, 2), 2), ((40, 2, 24), 3), ((300, 2, 2504), 313), ((50, 30), 10)], ids=ids)
+def test_groups_that_the_mask_leaves_empty_beside_others(shape, groups):
+    x, dy, w, b = _case(shape, groups, torch.float32)
+    assert not O.keep(shape, 0.9, _rng(), 2).view(shape[0], -1, groups, shape[-1] // groups).any(3).any(1).all()          # some are
+    for act in ("none", "relu", "silu"):
+        _check(x, dy, w, None, groups, act, 0.9, _rng())
+        _check(x, dy, w, b, groups, act, 0.9, _rng())
