@@ -1,5 +1,5 @@
 // regularise.hip -- the C ABI of include/plenreg.h (argument checks, launch plans) and the dropout kernel; the group-norm kernels are in regularise_norm.hip.
-// All of it is bound by memory traffic at size and by launch latency when small.
+// Small calls are bound by launch latency, dropout and long slabs by memory traffic, wide layers with dropout and SiLU by vector issue.
 #include "regularise.h"
 
 #define DROPOUT_SMALL (1 << 18)
@@ -9,7 +9,8 @@
 #define ROW_MAX_BACKWARD 4096
 
 // ---- dropout.  U chunks per thread: all loads are issued before the first mask is drawn.  In rows that are not contiguous (ROWS) a chunk that crosses
-//      the end of a row is loaded element by element.
+//      the end of a row is loaded element by element.  Memory: 32768 x 4096 bf16 77 us = 7.0 TB/s read and written, with the reads past the caches (92 with them in the caches; with the
+//      writes past them too the kernel alone is slower).  100 x 256 f32 2.3 us: the launch.
 struct DropArgs { const void *x; void *y; const uint64_t *rng; uint64_t *used; int64_t rows, cols, x_stride; uint32_t cut; int site; float scale; };
 template <int DT, int U, bool ROWS> __global__ __launch_bounds__(256) void k_dropout(DropArgs A) {
     typedef typename Elem<DT>::T T;
@@ -138,7 +139,7 @@ static MapLaunch map_plan(const PlenRegNorm &a, bool backward) {
     const int64_t threads = div_up(chunks, 64) * 64;
     m.NT = m.slab ? fill_threads(m.P.bcol, threads < 448 ? (int)threads : 448, 448) : fill_threads(m.P.bcol, 256, 512);
     m.P.R = m.NT / m.P.bcol;
-    // 2 workgroups per compute unit, or 4 where their threads then still have 16 chunks each; each thread in whole turns of 2 rows.  (8 x 4096 x 320: 512 workgroups 9.2 + 9.5 us,
+    // 2 workgroups per compute unit, or 4 where their threads then still have 16 chunks each; each thread in whole turns of 2 rows.  (Before the joins' present form, 8 x 4096 x 320: 512 workgroups 9.2 + 9.5 us,
     // 1024: 10.8 + 9.8; 2 x 262144 x 128: 47 + 42 and 40 + 43)
     const int64_t blocks = a.N * chunks >= (int64_t)1 << 22 ? 1024 : 512;
     const int64_t turn = (int64_t)m.P.R * 2, turns = div_up(m.P.rows, turn), groups = a.N * m.P.col_blocks;

@@ -214,6 +214,8 @@ template <int V> __device__ __forceinline__ void row_params(const NormArgs &A, c
     }
 }
 
+// Forward.  Bound by latency when small (100 x 512 f32: 2.8 us, a launch alone is 2.3), by vector issue when large: 16384 x 2048 bf16 with dropout and SiLU 34.6 us = 3.9 TB/s, 26
+// instructions an element, of them 2.4 64-bit multiply-adds of the generator and 2 transcendentals at a quarter of the rate; its 134 MB alone would be 26 us.  4096 x 512 f32 6.2 us.
 template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT) void k_row_forward(NormArgs A, RowPlan P) {
     __shared__ double2 lds[2][NT / 64];
     const RowPlace p = row_place<NT>(A, P);
@@ -286,7 +288,9 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
     }
 }
 
-// backward of the rows.  Each workgroup leaves one row of partial parameter gradients: part[blockIdx.x][0 / 1][C] = dw, db of its rows, summed over its teams in LDS.
+// Backward of the rows: one chunk a lane, since x, dy, dz, two parameters and their two gradients are held per element (two chunks: 200 registers, 59 us where this takes 53).  Sums
+// of a row in 32 bits: at most 4096 elements in a tree.  16384 x 2048 bf16 with dropout and SiLU 53 us, vector issue (47 instructions an element; its 201 MB alone would be 39 us); 4096 x 512
+// f32 10 us, 100 x 512 6 us.  Each workgroup leaves one row of partial parameter gradients: part[blockIdx.x][0 / 1][C] = dw, db of its rows, summed over its teams in LDS.
 template <int V, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT) void k_row_backward(NormArgs A, RowPlan P, float *part) {
     __shared__ double2 lds[2][NT / 64];
     __shared__ float joined[NT * 8];
@@ -367,7 +371,7 @@ template <int V, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT
     }
 }
 
-// dw, db = column sums of part[rows][2][C] in 64 bits: 16 columns per workgroup, blockDim / 16 rows at a time.  lds: [blockDim / 16][17]
+// dw, db = column sums of part[rows][2][C] in 64 bits (a fixed order instead of atomics; 3.4 us for 512 rows of 2 x 512, mostly launch, 4.3 for 2 x 2048): 16 columns per workgroup, blockDim / 16 rows at a time.  lds: [blockDim / 16][17]
 __device__ __forceinline__ void param_columns(const NormArgs &A, const float *part, int rows, int block, void *dw, void *db, double *lds) {
     const int64_t width = 2 * (int64_t)A.C, column = (int64_t)block * 16 + (threadIdx.x & 15);
     const int r0 = threadIdx.x >> 4, step = blockDim.x >> 4;
@@ -554,7 +558,8 @@ template <int V, bool DROP> __device__ __forceinline__ void span_sums(const Norm
     }
     if (V == 1 && off < t.lim) add(load_chunk<DT>(x + off, t.lim - off), t.lim - off);
 }
-// part[n][g][split][column block] = sums of (x - s), (x - s)^2.  Grid: splits, column blocks, slabs.
+// part[n][g][split][column block] = sums of (x - s), (x - s)^2.  Grid: splits, column blocks, slabs.  2 x 262144 x 128 bf16 26 us = 5.2 TB/s (memory; a kernel that only reads gets to 6.3);
+// 8 x 4096 x 320 7.7 us, latency: 5.4 for the reading by 2.5 waves a SIMD, the rest the join.  (Two or three chunks on their way instead of one: no faster.)
 template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_sums(NormArgs A, MapPlan P, double2 *part) {
     extern __shared__ double2 lds[];
     const Column c = my_column(P, blockIdx.y);
@@ -569,6 +574,7 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_sums(No
         join_groups<V>(s, q, A, P, c, lds, part + n * A.G * parts + blockIdx.x * P.col_blocks + blockIdx.y, parts);
     }
 }
+// one wave per (n, g), where a slab has too many partial pairs for every workgroup of the result to join them: ~4.3 us, a launch and two dependent loads
 template <bool DROP> __global__ __launch_bounds__(256) void k_map_stats(NormArgs A, int splits, const double2 *part) {
     Draw d = {};
     if (DROP) d = make_draw(A.rng, A.site, A.cut);
@@ -650,6 +656,7 @@ template <int V, bool DROP, bool STREAM, class F> __device__ __forceinline__ voi
     }
     if (V == 1 && off < t.lim) { result(load_chunk<DT>(x + off, t.lim - off), f); store_chunk<DT>(y + off, t.lim - off, f); }
 }
+// The result: x once more, out of the caches where it fits.  2 x 262144 x 128 bf16 42 us = 6.4 TB/s read and written (memory); 8 x 4096 x 320 10.6 us, of it ~1.6 the join: latency.
 // part: the sums' partial pairs, joined by every workgroup for itself (the first of a slab writes the statistics down), or null: the statistics are there already
 template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(512) void k_map_apply(NormArgs A, MapPlan P, const double2 *part) {
     extern __shared__ double2 lds[];
@@ -731,7 +738,7 @@ __device__ __forceinline__ void channel_sums(const double (&s1)[8], const double
         }
     }
 }
-// first launch: per workgroup the channel sums (params[workgroup][2][C]), per split their w-weighted group sums (part[n][g][split][column block] = sum w dz, sum w dz xh), in 64
+// Backward, first launch: 4 x 1089 x 195 f16 11.9 us, of it two joins in LDS; per workgroup the channel sums (params[workgroup][2][C]), per split their w-weighted group sums (part[n][g][split][column block] = sum w dz, sum w dz xh), in 64
 // bits.
 template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_sums(NormArgs A, MapPlan P, double2 *part, float *params) {
     extern __shared__ double2 lds[];
@@ -809,7 +816,8 @@ __device__ __forceinline__ void span_back_apply(const NormArgs &A, const MapPlan
         store_chunk<DT>(dx + off, t.lim - off, f);
     }
 }
-// part: the sums' partial pairs, joined by every workgroup for itself, and null: the means are there already.  The first P.param_z slices of the grid join the parameter gradients.
+// The gradient of x; 4 x 1089 x 195 f16 8.5 us with the joins, both passes of 8 x 4096 x 320 bf16 65 us.
+// part: the sums' partial pairs, joined by every workgroup for itself, or null: the means are there already.  The first P.param_z slices of the grid join the parameter gradients.
 template <int V, bool DROP, bool STREAM>
 __global__ __launch_bounds__(512) void k_map_back_apply(NormArgs A, MapPlan P, const double2 *part, const double2 *means, const float *params, int param_rows, void *dw, void *db) {
     extern __shared__ double2 lds[];
@@ -833,7 +841,8 @@ __global__ __launch_bounds__(512) void k_map_back_apply(NormArgs A, MapPlan P, c
         });
 }
 
-// ---- slabs that one workgroup goes over by itself: the same passes in one launch, the second reading out of the nearer caches.  `lds`: the join's space, then G pairs.
+// ---- slabs that one workgroup goes over by itself: the same passes in one launch, the second reading out of the nearer caches.
+//      256 x 512 x 320 bf16: forward 43 us, both passes 120 (split 44 and 167); 8 x 32 x 320 forward 6.3 (8.2).  `lds`: the join's space, then G pairs.
 template <int V, bool DROP> __global__ __launch_bounds__(512) void k_slab_forward(NormArgs A, MapPlan P) {
     extern __shared__ double2 lds[];
     double2 *groups = lds + blockDim.x * (V == 2 ? 1 : 8);

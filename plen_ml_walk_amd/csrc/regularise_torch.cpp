@@ -4,8 +4,8 @@
 // 120-160 us of host time (the engine's thread has to get hold of the interpreter for each node), with these about a third of that.  Nodes with plain
 // members rather than torch::autograd::Function, whose context (a map of values by name, wrapped inputs and outputs) costs several us a pass.
 // regularise.py's functions first hand their arguments over as they come (quick_*): what passes all of its checks here is launched at once, anything else comes back as None and
-// goes through the checks in Python, which say what is wrong with it.  (A call at 100 x 512, us of host time: dropout 4.7, norm 5.8 with the checks in Python; a library
-// multiplication is at 4.6.)  What concerns memory is checked once more behind the C ABI.
+// goes through the checks in Python, which say what is wrong with it.  (A call at 100 x 512, us of host time: dropout 3.5, norm 4.0; 4.7 and 5.8 with the checks in Python; a
+// library multiplication is at 4.5.)  What concerns memory is checked once more behind the C ABI.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
