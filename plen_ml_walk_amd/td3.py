@@ -32,7 +32,7 @@ def default_device():
 
 
 class _CapturedLinear(torch.autograd.Function):
-    """F.linear whose weight and bias gradients are one launch of csrc/td3_kernels.hip's weight-gradient kernel."""
+    """F.linear with the bias gradient as a product with ones instead of a sum."""
 
     @staticmethod
     def forward(ctx, x, weight, bias):
@@ -42,14 +42,11 @@ class _CapturedLinear(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        from . import td3_fused as TF
         x, weight = ctx.saved_tensors
-        dy, x = (t if t.stride(1) == 1 else t.contiguous() for t in (dy, x))
-        (n, k), rows = weight.shape, dy.shape[0]
-        g = torch.zeros(n * k + n, dtype=torch.float32, device=dy.device)
-        TF._chk(TF.load().plentd3_wgrad(TF._p(dy), dy.stride(0), TF._p(x), x.stride(0), TF._p(g), k, TF.C.c_void_p(g.data_ptr() + 4 * n * k), rows, n, k, 0,
-                                        TF.C.c_void_p(torch.cuda.current_stream(dy.device).cuda_stream)))
-        return dy @ weight if ctx.needs_input_grad[0] else None, g[:n * k].view(n, k), g[n * k:]
+        return (dy.mm(weight) if ctx.needs_input_grad[0] else None, dy.t().mm(x), dy.new_ones(1, dy.shape[0]).mm(dy).view(-1))
+
+
+ONE_BLOCK = 256          # rows that the library adds up within one block
 
 
 def _capturing(x):
@@ -57,9 +54,9 @@ def _capturing(x):
 
 
 def _linear(x, weight, bias):
-    """F.linear.  While a stream is being captured its gradients come from the framework's own kernel: the library's bias gradient, a sum over many blocks, clears
-    its counters with a memset, and such nodes leave wrong values from a graph's second replay on (at batch 4096 biases off by as much as they are large)."""
-    if torch.is_grad_enabled() and weight.requires_grad and x.dim() == 2 and x.dtype == weight.dtype == torch.float32 and _capturing(x):
+    """F.linear.  The library's bias gradient over many rows is a sum over several blocks that clears its counters with a memset, and such nodes leave wrong values from
+    a captured graph's second replay on (at 4096 rows the biases' gradients were off by as much as they are large): while a stream is being captured it is a product."""
+    if x.dim() == 2 and x.shape[0] > ONE_BLOCK and torch.is_grad_enabled() and weight.requires_grad and _capturing(x):
         return _CapturedLinear.apply(x, weight, bias)
     return F.linear(x, weight, bias)
 

@@ -29,7 +29,7 @@ def _batch(n, seed=9):
 
 
 @pytest.mark.parametrize("dropout,norm", KINDS + [(0.0, False)])
-@pytest.mark.parametrize("B", [100, 4096, 9000])
+@pytest.mark.parametrize("B", [100, 257, 4096, 9000])
 def test_captured_backward_equals_eager_at_every_replay(dropout, norm, B):
     """The critic's forward and backward captured once: each replay draws the masks of the calls counter as it stands and leaves the eager gradients (the same
     kernels on the same values; the library's products may sum in another order: 258 and B terms, 3 products deep, 2^-24 each, as in reg_critic)."""
