@@ -4,7 +4,7 @@
  * and the two in one pass, each with its gradient.  Bound with ctypes by plen_ml_walk_amd/regularise.py.
  *
  * Conventions: every pointer is a caller-owned DEVICE pointer; work is enqueued on the hipStream_t passed as `stream` and is capturable in a
- * hipGraph; nothing is allocated and no state is kept between calls.  Return 0, or a negative HIP error code (-1 = hipErrorInvalidValue:
+ * hipGraph; nothing is allocated and no state is kept between calls.  Outputs overlap neither inputs nor each other.  Return 0, or a negative HIP error code (-1 = hipErrorInvalidValue:
  * an argument is outside what this header allows; nothing was launched then).
  */
 #ifndef PLENREG_H

@@ -139,18 +139,22 @@ static MapLaunch map_plan(const PlenRegNorm &a, bool backward) {
     const int64_t threads = div_up(chunks, 64) * 64;
     m.NT = m.slab ? fill_threads(m.P.bcol, threads < 448 ? (int)threads : 448, 448) : fill_threads(m.P.bcol, 256, 512);
     m.P.R = m.NT / m.P.bcol;
-    // 2 workgroups per compute unit, or 4 where their threads then still have 16 chunks each; each thread in whole turns of 2 rows.  (Before the joins' present form, 8 x 4096 x 320: 512 workgroups 9.2 + 9.5 us,
-    // 1024: 10.8 + 9.8; 2 x 262144 x 128: 47 + 42 and 40 + 43)
-    const int64_t blocks = a.N * chunks >= (int64_t)1 << 22 ? 1024 : 512;
-    const int64_t turn = (int64_t)m.P.R * 2, turns = div_up(m.P.rows, turn), groups = a.N * m.P.col_blocks;
+    // 2 workgroups per compute unit, or 4 where their threads then still have 16 chunks each; each thread in whole turns of 2 rows.  One, where their joins weigh more than their number
+    // helps: a slab with more than 2048 partial pairs, and the backward pass of groups that share chunks.  (us; 512 / 256 / 1024 workgroups: 8 x 4096 x 320 forward 17.0 / 18.3 / 19.5,
+    // backward 42.4 / 35.6 / 56.9; 1 x 4096 x 512 in 8 groups 9.0 / 8.1 / 9.0 and 16.6 / 14.2 / 16.2; 2 x 16384 x 128 in 8 groups 9.8 / 10.1 / 12.0 and 16.6 / 18.5 / 20.9; 2 x 262144 x 128
+    // sums 47 with 512, 40 with 1024)
+    const bool whole = a.C % 8 == 0 && D % 8 == 0;
+    const int64_t groups = a.N * m.P.col_blocks;
+    int64_t blocks = a.N * chunks >= (int64_t)1 << 22 ? 1024 : 512;
+    if (blocks == 512 && ((backward && !whole) || div_up(512, groups) * a.G * m.P.col_blocks > 2048)) blocks = 256;
+    const int64_t turn = (int64_t)m.P.R * 2, turns = div_up(m.P.rows, turn);
     const int64_t most = MAP_MAX_SPAN / (turn * ((int64_t)a.C << m.P.q_log));              // turns of a workgroup, so that its offsets fit
-    const int64_t sum_turns = div_up(turns, groups >= blocks ? 1 : div_up(blocks, groups)), apply_turns = div_up(turns, groups >= blocks ? 1 : div_up(blocks, groups));
-    m.P.rows_per = (sum_turns < most ? sum_turns : most) * turn;
+    const int64_t per = div_up(turns, groups >= blocks ? 1 : div_up(blocks, groups));
+    m.P.rows_per = m.P.apply_rows = (per < most ? per : most) * turn;
     m.P.splits = (int)div_up(m.P.rows, m.P.rows_per);
-    m.P.apply_rows = (apply_turns < most ? apply_turns : most) * turn;
     const int64_t row_blocks = div_up(m.P.rows, m.P.apply_rows);
     // lanes that join a group (a channel) of a workgroup's entries: all of them at a time where there are as many
-    const int units = a.C % 8 == 0 && D % 8 == 0 ? D / 8 : D >= 8 ? (D + 14) / 8 : D, local = (int)(m.P.q_log || m.P.bcol * 8 > a.C ? a.C : m.P.bcol * 8);
+    const int units = whole ? D / 8 : D >= 8 ? (D + 14) / 8 : D, local = (int)(m.P.q_log || m.P.bcol * 8 > a.C ? a.C : m.P.bcol * 8);
     m.P.lanes_log = lanes_for(m.NT / a.G, (units * m.P.R) << m.P.q_log);
     m.P.chan_log = lanes_for(m.NT / local, m.P.R << m.P.q_log);
     // slabs beyond what fills the chip (and the grid's limit of 65535) are walked by the workgroups

@@ -816,7 +816,7 @@ __device__ __forceinline__ void span_back_apply(const NormArgs &A, const MapPlan
         store_chunk<DT>(dx + off, t.lim - off, f);
     }
 }
-// The gradient of x; 4 x 1089 x 195 f16 8.5 us with the joins, both passes of 8 x 4096 x 320 bf16 65 us.
+// The gradient of x; 4 x 1089 x 195 f16 8.5 us with the joins, both passes of 8 x 4096 x 320 bf16 53 us.
 // part: the sums' partial pairs, joined by every workgroup for itself, or null: the means are there already.  The first P.param_z slices of the grid join the parameter gradients.
 template <int V, bool DROP, bool STREAM>
 __global__ __launch_bounds__(512) void k_map_back_apply(NormArgs A, MapPlan P, const double2 *part, const double2 *means, const float *params, int param_rows, void *dw, void *db) {

@@ -8,7 +8,8 @@ The twin critics' hidden rows lie side by side in one [B, 512] matrix, so group 
 Random state: an int64[2] device tensor {seed, calls so far}, the form every draw of this package uses (`new_rng`).  Which mask a call draws depends
 on that state, on `site` (one number per place in the model) and on the element's index alone, not on type, strides or launch shape.  A call only READS the
 state; `advance` moves it on, once per iteration, as a kernel (so a captured graph draws new masks at every replay).  The backward pass draws the
-forward's mask again from a 16-byte snapshot that the forward kernel takes.
+forward's mask again from a 16-byte snapshot that the forward kernel takes.  (Who runs a forward pass a second time, as activation checkpointing does, has to do so before
+`advance`: it draws from the state as it then stands.)
 
 CPU tensors take the same definitions as elementary torch operations (autograd differentiates them): the multi-process CPU path of td3.py."""
 import ctypes as C
