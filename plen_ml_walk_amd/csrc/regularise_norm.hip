@@ -221,7 +221,9 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
     const RowPlace p = row_place<NT>(A, P);
     int c[K], valid[K];
     row_chunks<K>(A, P, p, c, valid);
-    int64_t n = (int64_t)blockIdx.x * P.rb + p.row;
+    // where a lane's row begins in x, in y and the mask (at), among the statistics: walked along by additions (a 64-bit product is a dozen slots); past the last row they stay
+    const int64_t rows = (int64_t)gridDim.x * P.rb, x_step = rows * A.x_stride, step = rows * A.C, st_step = rows * A.G;
+    int64_t n = (int64_t)blockIdx.x * P.rb + p.row, at = (n < A.N ? n : A.N - 1) * A.C, st_at = (n < A.N ? n : A.N - 1) * A.G + p.g;
     const T *px = (const T *)A.x + (n < A.N ? n : A.N - 1) * A.x_stride;
     Chunk<DT> x[K];
 #pragma unroll
@@ -234,18 +236,19 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
 #pragma unroll 1
     for (int turn = 0; turn < P.trips; turn++) {
         const bool on = p.mine && n < A.N;
-        const int64_t next = n + (int64_t)gridDim.x * P.rb;
+        const int64_t next = n + rows;
+        const T *row = px;
         float v[K][8];
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const Mask<DROP ? V + 1 : 0> m(d, n * A.C + c[k]);
+            const Mask<DROP ? V + 1 : 0> m(d, at + c[k]);
             unpack(x[k], v[k]);
             move_down<V>(v[k], c[k], A.C);
 #pragma unroll
             for (int e = 0; e < 8; e++) v[k][e] = m.keep(e, v[k][e]);
         }
         if (turn + 1 < P.trips) {                               // the next row's, while this one is worked on
-            px = (const T *)A.x + (next < A.N ? next : A.N - 1) * A.x_stride;
+            if (next < A.N) px += x_step;
 #pragma unroll
             for (int k = 0; k < K; k++) x[k] = load_inside<V, DT, STREAM>(px, c[k], A.C);
         }
@@ -253,9 +256,8 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
         float first;
         if (P.team_log <= 6) first = __shfl(v[0][0], (threadIdx.x & 63) >> P.team_log << P.team_log);
         else {
-            const int64_t row = n < A.N ? n : A.N - 1;
-            first = (float)((const T *)A.x)[row * A.x_stride + c[0] - 8 * p.lane];
-            if (DROP && !kept(d, row * A.C + c[0] - 8 * p.lane)) first = 0.f;
+            first = (float)row[c[0] - 8 * p.lane];
+            if (DROP && !kept(d, at + c[0] - 8 * p.lane)) first = 0.f;
         }
         const double shift = (double)first;
         double s = 0.0, q = 0.0;
@@ -273,7 +275,7 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
         team_sum2<NT>(s, q, P.team_log, turn, lds);
         const double2 st = finish_stats(A, shift, s, q);
         if (on) {
-            if (A.stats && p.lane == 0) A.stats[n * A.G + p.g] = st;
+            if (A.stats && p.lane == 0) A.stats[st_at] = st;
             const float mean = (float)st.x, rest = (float)(st.x - (double)mean), rstd = (float)st.y;
 #pragma unroll
             for (int k = 0; k < K; k++) {
@@ -281,10 +283,11 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
 #pragma unroll
                 for (int e = 0; e < 8; e++) v[k][e] = from_mean(v[k][e], mean, rest) * rstd * w[k][e] + b[k][e];
                 activate(v[k], A.act);
-                row_store<V, STREAM>((T *)A.out + n * A.C + c[k], valid[k], v[k]);
+                row_store<V, STREAM>((T *)A.out + at + c[k], valid[k], v[k]);
             }
         }
         n = next;
+        if (n < A.N) { at += step; st_at += st_step; }
     }
 }
 
@@ -298,10 +301,13 @@ template <int V, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT
     int c[1], valid[1];
     row_chunks<1>(A, P, p, c, valid);
     const int c0 = c[0], g0 = p.g < A.G ? p.g : A.G - 1;
-    int64_t n = (int64_t)blockIdx.x * P.rb + p.row, row = n < A.N ? n : A.N - 1;
-    const T *px = (const T *)A.x + row * A.x_stride;
-    Chunk<DT> x = load_inside<V, DT, STREAM>(px, c0, A.C), g = load_inside<V, DT, STREAM>((const T *)A.dy + row * A.dy_stride, c0, A.C);
-    double2 st = A.stats[row * A.G + g0];
+    // (as in the forward pass, additions instead of products)
+    const int64_t rows = (int64_t)gridDim.x * P.rb, x_step = rows * A.x_stride, dy_step = rows * A.dy_stride, step = rows * A.C, st_step = rows * A.G;
+    int64_t n = (int64_t)blockIdx.x * P.rb + p.row, at = (n < A.N ? n : A.N - 1) * A.C + c0;
+    const T *px = (const T *)A.x + (n < A.N ? n : A.N - 1) * A.x_stride, *pdy = (const T *)A.dy + (n < A.N ? n : A.N - 1) * A.dy_stride;
+    const double2 *pst = A.stats + (n < A.N ? n : A.N - 1) * A.G + g0;
+    Chunk<DT> x = load_inside<V, DT, STREAM>(px, c0, A.C), g = load_inside<V, DT, STREAM>(pdy, c0, A.C);
+    double2 st = *pst;
     float w[8], b[8], dw[8] = {}, db[8] = {};
     row_params<V>(A, A.w, c0, 1.f, w);
     row_params<V>(A, A.b, c0, 0.f, b);
@@ -311,7 +317,7 @@ template <int V, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT
     for (int turn = 0; turn < P.trips; turn++) {
         const bool on = n < A.N && valid[0];
         float xh[8] = {}, gw[8] = {}, s = 0.f, q = 0.f, rstd = 0.f;
-        const Mask<DROP ? V + 1 : 0> m(d, n * A.C + c0);
+        const Mask<DROP ? V + 1 : 0> m(d, at);
         if (on) {
             const float mean = (float)st.x, rest = (float)(st.x - (double)mean);
             rstd = (float)st.y;
@@ -334,13 +340,12 @@ template <int V, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT
                 db[e] += dz[e]; dw[e] = fmaf(dz[e], xh[e], dw[e]);
             }
         }
-        const int64_t here = n;
-        n += (int64_t)gridDim.x * P.rb;
+        const int64_t here = at;
+        n += rows;
+        if (n < A.N) { px += x_step; pdy += dy_step; pst += st_step; at += step; }
         if (turn + 1 < P.trips) {                               // the next row's, while this one's sums are joined
-            row = n < A.N ? n : A.N - 1;
-            px = (const T *)A.x + row * A.x_stride;
-            x = load_inside<V, DT, STREAM>(px, c0, A.C); g = load_inside<V, DT, STREAM>((const T *)A.dy + row * A.dy_stride, c0, A.C);
-            st = A.stats[row * A.G + g0];
+            x = load_inside<V, DT, STREAM>(px, c0, A.C); g = load_inside<V, DT, STREAM>(pdy, c0, A.C);
+            st = *pst;
         }
         team_sum2<NT>(s, q, P.team_log, turn, lds);
         if (on) {
@@ -349,7 +354,7 @@ template <int V, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT
             for (int e = 0; e < 8; e++) {
                 gw[e] = m.keep(e, rstd * (gw[e] - m1 - xh[e] * m2));
             }
-            row_store<V, STREAM>((T *)A.out + here * A.C + c0, valid[0], gw);
+            row_store<V, STREAM>((T *)A.out + here, valid[0], gw);
         }
     }
     if (!part) return;
