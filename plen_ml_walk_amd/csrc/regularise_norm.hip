@@ -423,6 +423,7 @@ __device__ __forceinline__ Column my_column(const MapPlan &P, int col_block) {
     c.r = small_quotient(threadIdx.x, P.inv_bcol);
     c.col = c.first + (int)threadIdx.x - c.r * P.bcol;
     c.mine = c.r < P.R && c.col < P.ncol;
+    if (c.col >= P.ncol) c.col = P.ncol - 1;             // (of the last, narrower block: its idle threads look at the parameters of the last column, not behind them)
     return c;
 }
 // a workgroup's rows of slab n: `base` elements into it, `lim` elements; a thread takes the chunks at off, off + step, ... that are whole, and if it then stands at off < lim,

@@ -454,7 +454,7 @@ def test_forward_mode_is_refused():
 
 @pytest.mark.parametrize("shape,groups", [((40, 2, 8192), 4), ((3, 2, 8192), 1), ((2, 3, 4104), 27), ((700, 40, 448), 448), ((4, 1089, 195), 13), ((2, 4096, 64), 64), ((1, 4096, 512), 8),
                                           ((1, 4096, 512), 16), ((2, 700, 200), 200), ((5, 1100, 90), 45),
-                                          ((600, 2, 4096), 4096), ((300, 2, 2504), 2504), ((260, 30, 512), 512), ((300, 1000, 40), 8)], ids=ids)
+                                          ((600, 2, 4096), 4096), ((300, 2, 2504), 2504), ((3, 70, 4104), 513), ((2, 9, 8184), 3), ((2, 300, 5000), 25), ((260, 30, 512), 512), ((300, 1000, 40), 8)], ids=ids)
 def test_statistics_joined_in_the_results_launch_or_in_one_of_their_own(shape, groups):
     """Few partial sums per slab and many; few workgroups per slab beside many channels; groups of one channel."""
     x, dy, w, b = _case(shape, groups, torch.bfloat16)
