@@ -181,6 +181,10 @@ static __device__ __forceinline__ int small_quotient(int i, float inv_n) { retur
 // rows of one position: 2^team_log lanes per (row, group); a workgroup covers gb neighbouring groups of rb rows per turn
 struct RowPlan { int team_log, gb, rb, trips; float inv_gb; };
 struct RowLaunch { RowPlan P; int K, NT; dim3 grid; bool stream; };
+// rows too wide for that: grid of (n, group) pairs, and of the parameter gradients
+#define WIDE_LOG 9
+#define WIDE_NT (1 << WIDE_LOG)
+struct WideLaunch { unsigned grid; dim3 params; bool stream; };
 // many positions.  A slab as `rows` rows of `ncol` chunk columns (2^q_log positions to a row); bcol columns in a workgroup, R rows per turn of it; rows_per rows in a
 // workgroup of the sums, apply_rows in one of the result; 2^lanes_log lanes join one group
 struct MapPlan { int q_log, ncol, bcol, col_blocks, R, splits, lanes_log, chan_log, join_log, param_z; int64_t rows, rows_per, apply_rows; float inv_bcol; };
@@ -191,6 +195,8 @@ struct MapLaunch { MapPlan P; dim3 sums, apply; int NT, param_rows; unsigned sta
 struct NormEntry {
     void (*row_forward)(const NormArgs &, const RowLaunch &, hipStream_t);
     void (*row_backward)(const NormArgs &, const RowLaunch &, float *part, hipStream_t);
+    void (*wide_forward)(const NormArgs &, const WideLaunch &, hipStream_t);
+    void (*wide_backward)(const NormArgs &, const WideLaunch &, float *part, hipStream_t);
     void (*map_forward)(const NormArgs &, const MapLaunch &, double2 *part, hipStream_t);
     void (*map_backward)(const NormArgs &, const MapLaunch &, double2 *part, double2 *means, float *params, void *dw, void *db, hipStream_t);
     void (*params)(const NormArgs &, const float *part, int rows, void *dw, void *db, hipStream_t);

@@ -102,6 +102,19 @@ static RowLaunch row_plan(const PlenRegNorm &a, bool backward) {
     r.stream = streams(a);
     return r;
 }
+static WideLaunch wide_plan(const PlenRegNorm &a) {
+    WideLaunch m;
+    m.grid = (unsigned)(a.N * a.G < 2048 ? a.N * a.G : 2048);
+    // parameter gradients: about 1024 workgroups, of at least 8 rows (each leaves 2 C partial sums) and at most 256 (their sums are in 32 bits)
+    const int64_t x = div_up((int64_t)a.G * div_up(a.C / a.G, 8), 256);
+    int64_t y = div_up(1024, x);
+    if (y > div_up(a.N, 8)) y = div_up(a.N, 8);
+    if (y < div_up(a.N, 256)) y = div_up(a.N, 256);
+    if (y > a.N) y = a.N;
+    m.params = dim3((unsigned)x, (unsigned)(y < 65535 ? y : 65535));
+    m.stream = streams(a);
+    return m;
+}
 // threads (a multiple of 64) of which the fewest idle when `ncol` of them make a row
 static int fill_threads(int ncol, int lo, int hi) {
     int best = lo;
@@ -221,6 +234,7 @@ int plenreg_dropout(const PlenRegDropout *a, void *stream) {
 int64_t plenreg_norm_workspace(const PlenRegNorm *a, int backward) {
     if (bad_norm(a)) return PLENREG_REFUSE;
     if (by_rows(*a, backward)) return backward ? (int64_t)row_plan(*a, true).grid.x * 2 * a->C * 4 : 0;
+    if (a->L == 1) return backward ? (int64_t)wide_plan(*a).params.y * 2 * a->C * 4 : 0;
     const MapLaunch m = map_plan(*a, backward);
     if (m.slab) return backward ? (int64_t)m.param_rows * 2 * a->C * 4 : 0;
     return part_bytes(*a, m) + a->N * a->G * 16 + (backward ? (int64_t)m.param_rows * 2 * a->C * 4 : 0);
@@ -233,6 +247,10 @@ int plenreg_norm_forward(const PlenRegNorm *a, void *stream) {
         entry(*a).row_forward(k, row_plan(*a, false), (hipStream_t)stream);
         return launched();
     }
+    if (a->L == 1) {
+        entry(*a).wide_forward(k, wide_plan(*a), (hipStream_t)stream);
+        return launched();
+    }
     const MapLaunch m = map_plan(*a, false);
     if (!a->ws && !m.slab) return PLENREG_REFUSE;
     if (!k.stats && !m.slab) k.stats = (double2 *)((char *)a->ws + part_bytes(*a, m));
@@ -243,13 +261,19 @@ int plenreg_norm_forward(const PlenRegNorm *a, void *stream) {
 int plenreg_norm_backward(const PlenRegNorm *a, void *stream) {
     if (bad_norm(a) || !a->x || !a->dy || !a->out || !a->stats || a->x_stride < 0 || a->dy_stride < 0 || (a->cut && !a->rng)) return PLENREG_REFUSE;
     const bool params = a->dw || a->db, rows = by_rows(*a, true);
-    if (plenreg_norm_workspace(a, 1) > 0 && (params || !rows) && !a->ws) return PLENREG_REFUSE;
+    if (plenreg_norm_workspace(a, 1) > 0 && (params || a->L > 1) && !a->ws) return PLENREG_REFUSE;
     const NormArgs k = kernel_args(*a);
     const NormEntry &e = entry(*a);
     if (rows) {
         const RowLaunch r = row_plan(*a, true);
         e.row_backward(k, r, params ? (float *)a->ws : nullptr, (hipStream_t)stream);
         if (params) e.params(k, (const float *)a->ws, (int)r.grid.x, a->dw, a->db, (hipStream_t)stream);
+        return launched();
+    }
+    if (a->L == 1) {
+        const WideLaunch m = wide_plan(*a);
+        e.wide_backward(k, m, params ? (float *)a->ws : nullptr, (hipStream_t)stream);
+        if (params) e.params(k, (const float *)a->ws, (int)m.params.y, a->dw, a->db, (hipStream_t)stream);
         return launched();
     }
     const MapLaunch m = map_plan(*a, true);

@@ -412,7 +412,160 @@ __global__ __launch_bounds__(1024) void k_row_params(NormArgs A, const float *pa
     param_columns(A, part, rows, blockIdx.x, dw, db, lds);
 }
 
-// ---- many positions (or rows too wide for a workgroup's lanes): a slab is size = L C contiguous elements, seen as rows of q C (q = the smallest number of positions that
+// ---- rows too wide for a workgroup's registers: one workgroup goes over a group twice, the second time out of the caches; the parameters are read with each chunk.  Its parameter gradients
+//      are a launch of their own, in which a thread owns a chunk column and walks down the rows.  8192 x 8192 bf16: backward 175 us (memory: x and dy come from there twice, once for either
+//      launch; 551 as slabs of one position); 4096 x 16384: forward 62 (198 as slabs), backward 177 (628).
+template <int V> __device__ __forceinline__ int wide_valid(const NormArgs &A, int off) { return V || A.D - off > 8 ? 8 : A.D - off; }
+// forward; grid: (n, g) pairs
+template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(WIDE_NT) void k_wide_forward(NormArgs A) {
+    __shared__ double2 lds[2][WIDE_NT / 64];
+    Draw d = {};
+    if (DROP) { d = make_draw(A.rng, A.site, A.cut); write_used(A); }
+    int turn = 0;
+#pragma unroll 1
+    for (int64_t item = blockIdx.x; item < A.N * A.G; item += gridDim.x, turn++) {
+        const int64_t n = item / A.G;
+        const int c0 = (int)(item - n * A.G) * A.D;
+        const T *px = (const T *)A.x + n * A.x_stride;
+        float first = (float)px[c0];
+        if (DROP && !kept(d, n * A.C + c0)) first = 0.f;
+        const double shift = (double)first;
+        double s = 0.0, q = 0.0;
+        int off = 8 * threadIdx.x;
+        Chunk<DT> x = load_inside<V, DT>(px, c0 + (off < A.D ? off : 0), A.C);
+#pragma unroll 1
+        for (; off < A.D; off += 8 * WIDE_NT) {
+            float v[8];
+            unpack(x, v);
+            move_down<V>(v, c0 + off, A.C);
+            const int next = off + 8 * WIDE_NT, valid = wide_valid<V>(A, off);
+            x = load_inside<V, DT>(px, c0 + (next < A.D ? next : off), A.C);
+            const Mask<DROP ? V + 1 : 0> m(d, n * A.C + c0 + off);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const double t = !V && e >= valid ? 0.0 : (double)m.keep(e, v[e]) - shift;
+                s += t; q = fma(t, t, q);
+            }
+        }
+        team_sum2<WIDE_NT>(s, q, WIDE_LOG, turn, lds);
+        const double2 st = finish_stats(A, shift, s, q);
+        if (A.stats && threadIdx.x == 0) A.stats[item] = st;
+        const float mean = (float)st.x, rest = (float)(st.x - (double)mean), rstd = (float)st.y;
+        T *y = (T *)A.out + n * A.C + c0;
+        off = 8 * threadIdx.x;
+        x = load_inside<V, DT, STREAM>(px, c0 + (off < A.D ? off : 0), A.C);
+#pragma unroll 1
+        for (; off < A.D; off += 8 * WIDE_NT) {
+            float v[8], w[8], b[8];
+            unpack(x, v);
+            move_down<V>(v, c0 + off, A.C);
+            const int next = off + 8 * WIDE_NT;
+            x = load_inside<V, DT, STREAM>(px, c0 + (next < A.D ? next : off), A.C);
+            row_params<V>(A, A.w, c0 + off, 1.f, w);
+            row_params<V>(A, A.b, c0 + off, 0.f, b);
+            const Mask<DROP ? V + 1 : 0> m(d, n * A.C + c0 + off);
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = from_mean(m.keep(e, v[e]), mean, rest) * rstd * w[e] + b[e];
+            activate(v, A.act);
+            row_store<V, STREAM>(y + off, wide_valid<V>(A, off), v);
+        }
+    }
+}
+// dz, xh and w of a chunk (zeros in dz behind the group's end)
+template <int V, bool DROP>
+__device__ __forceinline__ void wide_back(const NormArgs &A, const Mask<DROP ? V + 1 : 0> &m, const Chunk<DT> &x, const Chunk<DT> &g, const T *px, int64_t n, int c, int valid, double2 st, float (&w)[8], float (&xh)[8],
+                                          float (&dz)[8]) {
+    float b[8], dy[8];
+    row_params<V>(A, A.w, c, 1.f, w);
+    row_params<V>(A, A.b, c, 0.f, b);
+    unpack(x, xh);
+    unpack(g, dy);
+    move_down<V>(xh, c, A.C);
+    move_down<V>(dy, c, A.C);
+    const float mean = (float)st.x, rest = (float)(st.x - (double)mean), rstd = (float)st.y;
+#pragma unroll
+    for (int e = 0; e < 8; e++) xh[e] = ((m.keep(e, xh[e]) - mean) - rest) * rstd;
+    back_activation(A, px + c, n, c, valid, m, xh, dy, w, b, dz);
+    if (!V) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) dz[e] = e < valid ? dz[e] : 0.f;
+    }
+}
+// the gradient of x; grid: (n, g) pairs.  (Sums in 32 bits: a lane adds at most 64 elements before the lanes are joined.)
+template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(WIDE_NT) void k_wide_backward(NormArgs A) {
+    __shared__ double2 lds[2][WIDE_NT / 64];
+    Draw d = {};
+    if (DROP) d = make_draw(A.rng, A.site, A.cut);
+    int turn = 0;
+#pragma unroll 1
+    for (int64_t item = blockIdx.x; item < A.N * A.G; item += gridDim.x, turn++) {
+        const int64_t n = item / A.G;
+        const int c0 = (int)(item - n * A.G) * A.D;
+        const T *px = (const T *)A.x + n * A.x_stride, *pdy = (const T *)A.dy + n * A.dy_stride;
+        const double2 st = A.stats[item];
+        float s = 0.f, q = 0.f, xh[8], dz[8], w[8];
+        int off = 8 * threadIdx.x;
+        Chunk<DT> x = load_inside<V, DT>(px, c0 + (off < A.D ? off : 0), A.C), g = load_inside<V, DT>(pdy, c0 + (off < A.D ? off : 0), A.C);
+#pragma unroll 1
+        for (; off < A.D; off += 8 * WIDE_NT) {
+            const Chunk<DT> xn = x, gn = g;
+            const int next = off + 8 * WIDE_NT, at = c0 + (next < A.D ? next : off);
+            x = load_inside<V, DT>(px, at, A.C); g = load_inside<V, DT>(pdy, at, A.C);
+            const Mask<DROP ? V + 1 : 0> m(d, n * A.C + c0 + off);
+            wide_back<V, DROP>(A, m, xn, gn, px, n, c0 + off, wide_valid<V>(A, off), st, w, xh, dz);
+#pragma unroll
+            for (int e = 0; e < 8; e++) { const float gw = dz[e] * w[e]; s += gw; q = fmaf(gw, xh[e], q); }
+        }
+        team_sum2<WIDE_NT>(s, q, WIDE_LOG, turn, lds);
+        const float m1 = s * (float)A.inv_count, m2 = q * (float)A.inv_count, rstd = (float)st.y;
+        T *dx = (T *)A.out + n * A.C + c0;
+        off = 8 * threadIdx.x;
+        x = load_inside<V, DT, STREAM>(px, c0 + (off < A.D ? off : 0), A.C); g = load_inside<V, DT, STREAM>(pdy, c0 + (off < A.D ? off : 0), A.C);
+#pragma unroll 1
+        for (; off < A.D; off += 8 * WIDE_NT) {
+            const Chunk<DT> xn = x, gn = g;
+            const int next = off + 8 * WIDE_NT, at = c0 + (next < A.D ? next : off), valid = wide_valid<V>(A, off);
+            x = load_inside<V, DT, STREAM>(px, at, A.C); g = load_inside<V, DT, STREAM>(pdy, at, A.C);
+            const Mask<DROP ? V + 1 : 0> m(d, n * A.C + c0 + off);
+            wide_back<V, DROP>(A, m, xn, gn, px, n, c0 + off, valid, st, w, xh, dz);
+#pragma unroll
+            for (int e = 0; e < 8; e++) dz[e] = m.keep(e, rstd * (dz[e] * w[e] - m1 - xh[e] * m2));
+            row_store<V, STREAM>(dx + off, valid, dz);
+        }
+    }
+}
+// part[split][0 / 1][C] = dw, db of rows split, split + splits, ...; grid: blocks of 256 chunk columns (per group: its chunks), splits
+template <int V, bool DROP> __global__ __launch_bounds__(256) void k_wide_params(NormArgs A, float *part) {
+    const int per = (A.D + 7) >> 3, j = blockIdx.x * 256 + threadIdx.x;
+    if (j >= per * A.G) return;
+    const int grp = j / per, off = 8 * (j - grp * per), c = grp * A.D + off, valid = wide_valid<V>(A, off);
+    Draw d = {};
+    if (DROP) d = make_draw(A.rng, A.site, A.cut);
+    int64_t n = blockIdx.y;
+    const T *px = (const T *)A.x + n * A.x_stride, *pdy = (const T *)A.dy + n * A.dy_stride;
+    Chunk<DT> x = load_inside<V, DT>(px, c, A.C), g = load_inside<V, DT>(pdy, c, A.C);
+    double2 st = A.stats[n * A.G + grp];
+    float dw[8] = {}, db[8] = {};
+#pragma unroll 1
+    for (; n < A.N; n += gridDim.y) {
+        const Chunk<DT> xn = x, gn = g;
+        const double2 now = st;
+        const T *here = px;
+        if (n + gridDim.y < A.N) { px += gridDim.y * A.x_stride; pdy += gridDim.y * A.dy_stride; st = A.stats[(n + gridDim.y) * A.G + grp]; }
+        x = load_inside<V, DT>(px, c, A.C); g = load_inside<V, DT>(pdy, c, A.C);
+        const Mask<DROP ? V + 1 : 0> m(d, n * A.C + c);
+        float w[8], xh[8], dz[8];
+        wide_back<V, DROP>(A, m, xn, gn, here, n, c, valid, now, w, xh, dz);
+#pragma unroll
+        for (int e = 0; e < 8; e++) { db[e] += dz[e]; dw[e] = fmaf(dz[e], xh[e], dw[e]); }
+    }
+    float *to = part + (int64_t)blockIdx.y * 2 * A.C + c;
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        if (e < valid) { to[e] = dw[e]; to[A.C + e] = db[e]; }
+}
+
+// ---- many positions: a slab is size = L C contiguous elements, seen as rows of q C (q = the smallest number of positions that
 //      fill whole chunks, so that odd channel counts load whole chunks too; the last row may be cut short, and of its last chunk there may be a part).  A thread owns one
 //      chunk column (8 fixed virtual channels v, channel v % C) and walks down the rows; workgroups split the rows and, where they are wide, the columns.  Statistics, their
 //      join, and the result are launches of their own: the second reading of x comes out of the caches while it fits.
@@ -914,6 +1067,26 @@ void row_backward(const NormArgs &a, const RowLaunch &r, float *part, hipStream_
     else a.cut ? row_backward_v<1, true, false>(a, r, part, s) : row_backward_v<1, false, false>(a, r, part, s);
 }
 unsigned column_blocks(const NormArgs &a) { return (unsigned)((2 * (int64_t)a.C + 15) / 16); }
+template <int V, bool STREAM> void wide_forward_v(const NormArgs &a, const WideLaunch &m, hipStream_t s) {
+    if (a.cut) k_wide_forward<V, true, STREAM><<<m.grid, WIDE_NT, 0, s>>>(a);
+    else k_wide_forward<V, false, STREAM><<<m.grid, WIDE_NT, 0, s>>>(a);
+}
+void wide_forward(const NormArgs &a, const WideLaunch &m, hipStream_t s) {
+    if (a.D % 8) wide_forward_v<0, false>(a, m, s);
+    else m.stream ? wide_forward_v<1, true>(a, m, s) : wide_forward_v<1, false>(a, m, s);
+}
+template <int V, bool STREAM> void wide_backward_v(const NormArgs &a, const WideLaunch &m, float *part, hipStream_t s) {
+    if (part) {
+        if (a.cut) k_wide_params<V, true><<<m.params, 256, 0, s>>>(a, part);
+        else k_wide_params<V, false><<<m.params, 256, 0, s>>>(a, part);
+    }
+    if (a.cut) k_wide_backward<V, true, STREAM><<<m.grid, WIDE_NT, 0, s>>>(a);
+    else k_wide_backward<V, false, STREAM><<<m.grid, WIDE_NT, 0, s>>>(a);
+}
+void wide_backward(const NormArgs &a, const WideLaunch &m, float *part, hipStream_t s) {
+    if (a.D % 8) wide_backward_v<0, false>(a, m, part, s);
+    else m.stream ? wide_backward_v<1, true>(a, m, part, s) : wide_backward_v<1, false>(a, m, part, s);
+}
 void params(const NormArgs &a, const float *part, int rows, void *dw, void *db, hipStream_t s) { k_row_params<<<column_blocks(a), 1024, 0, s>>>(a, part, rows, dw, db); }
 
 bool one_group(const NormArgs &a) { return a.C % 8 == 0 && a.D % 8 == 0; }
@@ -965,6 +1138,6 @@ void map_backward(const NormArgs &a, const MapLaunch &m, double2 *part, double2 
 }  // namespace
 
 const NormEntry &REG_ENTRY() {
-    static const NormEntry e = {row_forward, row_backward, map_forward, map_backward, params};
+    static const NormEntry e = {row_forward, row_backward, wide_forward, wide_backward, map_forward, map_backward, params};
     return e;
 }

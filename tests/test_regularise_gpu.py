@@ -496,3 +496,17 @@ def test_groups_that_the_mask_leaves_empty_beside_others(shape, groups):
     for act in ("none", "relu", "silu"):
         _check(x, dy, w, None, groups, act, 0.9, _rng())
         _check(x, dy, w, b, groups, act, 0.9, _rng())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("shape,groups", [((3, 4104), 1), ((2, 4097), 1), ((5, 8192), 1), ((300, 8200), 1), ((3, 16388), 2), ((7, 32768), 1), ((2, 32765), 1), ((2, 32768), 4), ((2100, 4112), 1)], ids=ids)
+def test_rows_wider_than_a_workgroup_holds(shape, groups, dtype):
+    x, dy, w, b = _case(shape, groups, dtype)
+    for act, p in (("relu", 0.1), ("silu", None)):
+        _check(x, dy, w, b, groups, act, p, _rng())
+    _check(x, dy, None, b, groups, "none", 0.5, _rng())
+    wide = torch.zeros(shape[0], shape[1] + 5, dtype=dtype, device="cuda")
+    wide[:, 3:3 + shape[1]] = x.detach()
+    part = wide[:, 3:3 + shape[1]].requires_grad_()
+    y, z = R.group_norm_act(x, groups, w, b), R.group_norm_act(part, groups, w, b)
+    assert torch.equal(y, z) and all(torch.equal(s, t) for s, t in zip(torch.autograd.grad(y, (x, w, b), dy), torch.autograd.grad(z, (part, w, b), dy)))
