@@ -133,6 +133,7 @@ template <int M> struct Mask;
 template <> struct Mask<2> {
     u4 w;
     uint32_t cut;
+    Mask() = default;
     __device__ __forceinline__ Mask(const Draw &d, int64_t i) : w(block_words(d, (uint32_t)(i >> 3))), cut(d.cut) {}
     __device__ __forceinline__ float keep(int e, float v) const {          // (e is a constant where this is inlined)
         const uint32_t word = e < 2 ? w.x : e < 4 ? w.y : e < 6 ? w.z : w.w;
@@ -147,6 +148,7 @@ template <> struct Mask<2> {
 };
 template <> struct Mask<1> {
     uint32_t m;
+    Mask() = default;
     __device__ __forceinline__ Mask(const Draw &d, int64_t i) {
         const uint32_t block = (uint32_t)(i >> 3), shift = (uint32_t)i & 7u;
         m = block_mask(d, block);
@@ -156,6 +158,7 @@ template <> struct Mask<1> {
     __device__ __forceinline__ uint32_t bits() const { return m; }
 };
 template <> struct Mask<0> {
+    Mask() = default;
     __device__ __forceinline__ Mask(const Draw &, int64_t) {}
     __device__ __forceinline__ float keep(int, float v) const { return v; }
     __device__ __forceinline__ uint32_t bits() const { return 255u; }

@@ -5,8 +5,7 @@
 #define DROPOUT_SMALL (1 << 18)
 #define STREAM_BYTES ((int64_t)64 << 20)     // tensors from here on go past the caches where nobody reads them next (2 x 262144 x 128 bf16: sums 47 -> 26 us, result 42 -> 40)
 #define MAP_MAX_SPAN ((int64_t)1 << 28)      // elements of a slab that one workgroup walks over
-#define ROW_MAX_FORWARD 8192            // widest group that the lanes of one workgroup hold: 256 lanes of 4 chunks, or in the backward pass (which holds four times as much) 512 of one
-#define ROW_MAX_BACKWARD 4096
+#define ROW_MAX 8192                    // widest group that the lanes of one workgroup hold: 256 lanes of 4 chunks, or in the backward pass (which holds four times as much) 512 of one or two
 
 // ---- dropout.  U chunks per thread: all loads are issued before the first mask is drawn.  In rows that are not contiguous (ROWS) a chunk that crosses
 //      the end of a row is loaded element by element.  Memory: 32768 x 4096 bf16 77 us = 7.0 TB/s read and written, with the reads past the caches (92 with them in the caches; with the
@@ -78,14 +77,14 @@ static double drop_scale(uint32_t cut) { return cut < 65536u ? 65536.0 / (65536.
 static int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static int log2_up(int64_t v) { int k = 0; while (((int64_t)1 << k) < v) k++; return k; }
 
-static bool by_rows(const PlenRegNorm &a, bool backward) { return a.L == 1 && a.C / a.G <= (backward ? ROW_MAX_BACKWARD : ROW_MAX_FORWARD); }
+static bool by_rows(const PlenRegNorm &a) { return a.L == 1 && a.C / a.G <= ROW_MAX; }
 // is a tensor of x's shape beyond what the caches keep for whoever reads it next?
 static bool streams(const PlenRegNorm &a) { return a.N * a.L * a.C * (a.dtype == PLENREG_F32 ? 4 : 2) >= STREAM_BYTES; }
 static RowLaunch row_plan(const PlenRegNorm &a, bool backward) {
     const int64_t chunks = div_up(a.C / a.G, 8);
     RowLaunch r;
     // forward: up to 4 chunks per lane, so that rows of up to 2048 elements need no barrier
-    r.K = backward || chunks <= 64 ? 1 : chunks <= 128 ? 2 : 4;
+    r.K = backward ? (chunks <= 512 ? 1 : 2) : chunks <= 64 ? 1 : chunks <= 128 ? 2 : 4;
     r.NT = backward ? 512 : 256;
     r.P.team_log = log2_up(div_up(chunks, r.K));
     const int teams = r.NT >> r.P.team_log;
@@ -233,7 +232,7 @@ int plenreg_dropout(const PlenRegDropout *a, void *stream) {
 
 int64_t plenreg_norm_workspace(const PlenRegNorm *a, int backward) {
     if (bad_norm(a)) return PLENREG_REFUSE;
-    if (by_rows(*a, backward)) return backward ? (int64_t)row_plan(*a, true).grid.x * 2 * a->C * 4 : 0;
+    if (by_rows(*a)) return backward ? (int64_t)row_plan(*a, true).grid.x * 2 * a->C * 4 : 0;
     if (a->L == 1) return backward ? (int64_t)wide_plan(*a).params.y * 2 * a->C * 4 : 0;
     const MapLaunch m = map_plan(*a, backward);
     if (m.slab) return backward ? (int64_t)m.param_rows * 2 * a->C * 4 : 0;
@@ -243,7 +242,7 @@ int64_t plenreg_norm_workspace(const PlenRegNorm *a, int backward) {
 int plenreg_norm_forward(const PlenRegNorm *a, void *stream) {
     if (bad_norm(a) || !a->x || !a->out || a->x_stride < 0 || (a->cut && !a->rng)) return PLENREG_REFUSE;
     NormArgs k = kernel_args(*a);
-    if (by_rows(*a, false)) {
+    if (by_rows(*a)) {
         entry(*a).row_forward(k, row_plan(*a, false), (hipStream_t)stream);
         return launched();
     }
@@ -260,7 +259,7 @@ int plenreg_norm_forward(const PlenRegNorm *a, void *stream) {
 
 int plenreg_norm_backward(const PlenRegNorm *a, void *stream) {
     if (bad_norm(a) || !a->x || !a->dy || !a->out || !a->stats || a->x_stride < 0 || a->dy_stride < 0 || (a->cut && !a->rng)) return PLENREG_REFUSE;
-    const bool params = a->dw || a->db, rows = by_rows(*a, true);
+    const bool params = a->dw || a->db, rows = by_rows(*a);
     if (plenreg_norm_workspace(a, 1) > 0 && (params || a->L > 1) && !a->ws) return PLENREG_REFUSE;
     const NormArgs k = kernel_args(*a);
     const NormEntry &e = entry(*a);

@@ -294,84 +294,95 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
 // Backward of the rows: one chunk a lane, since x, dy, dz, two parameters and their two gradients are held per element (two chunks: 200 registers, 59 us where this takes 53).  Sums
 // of a row in 32 bits: at most 4096 elements in a tree.  16384 x 2048 bf16 with dropout and SiLU 53 us, vector issue (47 instructions an element; its 201 MB alone would be 39 us); 4096 x 512
 // f32 10 us, 100 x 512 6 us.  Each workgroup leaves one row of partial parameter gradients: part[blockIdx.x][0 / 1][C] = dw, db of its rows, summed over its teams in LDS.
-template <int V, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT) void k_row_backward(NormArgs A, RowPlan P, float *part) {
+template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT) void k_row_backward(NormArgs A, RowPlan P, float *part) {
     __shared__ double2 lds[2][NT / 64];
-    __shared__ float joined[NT * 8];
+    __shared__ float joined[NT * 8 * K];
     const RowPlace p = row_place<NT>(A, P);
-    int c[1], valid[1];
-    row_chunks<1>(A, P, p, c, valid);
-    const int c0 = c[0], g0 = p.g < A.G ? p.g : A.G - 1;
+    int c[K], valid[K];
+    row_chunks<K>(A, P, p, c, valid);
+    const int g0 = p.g < A.G ? p.g : A.G - 1;
     // (as in the forward pass, additions instead of products)
     const int64_t rows = (int64_t)gridDim.x * P.rb, x_step = rows * A.x_stride, dy_step = rows * A.dy_stride, step = rows * A.C, st_step = rows * A.G;
-    int64_t n = (int64_t)blockIdx.x * P.rb + p.row, at = (n < A.N ? n : A.N - 1) * A.C + c0;
+    int64_t n = (int64_t)blockIdx.x * P.rb + p.row, at = (n < A.N ? n : A.N - 1) * A.C;
     const T *px = (const T *)A.x + (n < A.N ? n : A.N - 1) * A.x_stride, *pdy = (const T *)A.dy + (n < A.N ? n : A.N - 1) * A.dy_stride;
     const double2 *pst = A.stats + (n < A.N ? n : A.N - 1) * A.G + g0;
-    Chunk<DT> x = load_inside<V, DT, STREAM>(px, c0, A.C), g = load_inside<V, DT, STREAM>(pdy, c0, A.C);
+    Chunk<DT> x[K], g[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) { x[k] = load_inside<V, DT, STREAM>(px, c[k], A.C); g[k] = load_inside<V, DT, STREAM>(pdy, c[k], A.C); }
     double2 st = *pst;
-    float w[8], b[8], dw[8] = {}, db[8] = {};
-    row_params<V>(A, A.w, c0, 1.f, w);
-    row_params<V>(A, A.b, c0, 0.f, b);
+    float w[K][8], b[K][8], dw[K][8] = {}, db[K][8] = {};
+#pragma unroll
+    for (int k = 0; k < K; k++) { row_params<V>(A, A.w, c[k], 1.f, w[k]); row_params<V>(A, A.b, c[k], 0.f, b[k]); }
     Draw d = {};
     if (DROP) d = make_draw(A.rng, A.site, A.cut);
 #pragma unroll 1
     for (int turn = 0; turn < P.trips; turn++) {
         const bool on = n < A.N && valid[0];
-        float xh[8] = {}, gw[8] = {}, s = 0.f, q = 0.f, rstd = 0.f;
-        const Mask<DROP ? V + 1 : 0> m(d, at);
-        if (on) {
-            const float mean = (float)st.x, rest = (float)(st.x - (double)mean);
-            rstd = (float)st.y;
-            float dy[8], dz[8];
-            unpack(x, xh);
-            unpack(g, dy);
-            move_down<V>(xh, c0, A.C);
-            move_down<V>(dy, c0, A.C);
+        float xh[K][8] = {}, gw[K][8] = {}, s = 0.f, q = 0.f, rstd = 0.f;
+        Mask<DROP ? V + 1 : 0> m[K];
 #pragma unroll
-            for (int e = 0; e < 8; e++) xh[e] = ((m.keep(e, xh[e]) - mean) - rest) * rstd;
-            back_activation(A, px + c0, n, c0, valid[0], m, xh, dy, w, b, dz);
-            if (!V) {
+        for (int k = 0; k < K; k++) {
+            m[k] = Mask<DROP ? V + 1 : 0>(d, at + c[k]);
+            if (on && (K == 1 || valid[k])) {
+                const float mean = (float)st.x, rest = (float)(st.x - (double)mean);
+                rstd = (float)st.y;
+                float dy[8], dz[8];
+                unpack(x[k], xh[k]);
+                unpack(g[k], dy);
+                move_down<V>(xh[k], c[k], A.C);
+                move_down<V>(dy, c[k], A.C);
 #pragma unroll
-                for (int e = 0; e < 8; e++) dz[e] = e < valid[0] ? dz[e] : 0.f;
-            }
+                for (int e = 0; e < 8; e++) xh[k][e] = ((m[k].keep(e, xh[k][e]) - mean) - rest) * rstd;
+                back_activation(A, px + c[k], n, c[k], valid[k], m[k], xh[k], dy, w[k], b[k], dz);
+                if (!V) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                gw[e] = dz[e] * w[e];
-                s += gw[e]; q = fmaf(gw[e], xh[e], q);
-                db[e] += dz[e]; dw[e] = fmaf(dz[e], xh[e], dw[e]);
+                    for (int e = 0; e < 8; e++) dz[e] = e < valid[k] ? dz[e] : 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    gw[k][e] = dz[e] * w[k][e];
+                    s += gw[k][e]; q = fmaf(gw[k][e], xh[k][e], q);
+                    db[k][e] += dz[e]; dw[k][e] = fmaf(dz[e], xh[k][e], dw[k][e]);
+                }
             }
         }
         const int64_t here = at;
         n += rows;
         if (n < A.N) { px += x_step; pdy += dy_step; pst += st_step; at += step; }
         if (turn + 1 < P.trips) {                               // the next row's, while this one's sums are joined
-            x = load_inside<V, DT, STREAM>(px, c0, A.C); g = load_inside<V, DT, STREAM>(pdy, c0, A.C);
+#pragma unroll
+            for (int k = 0; k < K; k++) { x[k] = load_inside<V, DT, STREAM>(px, c[k], A.C); g[k] = load_inside<V, DT, STREAM>(pdy, c[k], A.C); }
             st = *pst;
         }
         team_sum2<NT>(s, q, P.team_log, turn, lds);
         if (on) {
             const float m1 = s * (float)A.inv_count, m2 = q * (float)A.inv_count;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                gw[e] = m.keep(e, rstd * (gw[e] - m1 - xh[e] * m2));
+            for (int k = 0; k < K; k++) {
+                if (K > 1 && !valid[k]) continue;
+#pragma unroll
+                for (int e = 0; e < 8; e++) gw[k][e] = m[k].keep(e, rstd * (gw[k][e] - m1 - xh[k][e] * m2));
+                row_store<V, STREAM>((T *)A.out + here + c[k], valid[k], gw[k]);
             }
-            row_store<V, STREAM>((T *)A.out + here, valid[0], gw);
         }
     }
     if (!part) return;
-    const int width = 8 << P.team_log, columns = P.gb * width;                  // joined[row][group of the workgroup][channel of the group, padded to whole chunks]
+    const int width = 8 * K << P.team_log, columns = P.gb * width;              // joined[row][group of the workgroup][channel of the group, padded to whole chunks]
 #pragma unroll 1
     for (int pass = 0; pass < 2; pass++) {
         __syncthreads();
         if (p.row < P.rb)
 #pragma unroll
-            for (int e = 0; e < 8; e++) joined[p.row * columns + p.gl * width + 8 * p.lane + e] = pass ? db[e] : dw[e];
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) joined[p.row * columns + p.gl * width + 8 * (p.lane + (k << P.team_log)) + e] = pass ? db[k][e] : dw[k][e];
         __syncthreads();
         for (int j = threadIdx.x; j < columns; j += NT) {
-            const int gj = j >> (P.team_log + 3), c = j & (width - 1), g = blockIdx.y * P.gb + gj;
-            if (g >= A.G || c >= A.D) continue;
+            const int gj = j >> (P.team_log + 2 + K), cc = j & (width - 1), gg = blockIdx.y * P.gb + gj;
+            if (gg >= A.G || cc >= A.D) continue;
             float t = 0.f;
             for (int r = 0; r < P.rb; r++) t += joined[r * columns + j];
-            part[((int64_t)blockIdx.x * 2 + pass) * A.C + g * A.D + c] = t;
+            part[((int64_t)blockIdx.x * 2 + pass) * A.C + gg * A.D + cc] = t;
         }
     }
 }
@@ -1059,7 +1070,8 @@ void row_forward(const NormArgs &a, const RowLaunch &r, hipStream_t s) {
     else a.cut ? row_forward_v<1, true, false>(a, r, s) : row_forward_v<1, false, false>(a, r, s);
 }
 template <int V, bool DROP, bool STREAM> void row_backward_v(const NormArgs &a, const RowLaunch &r, float *part, hipStream_t s) {
-    k_row_backward<V, 512, DROP, STREAM><<<r.grid, 512, 0, s>>>(a, r.P, part);
+    if (r.K == 1) k_row_backward<V, 1, 512, DROP, STREAM><<<r.grid, 512, 0, s>>>(a, r.P, part);
+    else k_row_backward<V, 2, 512, DROP, STREAM><<<r.grid, 512, 0, s>>>(a, r.P, part);
 }
 void row_backward(const NormArgs &a, const RowLaunch &r, float *part, hipStream_t s) {
     if (a.D % 8) a.cut ? row_backward_v<0, true, false>(a, r, part, s) : row_backward_v<0, false, false>(a, r, part, s);
