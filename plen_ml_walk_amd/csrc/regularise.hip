@@ -83,7 +83,8 @@ static bool streams(const PlenRegNorm &a) { return a.N * a.L * a.C * (a.dtype ==
 static RowLaunch row_plan(const PlenRegNorm &a, bool backward) {
     const int64_t chunks = div_up(a.C / a.G, 8);
     RowLaunch r;
-    // forward: up to 4 chunks per lane, so that rows of up to 2048 elements need no barrier
+    // forward: up to 4 chunks per lane, so that rows of up to 2048 elements need no barrier; backward: one while 512 lanes are enough (us, one / two chunks, bf16: 16384 x 4096 92 / 104,
+    // 16384 x 2048 49 / 59; f32 177 / 203, 89 / 108)
     r.K = backward ? (chunks <= 512 ? 1 : 2) : chunks <= 64 ? 1 : chunks <= 128 ? 2 : 4;
     r.NT = backward ? 512 : 256;
     r.P.team_log = log2_up(div_up(chunks, r.K));

@@ -291,9 +291,9 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
     }
 }
 
-// Backward of the rows: one chunk a lane, since x, dy, dz, two parameters and their two gradients are held per element (two chunks: 200 registers, 59 us where this takes 53).  Sums
-// of a row in 32 bits: at most 4096 elements in a tree.  16384 x 2048 bf16 with dropout and SiLU 53 us, vector issue (47 instructions an element; its 201 MB alone would be 39 us); 4096 x 512
-// f32 10 us, 100 x 512 6 us.  Each workgroup leaves one row of partial parameter gradients: part[blockIdx.x][0 / 1][C] = dw, db of its rows, summed over its teams in LDS.
+// Backward of the rows: one chunk a lane where that is enough, since x, dy, dz, two parameters and their two gradients are held per element (two chunks: 200 registers, half the waves).  Sums
+// of a row in 32 bits: at most 8192 elements in a tree.  16384 x 2048 bf16 with dropout and SiLU 50 us, vector issue (47 instructions an element; its 201 MB alone would be 39 us); 4096 x 512
+// f32 10 us, 100 x 512 6 us; 8192 x 8192 bf16 117 us (as two launches that read x and dy again 174).  Each workgroup leaves one row of partial parameter gradients: part[blockIdx.x][0 / 1][C] = dw, db of its rows, summed over its teams in LDS.
 template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT) void k_row_backward(NormArgs A, RowPlan P, float *part) {
     __shared__ double2 lds[2][NT / 64];
     __shared__ float joined[NT * 8 * K];
@@ -424,8 +424,8 @@ __global__ __launch_bounds__(1024) void k_row_params(NormArgs A, const float *pa
 }
 
 // ---- rows too wide for a workgroup's registers: one workgroup goes over a group twice, the second time out of the caches; the parameters are read with each chunk.  Its parameter gradients
-//      are a launch of their own, in which a thread owns a chunk column and walks down the rows.  8192 x 8192 bf16: backward 175 us (memory: x and dy come from there twice, once for either
-//      launch; 551 as slabs of one position); 4096 x 16384: forward 62 (198 as slabs), backward 177 (628).
+//      are a launch of their own, in which a thread owns a chunk column and walks down the rows.  4096 x 16384 bf16: forward 62 us = 4.3 TB/s, backward 177 (memory: x and dy come from
+//      there twice, once for either launch); as slabs of one position 198 and 628.
 template <int V> __device__ __forceinline__ int wide_valid(const NormArgs &A, int off) { return V || A.D - off > 8 ? 8 : A.D - off; }
 // forward; grid: (n, g) pairs
 template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(WIDE_NT) void k_wide_forward(NormArgs A) {
