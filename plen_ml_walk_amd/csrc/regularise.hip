@@ -143,12 +143,15 @@ static MapLaunch map_plan(const PlenRegNorm &a, bool backward) {
     m.P.col_blocks = (int)div_up(m.P.ncol, 512);
     m.P.bcol = (int)div_up(m.P.ncol, m.P.col_blocks);
     m.P.inv_bcol = 1.f / (float)m.P.bcol;
-    // one workgroup per slab: one launch instead of three, and the slab is read once from memory; but only as many compute units work as there are slabs.
-    // Measured (us, slab / split; N x L x C bf16): forward 8 x 32 x 320 6.3 / 8.2, 8 x 128 x 195 8.1 / 8.5, 8 x 1024 x 32 7.5 / 6.7, 64 x 128 x 320 10.8 / 11.0, 64 x 512 x 128 12.4 / 9.5,
-    // 256 x 128 x 320 13.6 / 16.5, 256 x 512 x 320 42.9 / 44.2; both passes 8 x 32 x 320 20.3 / 21.9 (1.9 of it forward), 8 x 512 x 32 18.7 / 17.4, 64 x 128 x 195 35.2 / 32.4,
-    // 256 x 32 x 320 23.5 / 38.6, 256 x 512 x 128 56.1 / 56.9, 256 x 512 x 320 120 / 167.
+    // one workgroup per slab: one launch instead of two or three, and the slab is read once from memory; but only as many compute units work as there are slabs, and nothing goes past
+    // the caches.  Measured (us, slab / split; N x L x C bf16): forward 8 x 32 x 320 6.3 / 8.2, 8 x 128 x 195 8.1 / 8.5, 8 x 1024 x 32 7.5 / 6.7, 64 x 128 x 320 10.8 / 11.0, 64 x 512 x 128
+    // 12.4 / 9.5, 256 x 128 x 320 13.6 / 16.5, 256 x 512 x 320 42.9 / 44.2, 2048 x 64 x 320 47 / 53, 20000 x 16 x 64 32 / 77, beyond what the caches hold 1024 x 512 x 320 203 / 170,
+    // 8192 x 256 x 64 145 / 132.  Backward, groups that share chunks: 8 x 32 x 320 14.0 / 13.7, 64 x 128 x 195 26.7 / 23.4, 256 x 32 x 320 16.4 / 27.8, 256 x 512 x 320 77 / 123, 1024 x 512 x 320
+    // 329 / 418; groups of whole chunks: 256 x 512 x 128 38.1 / 35.9, 2048 x 256 x 64 91 / 67, 20000 x 49 x 96 522 / 454, 20000 x 16 x 64 106 / 164.
+    const bool whole = a.C % 8 == 0 && D % 8 == 0, many = a.N >= 256 && size <= 262144;
     m.slab = m.P.bcol <= 448 && m.P.col_blocks == 1 && a.G <= 512
-             && ((a.N >= 256 && size <= 262144) || (backward ? size <= 8192 : size <= 25600 || (a.N >= 64 && size <= 40960)));
+             && (backward ? size <= (whole ? 4096 : 8192) || (many && !whole)
+                          : size <= 4096 || ((size <= 25600 || (a.N >= 64 && size <= 40960) || many) && a.N * size * (a.dtype == PLENREG_F32 ? 4 : 2) < (int64_t)192 << 20));
     const int64_t threads = div_up(chunks, 64) * 64;
     m.NT = m.slab ? fill_threads(m.P.bcol, threads < 448 ? (int)threads : 448, 448) : fill_threads(m.P.bcol, 256, 512);
     m.P.R = m.NT / m.P.bcol;
@@ -156,7 +159,6 @@ static MapLaunch map_plan(const PlenRegNorm &a, bool backward) {
     // helps: a slab with more than 2048 partial pairs, and the backward pass of groups that share chunks.  (us; 512 / 256 / 1024 workgroups: 8 x 4096 x 320 forward 17.0 / 18.3 / 19.5,
     // backward 42.4 / 35.6 / 56.9; 1 x 4096 x 512 in 8 groups 9.0 / 8.1 / 9.0 and 16.6 / 14.2 / 16.2; 2 x 16384 x 128 in 8 groups 9.8 / 10.1 / 12.0 and 16.6 / 18.5 / 20.9; 2 x 262144 x 128
     // sums 47 with 512, 40 with 1024)
-    const bool whole = a.C % 8 == 0 && D % 8 == 0;
     const int64_t groups = a.N * m.P.col_blocks;
     int64_t blocks = a.N * chunks >= (int64_t)1 << 22 ? 1024 : 512;
     if (blocks == 512 && ((backward && !whole) || div_up(512, groups) * a.G * m.P.col_blocks > 2048)) blocks = 256;
