@@ -292,7 +292,7 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
 }
 
 // Backward of the rows: one chunk a lane where that is enough, since x, dy, dz, two parameters and their two gradients are held per element (two chunks: 200 registers, half the waves).  Sums
-// of a row in 32 bits: at most 8192 elements in a tree.  16384 x 2048 bf16 with dropout and SiLU 50 us, vector issue (47 instructions an element; its 201 MB alone would be 39 us); 4096 x 512
+// of a row in 32 bits: at most 8192 elements in a tree.  16384 x 2048 bf16 with dropout and SiLU 50 us, vector issue (44 instructions an element; its 201 MB alone would be 39 us); 4096 x 512
 // f32 10 us, 100 x 512 6 us; 8192 x 8192 bf16 117 us (as two launches that read x and dy again 174).  Each workgroup leaves one row of partial parameter gradients: part[blockIdx.x][0 / 1][C] = dw, db of its rows, summed over its teams in LDS.
 template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_bounds__(NT) void k_row_backward(NormArgs A, RowPlan P, float *part) {
     __shared__ double2 lds[2][NT / 64];
