@@ -1,9 +1,9 @@
 // regularise_norm.hip -- group norm with an activation, with dropout before it or without, for one pair of element types: REG_DT of x and of the results, REG_WT of
 // the parameters; REG_ENTRY names the table of launches.
 //
-// Statistics are sums of (x - s) and (x - s)^2 in 64 bits, s = an element of the input: a 64-bit addition costs a vector slot like a 32-bit one on this chip, one
-// pass over the data is enough, the sums of different workgroups join by addition, a constant input has exactly no variance, and the variance survives a
-// mean of any size.  (It is also what the gate of ReLU's gradient is decided with.)  The rest is in 32 bits, with the mean as a sum of two floats, so that x - mean is
+// Statistics are sums of (x - s) and (x - s)^2 in 64 bits, s = the group's own first element: a 64-bit addition costs a vector slot like a 32-bit one on this chip, one
+// pass over the data is enough, the sums of different workgroups join by addition, a constant group has exactly no variance, the variance survives a
+// mean of any size, and a group's NaN or infinity stays its own.  (It is also what the gate of ReLU's gradient is decided with.)  The rest is in 32 bits, with the mean as a sum of two floats, so that x - mean is
 // exact to a rounding of its own.
 //
 // Code size counts: the instruction cache is cold at each launch, and a kernel that runs its text once is bound by fetching it.  So: quotients come from the
@@ -41,8 +41,7 @@ __device__ __forceinline__ double inverse_sqrt(double v) {
 }
 // sums of (x - s), (x - s)^2 -> the pair that NormArgs.stats holds
 __device__ __forceinline__ double2 finish_stats(const NormArgs &A, double s, double sum, double squares) {
-    double m = sum * A.inv_count;
-    m = fma(fma(-m, A.count, sum), A.inv_count, m);          // the quotient to its last bit: a group that is constant, or wholly dropped, beside a slab's other first element has exactly its mean
+    const double m = sum * A.inv_count;
     double var = fma(-m, m, squares * A.inv_count);
     if (var < 0.0) var = 0.0;
     return double2{s + m, A.scale * inverse_sqrt(fma(var, A.scale * A.scale, A.eps))};
@@ -623,10 +622,13 @@ struct Channel {
         if (c == A.C) { c = 0; g = 0; }
     }
 };
-// sums over the workgroup's threads of a[8], b[8] per virtual channel, joined per group: out[g stride] (zeros for a group with no channel in this workgroup's columns).
+struct Nothing { __device__ __forceinline__ float operator()(int) const { return 0.f; } };
+// sums over the workgroup's threads of a[8], b[8] per virtual channel, joined per group: result(g, before(g), sums) from one lane each (zeros for a group with no channel in this
+// workgroup's columns); before: what the result has to wait for, asked for first.
 // A thread leaves one pair per group that its chunk can reach: one (V = 2), two (groups of 8 and more channels) or eight.  `lds`: blockDim.x times as many.
 // (8 x 4096 x 320 with 32 groups, forward sums: 9.1 us with eight pairs always and the copies of a row one after the other; without any join 5.4.)
-template <int V> __device__ __forceinline__ void join_groups(const double (&a)[8], const double (&b)[8], const NormArgs &A, const MapPlan &P, const Column &c, double2 *lds, double2 *out, int64_t stride) {
+template <int V, class B, class F>
+__device__ __forceinline__ void join_groups(const double (&a)[8], const double (&b)[8], const NormArgs &A, const MapPlan &P, const Column &c, double2 *lds, B before, F result) {
     const int NT = blockDim.x, at = c.r * P.bcol + c.col - c.first;
     const bool two = V == 1 && A.D >= 8;
     __syncthreads();
@@ -654,6 +656,7 @@ template <int V> __device__ __forceinline__ void join_groups(const double (&a)[8
 #pragma unroll 1
     for (int g0 = 0; g0 < A.G; g0 += teams) {                        // (every lane takes every turn: the exchange needs them all)
         const int g = g0 + (threadIdx.x >> P.lanes_log);
+        const float first = before(g < A.G ? g : A.G - 1);
         double s = 0.0, q = 0.0;
         if (g < A.G)
 #pragma unroll 1
@@ -665,7 +668,7 @@ template <int V> __device__ __forceinline__ void join_groups(const double (&a)[8
                 s += t.x; q += t.y;
             }
         lanes_sum2(s, q, P.lanes_log);
-        if (g < A.G && lane == 0) out[(int64_t)g * stride] = double2{s, q};
+        if (g < A.G && lane == 0) result(g, first, s, q);
     }
 }
 // sums over the `splits` partial pairs of one (n, g), by one wave
@@ -675,13 +678,14 @@ __device__ __forceinline__ double2 join_splits(const double2 *part, int splits) 
     lanes_sum2(s, q, 6);
     return double2{s, q};
 }
-// the sums over the partial pairs of every group of a slab, by a whole workgroup: result(g, sums) from one lane each
-template <class F> __device__ __forceinline__ void join_slab(const NormArgs &A, const MapPlan &P, const double2 *part, F result) {
+// the sums over the partial pairs of every group of a slab, by a whole workgroup: before and result as in join_groups
+template <class B, class F> __device__ __forceinline__ void join_slab(const NormArgs &A, const MapPlan &P, const double2 *part, B before, F result) {
     const int parts = P.splits * P.col_blocks, step = 1 << P.join_log, lane = threadIdx.x & (step - 1), teams = blockDim.x >> P.join_log;
 #pragma unroll 1
     for (int g0 = 0; g0 < A.G; g0 += teams) {                        // (every lane takes every turn: the exchange needs them all)
         const int g = g0 + (threadIdx.x >> P.join_log);
         const double2 *p = part + (int64_t)(g < A.G ? g : A.G - 1) * parts;
+        const float first = before(g < A.G ? g : A.G - 1);
         double s = 0.0, q = 0.0;
 #pragma unroll 1
         for (int k = lane; k < parts; k += 8 * step) {
@@ -693,28 +697,54 @@ template <class F> __device__ __forceinline__ void join_slab(const NormArgs &A, 
                 if (k + j * step < parts) { s += t[j].x; q += t[j].y; }
         }
         lanes_sum2(s, q, P.join_log);
-        if (g < A.G && lane == 0) result(g, s, q);
+        if (g < A.G && lane == 0) result(g, first, s, q);
     }
 }
-// s of a slab: its first element, after the mask
-template <bool DROP> __device__ __forceinline__ double slab_shift(const NormArgs &A, const Draw &d, int64_t n) {
-    const float v = (float)((const T *)A.x)[n * A.x_stride];
-    return DROP && !kept(d, n * A.size) ? 0.0 : (double)v;
+// s of a group of a slab: its first element, after the mask.  (Not one for all of them: groups far from it would lose their variance, and its NaN or infinity would be theirs.)
+template <bool DROP> __device__ __forceinline__ float group_shift(const NormArgs &A, const Draw &d, int64_t n, int g) {
+    const float v = (float)((const T *)A.x)[n * A.x_stride + g * A.D];
+    return DROP && !kept(d, n * A.size + g * A.D) ? 0.f : v;
+}
+// ... of a thread's 8 virtual channels (V = 2: one group, element 0).  Masked and of more than two groups to a chunk: drawn once per group and shared in `lds` (G floats of the join's space),
+// rather than up to eight times by every thread.
+template <int V, bool DROP> __device__ __forceinline__ void load_shifts(const NormArgs &A, const Draw &d, int col, int64_t n, double2 *lds, float (&s)[V == 2 ? 1 : 8]) {
+    asm volatile("" : "+v"(col));                    // (as in load_constants)
+    Channel ch(A, 8 * col);
+    if (V == 2) s[0] = group_shift<DROP>(A, d, n, ch.g);
+    else if (A.D >= 8) {                             // the chunk reaches into one more group at most
+        const int split = A.D - ch.d;
+        const float s0 = group_shift<DROP>(A, d, n, ch.g), s1 = group_shift<DROP>(A, d, n, ch.g + 1 < A.G ? ch.g + 1 : 0);
+#pragma unroll
+        for (int e = 0; e < (V == 2 ? 1 : 8); e++) s[e] = e < split ? s0 : s1;
+    } else {
+        float *all = (float *)lds;
+        if (DROP) {
+            __syncthreads();
+            for (int g = threadIdx.x; g < A.G; g += blockDim.x) all[g] = group_shift<DROP>(A, d, n, g);
+            __syncthreads();
+        }
+#pragma unroll
+        for (int e = 0; e < (V == 2 ? 1 : 8); e++) { s[e] = DROP ? all[ch.g] : group_shift<DROP>(A, d, n, ch.g); ch.next(A); }
+    }
 }
 
-// s, q += the sums of (x - s), (x - s)^2 of a span of slab n, per virtual channel
-template <int V, bool DROP> __device__ __forceinline__ void span_sums(const NormArgs &A, const Draw &d, const Column &c, const Span &t, int64_t n, double (&s)[8], double (&q)[8]) {
+// s, q += the sums of (x - s), (x - s)^2 of a span of slab n, per virtual channel.  LEAN: a chunk's eight shifts stay in 32 bits until their use; carried in 64 bits through the loop they cost
+// one or two waves a SIMD (split sums of 1024 x 512 x 320: both forward launches 199 -> 176 us; slabs of one workgroup with dropout, 20000 x 16 x 66: 371 -> 332; without, small ones lose: 8 x 32 x 320
+// 6.9 -> 7.1)
+template <int V, bool DROP, bool LEAN> __device__ __forceinline__ void span_sums(const NormArgs &A, const Draw &d, const Column &c, const Span &t, int64_t n, double2 *lds, double (&s)[8], double (&q)[8]) {
     const T *x = (const T *)A.x + n * A.x_stride + t.base;
     int off = t.off;
     Chunk<DT> v;
     if (t.lim >= 8) v = span_load(x, t, off);
-    const double shift = slab_shift<DROP>(A, d, n);
+    float shift[V == 2 ? 1 : 8];
+    load_shifts<V, DROP>(A, d, c.col, n, lds, shift);
     const auto add = [&](const Chunk<DT> &chunk, int valid) {
         float f[8];
         unpack(chunk, Mask<DROP ? V : 0>(d, n * A.size + t.base + off), f);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const double u = e < valid ? (double)f[e] - shift : 0.0;
+            if (V == 1 && LEAN) asm("" : "+v"(shift[V == 2 ? 0 : e]));
+            const double u = e < valid ? (double)f[e] - (double)shift[V == 2 ? 0 : e] : 0.0;
             s[e] += u; q[e] = fma(u, u, q[e]);
         }
     };
@@ -730,7 +760,7 @@ template <int V, bool DROP> __device__ __forceinline__ void span_sums(const Norm
 }
 // part[n][g][split][column block] = sums of (x - s), (x - s)^2.  Grid: splits, column blocks, slabs.  2 x 262144 x 128 bf16 26 us = 5.2 TB/s (memory; a kernel that only reads gets to 6.3);
 // 8 x 4096 x 320 7.7 us, latency: 5.4 for the reading by 2.5 waves a SIMD, the rest the join.  (Two or three chunks on their way instead of one: no faster.)
-template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_sums(NormArgs A, MapPlan P, double2 *part) {
+template <int V, bool DROP> __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(DROP ? 5 : 6, 8))) void k_map_sums(NormArgs A, MapPlan P, double2 *part) {
     extern __shared__ double2 lds[];
     const Column c = my_column(P, blockIdx.y);
     const Span t = my_span(A, P, c, P.rows_per);
@@ -739,9 +769,10 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_sums(No
 #pragma unroll 1
     for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) {
         double s[8] = {}, q[8] = {};
-        span_sums<V, DROP>(A, d, c, t, n, s, q);
+        span_sums<V, DROP, true>(A, d, c, t, n, lds, s, q);
         const int64_t parts = (int64_t)P.splits * P.col_blocks;
-        join_groups<V>(s, q, A, P, c, lds, part + n * A.G * parts + blockIdx.x * P.col_blocks + blockIdx.y, parts);
+        double2 *out = part + n * A.G * parts + blockIdx.x * P.col_blocks + blockIdx.y;
+        join_groups<V>(s, q, A, P, c, lds, Nothing(), [&](int g, float, double a, double b) { out[g * parts] = double2{a, b}; });
     }
 }
 // one wave per (n, g), where a slab has too many partial pairs for every workgroup of the result to join them: ~4.3 us, a launch and two dependent loads
@@ -749,7 +780,8 @@ template <bool DROP> __global__ __launch_bounds__(256) void k_map_stats(NormArgs
     Draw d = {};
     if (DROP) d = make_draw(A.rng, A.site, A.cut);
     for (int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); item < A.N * A.G; item += (int64_t)gridDim.x * 4) {
-        const double shift = slab_shift<DROP>(A, d, item / A.G);
+        const int64_t n = item / A.G;
+        const double shift = group_shift<DROP>(A, d, n, (int)(item - n * A.G));
         const double2 t = join_splits(part + item * splits, splits);
         if ((threadIdx.x & 63) == 0) A.stats[item] = finish_stats(A, shift, t.x, t.y);
     }
@@ -838,12 +870,11 @@ template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(512) void 
     for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) 
         span_apply<V, DROP, STREAM>(A, P, d, c, t, n, [&]() -> const double2 * {
             if (!part) return A.stats + n * A.G;
-            const double shift = slab_shift<DROP>(A, d, n);
-            const bool first = A.stats && blockIdx.x == 0 && blockIdx.y == 0;
+            const bool writes = A.stats && blockIdx.x == 0 && blockIdx.y == 0;
             __syncthreads();
-            join_slab(A, P, part + n * A.G * P.splits * P.col_blocks, [&](int g, double sum, double squares) {
-                lds[g] = finish_stats(A, shift, sum, squares);
-                if (first) A.stats[n * A.G + g] = lds[g];
+            join_slab(A, P, part + n * A.G * P.splits * P.col_blocks, [&](int g) { return group_shift<DROP>(A, d, n, g); }, [&](int g, float shift, double sum, double squares) {
+                lds[g] = finish_stats(A, (double)shift, sum, squares);
+                if (writes) A.stats[n * A.G + g] = lds[g];
             });
             __syncthreads();
             return lds;
@@ -928,7 +959,8 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_su
 #pragma unroll
             for (int e = 0; e < 8; e++) { s1[e] *= (double)k.w[e]; s2[e] *= (double)k.w[e]; }
         const int64_t parts = (int64_t)P.splits * P.col_blocks;
-        join_groups<V>(s1, s2, A, P, c, lds, part + n * A.G * parts + blockIdx.x * P.col_blocks + blockIdx.y, parts);
+        double2 *out = part + n * A.G * parts + blockIdx.x * P.col_blocks + blockIdx.y;
+        join_groups<V>(s1, s2, A, P, c, lds, Nothing(), [&](int g, float, double a, double b) { out[g * parts] = double2{a, b}; });
     }
 }
 // second launch: the first workgroups join the splits of each (n, g) into {mean of w dz, mean of w dz xh}, the others the parameter gradients
@@ -1005,7 +1037,7 @@ __global__ __launch_bounds__(512) void k_map_back_apply(NormArgs A, MapPlan P, c
         span_back_apply<V, DROP, STREAM>(A, P, d, c, t, n, part ? A.inv_count : 1.0, [&]() -> const double2 * {
             if (!part) return means + n * A.G;
             __syncthreads();
-            join_slab(A, P, part + n * A.G * P.splits * P.col_blocks, [&](int g, double s1, double s2) { lds[g] = double2{s1, s2}; });
+            join_slab(A, P, part + n * A.G * P.splits * P.col_blocks, Nothing(), [&](int g, float, double s1, double s2) { lds[g] = double2{s1, s2}; });
             __syncthreads();
             return lds;
         });
@@ -1023,14 +1055,11 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_slab_forwar
 #pragma unroll 1
     for (int64_t n = blockIdx.y; n < A.N; n += gridDim.y) {
         double s[8] = {}, q[8] = {};
-        span_sums<V, DROP>(A, d, c, t, n, s, q);
-        join_groups<V>(s, q, A, P, c, lds, groups, 1);
-        __syncthreads();
-        const double shift = slab_shift<DROP>(A, d, n);
-        for (int g = threadIdx.x; g < A.G; g += blockDim.x) {
-            groups[g] = finish_stats(A, shift, groups[g].x, groups[g].y);
+        span_sums<V, DROP, DROP>(A, d, c, t, n, lds, s, q);
+        join_groups<V>(s, q, A, P, c, lds, [&](int g) { return group_shift<DROP>(A, d, n, g); }, [&](int g, float shift, double sum, double squares) {
+            groups[g] = finish_stats(A, (double)shift, sum, squares);
             if (A.stats) A.stats[n * A.G + g] = groups[g];
-        }
+        });
         __syncthreads();
         span_apply<V, DROP, false>(A, P, d, c, t, n, [&] { return groups; });
     }
@@ -1052,7 +1081,7 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_slab_backwa
 #pragma unroll
             for (int e = 0; e < 8; e++) { s1[e] *= (double)k.w[e]; s2[e] *= (double)k.w[e]; }
         }
-        join_groups<V>(s1, s2, A, P, c, lds, groups, 1);
+        join_groups<V>(s1, s2, A, P, c, lds, Nothing(), [&](int g, float, double a, double b) { groups[g] = double2{a, b}; });
         __syncthreads();
         span_back_apply<V, DROP, false>(A, P, d, c, t, n, A.inv_count, [&] { return groups; });
     }

@@ -510,3 +510,88 @@ def test_rows_wider_than_a_workgroup_holds(shape, groups, dtype):
     part = wide[:, 3:3 + shape[1]].requires_grad_()
     y, z = R.group_norm_act(x, groups, w, b), R.group_norm_act(part, groups, w, b)
     assert torch.equal(y, z) and all(torch.equal(s, t) for s, t in zip(torch.autograd.grad(y, (x, w, b), dy), torch.autograd.grad(z, (part, w, b), dy)))
+
+
+# ---- what one group holds is nothing to the others ---------------------------------------------------------------------------------------------
+# slabs by one workgroup, split ones joined in the result's launch and before it, of chunks that hold one group, two and more
+GROUPED = [((3, 50, 24), 3), ((3, 50, 30), 3), ((3, 50, 12), 4), ((300, 3, 2), 2), ((2, 20000, 16), 2),
+           ((2, 4096, 320), 32), ((2, 777, 195), 13), ((2, 4096, 64), 64), ((2, 4096, 512), 16), ((40, 2, 4096), 4096), ((300, 1000, 40), 8)]
+
+
+def _layer(x, dy, w, b, groups, act, p):
+    """y, dx, dw, db with dropout (p) or without."""
+    x, w, b = (t.detach().requires_grad_() for t in (x, w, b))
+    y = R.group_norm_act(x, groups, w, b, act=act) if p is None else R.dropout_norm_act(x, p, _rng(), groups, w, b, site=2, act=act)
+    return (y.detach(),) + torch.autograd.grad(y, (x, w, b), dy)
+
+
+def _spoil_elements(shape, groups, p):
+    """NaN and infinity as the first element of a slab, as the first channel of a group behind another, and as the last element: every other group's y, dx, dw and db are those of the
+    clean input, to the bit."""
+    d = shape[-1] // groups
+    x, dy, w, b = _case(shape, groups, torch.float32)
+    kept = torch.ones(shape, dtype=torch.bool) if p is None else O.keep(shape, p, _rng(), 2)
+    first_kept = lambda g: int(kept[1].view(-1, groups, d)[:, g].reshape(-1).nonzero()[0])  # noqa: E731
+    for act, bad in (("relu", float("nan")), ("silu", float("inf")), ("none", -float("inf"))):
+        clean = _layer(x, dy, w, b, groups, act, p)
+        for g, last in ((0, False), (1, False), (groups - 1, True)):
+            spoilt = x.detach().clone()
+            group = spoilt[1].view(-1, groups, d)[:, g]
+            at = first_kept(g)
+            if last:
+                at = int(kept[1].view(-1, groups, d)[:, g].reshape(-1).nonzero()[-1])
+            group[at // d, at % d] = bad
+            if p is not None:          # (whatever a dropped place holds)
+                drop = ~kept[1].view(-1, groups, d)[:, g].cuda()
+                group[drop] = float("nan")
+            hit = torch.zeros((shape[0], spoilt[0].numel() // shape[-1], groups, d), dtype=torch.bool, device="cuda")
+            hit[1, :, g] = True
+            hit, chan = hit.view(shape), hit.any(1).any(0).view(-1)
+            got = _layer(spoilt, dy, w, b, groups, act, p)
+            assert torch.isnan(got[0][hit]).all(), (act, g)
+            for name, a, c, at in zip(("y", "dx", "dw", "db"), got, clean, (~hit, ~hit, ~chan, ~chan)):
+                assert torch.equal(a[at], c[at]), (name, act, bad, g, last)
+
+
+def _spoil_parameters(shape, groups):
+    d = shape[-1] // groups
+    x, dy, w, b = _case(shape, groups, torch.float32)
+    for act in ("none", "silu"):
+        clean = _layer(x, dy, w, b, groups, act, None)
+        for which in (0, 1):
+            for bad in (float("nan"), float("inf")):
+                params = [w.detach().clone(), b.detach().clone()]
+                params[which][d] = bad               # the first channel of the second group
+                got = _layer(x, dy, params[0], params[1], groups, act, None)
+                others = torch.ones(groups, d, dtype=torch.bool, device="cuda")
+                others[1] = False
+                others = others.view(-1)
+                for name, a, c in zip(("y", "dx", "dw", "db"), got, clean):
+                    assert torch.equal(a[..., others], c[..., others]), (name, act, which, bad)
+
+
+@pytest.mark.parametrize("p", [None, 0.3])
+@pytest.mark.parametrize("shape,groups", GROUPED, ids=ids)
+def test_a_bad_element_spoils_its_own_group_only(shape, groups, p):
+    _spoil_elements(shape, groups, p)
+
+
+@pytest.mark.parametrize("shape,groups", GROUPED, ids=ids)
+def test_a_bad_parameter_spoils_its_own_group_only(shape, groups):
+    _spoil_parameters(shape, groups)
+
+
+@pytest.mark.parametrize("shape,groups", GROUPED, ids=ids)
+def test_groups_of_quite_different_sizes(shape, groups):
+    """The first group of each slab far away (an offset of 3e8, then 1e9 in its first element alone): the others keep their variance (64-bit sums around a value of another group would lose it)."""
+    x, dy, w, b = _case(shape, groups, torch.float32)
+    d = shape[-1] // groups
+    for p in (None, 0.3):
+        for far, part in ((3e8, slice(0, None)), (1e9, slice(0, 1))):
+            z = x.detach().clone()
+            group = z.view(shape[0], -1, groups, d)[:, :, 0]
+            if part.stop is None:
+                group += far
+            else:
+                group[:, 0, 0] = far
+            _check(z.requires_grad_(), dy, w, b, groups, "silu", p, _rng())
