@@ -171,6 +171,13 @@ template <int M> __device__ __forceinline__ void back_activation(const NormArgs 
     }
 }
 
+// zeros behind the first `valid` elements of a partial chunk.  What stands there is another group's, and zero times its NaN or infinity would be none of the zeros that sums count on.
+template <int V> __device__ __forceinline__ void clear_behind(float (&v)[8], int valid) {
+    if (V) return;
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = e < valid ? v[e] : 0.f;
+}
+
 // ---- rows of one position (L = 1): a team of lanes per (row, group), K chunks per lane held in registers, one pass.  Teams of one wave join their sums by lane exchange,
 //      wider ones through LDS.  A workgroup walks down the rows with its groups fixed, so that a lane keeps its channels: their parameters (and in the backward
 //      pass their gradients) stay in registers.
@@ -311,7 +318,7 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
     double2 st = *pst;
     float w[K][8], b[K][8], dw[K][8] = {}, db[K][8] = {};
 #pragma unroll
-    for (int k = 0; k < K; k++) { row_params<V>(A, A.w, c[k], 1.f, w[k]); row_params<V>(A, A.b, c[k], 0.f, b[k]); }
+    for (int k = 0; k < K; k++) { row_params<V>(A, A.w, c[k], 1.f, w[k]); row_params<V>(A, A.b, c[k], 0.f, b[k]); clear_behind<V>(w[k], valid[k]); }
     Draw d = {};
     if (DROP) d = make_draw(A.rng, A.site, A.cut);
 #pragma unroll 1
@@ -332,11 +339,9 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
                 move_down<V>(dy, c[k], A.C);
 #pragma unroll
                 for (int e = 0; e < 8; e++) xh[k][e] = ((m[k].keep(e, xh[k][e]) - mean) - rest) * rstd;
+                clear_behind<V>(xh[k], valid[k]);
                 back_activation(A, px + c[k], n, c[k], valid[k], m[k], xh[k], dy, w[k], b[k], dz);
-                if (!V) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) dz[e] = e < valid[k] ? dz[e] : 0.f;
-                }
+                clear_behind<V>(dz, valid[k]);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     gw[k][e] = dz[e] * w[k][e];
@@ -481,7 +486,7 @@ template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(WIDE_NT) v
         }
     }
 }
-// dz, xh and w of a chunk (zeros in dz behind the group's end)
+// dz, xh and w of a chunk (zeros behind the group's end)
 template <int V, bool DROP>
 __device__ __forceinline__ void wide_back(const NormArgs &A, const Mask<DROP ? V + 1 : 0> &m, const Chunk<DT> &x, const Chunk<DT> &g, const T *px, int64_t n, int c, int valid, double2 st, float (&w)[8], float (&xh)[8],
                                           float (&dz)[8]) {
@@ -495,11 +500,10 @@ __device__ __forceinline__ void wide_back(const NormArgs &A, const Mask<DROP ? V
     const float mean = (float)st.x, rest = (float)(st.x - (double)mean), rstd = (float)st.y;
 #pragma unroll
     for (int e = 0; e < 8; e++) xh[e] = ((m.keep(e, xh[e]) - mean) - rest) * rstd;
+    clear_behind<V>(xh, valid);
+    clear_behind<V>(w, valid);
     back_activation(A, px + c, n, c, valid, m, xh, dy, w, b, dz);
-    if (!V) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) dz[e] = e < valid ? dz[e] : 0.f;
-    }
+    clear_behind<V>(dz, valid);
 }
 // the gradient of x; grid: (n, g) pairs.  (Sums in 32 bits: a lane adds at most 64 elements before the lanes are joined.)
 template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(WIDE_NT) void k_wide_backward(NormArgs A) {

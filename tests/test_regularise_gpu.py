@@ -595,3 +595,27 @@ def test_groups_of_quite_different_sizes(shape, groups):
             else:
                 group[:, 0, 0] = far
             _check(z.requires_grad_(), dy, w, b, groups, "silu", p, _rng())
+
+
+# rows in whole and in partial chunks, and rows wider than a workgroup holds
+ROW_GROUPED = [((6, 512), 4), ((9, 26), 2), ((5, 3003), 3), ((300, 30), 10), ((2, 10002), 2), ((3, 24600), 3), ((3, 24603), 3)]
+
+
+@pytest.mark.parametrize("p", [None, 0.3])
+@pytest.mark.parametrize("shape,groups", ROW_GROUPED, ids=ids)
+def test_a_bad_element_of_a_row_spoils_its_own_group_only(shape, groups, p):
+    _spoil_elements(shape, groups, p)
+
+
+@pytest.mark.parametrize("shape,groups", ROW_GROUPED, ids=ids)
+def test_a_bad_parameter_of_a_row_spoils_its_own_group_only(shape, groups):
+    _spoil_parameters(shape, groups)
+
+
+@pytest.mark.parametrize("shape,groups", ROW_GROUPED, ids=ids)
+def test_groups_of_a_row_of_quite_different_sizes(shape, groups):
+    x, dy, w, b = _case(shape, groups, torch.float32)
+    with torch.no_grad():
+        x.view(shape[0], groups, -1)[:, 0] += 3e8
+    for p in (None, 0.3):
+        _check(x, dy, w, b, groups, "silu", p, _rng())
