@@ -46,9 +46,9 @@ __device__ __forceinline__ double2 finish_stats(const NormArgs &A, double s, dou
     if (var < 0.0) var = 0.0;
     return double2{s + m, A.scale * inverse_sqrt(fma(var, A.scale * A.scale, A.eps))};
 }
-// v - (mean + rest), the mean in two words, for a result.  What the first leaves out is below 2^-25 of the mean: for 16-bit elements, whose own steps are 2^-11 of theirs or more, it is
-// left out here too (one of about 40 instructions an element).  The backward pass, which has a gate to decide, takes both.
-__device__ __forceinline__ float from_mean(float v, float mean, float rest) { return DT == PLENREG_F32 ? (v - mean) - rest : v - mean; }
+// The normalised value with the mean in two words, mean + rest: (v - mean) rstd + offset, offset = -rest rstd once per group.  The first word alone is off by up to 2^-25 of the mean, which may be far
+// above the spread, in 16-bit types too: of 8000 elements around 1000, three of them a step higher, the others are half a percent off.
+__device__ __forceinline__ float from_mean(float v, float mean, float rstd, float offset) { return fmaf(v - mean, rstd, offset); }
 __device__ __forceinline__ void write_used(const NormArgs &A) {
     if (A.used && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) { A.used[0] = A.rng[0]; A.used[1] = A.rng[1]; }
 }
@@ -282,12 +282,12 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
         const double2 st = finish_stats(A, shift, s, q);
         if (on) {
             if (A.stats && p.lane == 0) A.stats[st_at] = st;
-            const float mean = (float)st.x, rest = (float)(st.x - (double)mean), rstd = (float)st.y;
+            const float mean = (float)st.x, rstd = (float)st.y, offset = -(float)(st.x - (double)mean) * rstd;
 #pragma unroll
             for (int k = 0; k < K; k++) {
                 if (!valid[k]) continue;
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[k][e] = from_mean(v[k][e], mean, rest) * rstd * w[k][e] + b[k][e];
+                for (int e = 0; e < 8; e++) v[k][e] = from_mean(v[k][e], mean, rstd, offset) * w[k][e] + b[k][e];
                 activate(v[k], A.act);
                 row_store<V, STREAM>((T *)A.out + at + c[k], valid[k], v[k]);
             }
@@ -465,7 +465,7 @@ template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(WIDE_NT) v
         team_sum2<WIDE_NT>(s, q, WIDE_LOG, turn, lds);
         const double2 st = finish_stats(A, shift, s, q);
         if (A.stats && threadIdx.x == 0) A.stats[item] = st;
-        const float mean = (float)st.x, rest = (float)(st.x - (double)mean), rstd = (float)st.y;
+        const float mean = (float)st.x, rstd = (float)st.y, offset = -(float)(st.x - (double)mean) * rstd;
         T *y = (T *)A.out + n * A.C + c0;
         off = 8 * threadIdx.x;
         x = load_inside<V, DT, STREAM>(px, c0 + (off < A.D ? off : 0), A.C);
@@ -480,7 +480,7 @@ template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(WIDE_NT) v
             row_params<V>(A, A.b, c0 + off, 0.f, b);
             const Mask<DROP ? V + 1 : 0> m(d, n * A.C + c0 + off);
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = from_mean(m.keep(e, v[e]), mean, rest) * rstd * w[e] + b[e];
+            for (int e = 0; e < 8; e++) v[e] = from_mean(m.keep(e, v[e]), mean, rstd, offset) * w[e] + b[e];
             activate(v, A.act);
             row_store<V, STREAM>(y + off, wide_valid<V>(A, off), v);
         }
@@ -842,11 +842,16 @@ template <int V, bool DROP, bool STREAM, class F> __device__ __forceinline__ voi
     Constants<V> k;
     load_constants<V>(A, P, ready(), c.col, k);
 #pragma unroll
-    for (int e = 0; e < 8; e++) k.w[e] *= k.rstd[V == 2 ? 0 : e];
+    for (int e = 0; e < 8; e++) {
+        // the result is (x - mean) w' + b', w' = w rstd, b' = b - rest w' (of an infinite w' the largest, so that no 0 inf comes in).  The mean's second word subtracted from each element instead: 1024 x 512 x 320 179 -> 214 us, registers.
+        const int i = V == 2 ? 0 : e;
+        k.w[e] *= k.rstd[i];
+        k.b[e] = fmaf(-k.rest[i], __builtin_amdgcn_fmed3f(k.w[e], -3e38f, 3e38f), k.b[e]);
+    }
     const auto result = [&](const Chunk<DT> &chunk, float (&f)[8]) {
         unpack(chunk, Mask<DROP ? V : 0>(d, n * A.size + t.base + off), f);
 #pragma unroll
-        for (int e = 0; e < 8; e++) f[e] = from_mean(f[e], k.mean[V == 2 ? 0 : e], k.rest[V == 2 ? 0 : e]) * k.w[e] + k.b[e];
+        for (int e = 0; e < 8; e++) f[e] = (f[e] - k.mean[V == 2 ? 0 : e]) * k.w[e] + k.b[e];
         activate(f, A.act);
     };
     float f[8];
@@ -864,7 +869,8 @@ template <int V, bool DROP, bool STREAM, class F> __device__ __forceinline__ voi
 }
 // The result: x once more, out of the caches where it fits.  2 x 262144 x 128 bf16 42 us = 6.4 TB/s read and written (memory); 8 x 4096 x 320 10.6 us, of it ~1.6 the join: latency.
 // part: the sums' partial pairs, joined by every workgroup for itself (the first of a slab writes the statistics down), or null: the statistics are there already
-template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(512) void k_map_apply(NormArgs A, MapPlan P, const double2 *part) {
+// (Waves per SIMD asked for, here, in k_map_sums and in k_slab_forward: the compiler's own choice took a register or two more and lost one of six, 1024 x 512 x 320 178 -> 214 us.)
+template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(DT == PLENREG_F32 || DROP ? 5 : 6, 8))) void k_map_apply(NormArgs A, MapPlan P, const double2 *part) {
     extern __shared__ double2 lds[];
     const Column c = my_column(P, blockIdx.y);
     const Span t = my_span(A, P, c, P.apply_rows);
@@ -1049,7 +1055,7 @@ __global__ __launch_bounds__(512) void k_map_back_apply(NormArgs A, MapPlan P, c
 
 // ---- slabs that one workgroup goes over by itself: the same passes in one launch, the second reading out of the nearer caches.
 //      256 x 512 x 320 bf16: forward 43 us, both passes 120 (split 44 and 167); 8 x 32 x 320 forward 6.3 (8.2).  `lds`: the join's space, then G pairs.
-template <int V, bool DROP> __global__ __launch_bounds__(512) void k_slab_forward(NormArgs A, MapPlan P) {
+template <int V, bool DROP> __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(DT == PLENREG_F32 ? 4 : 5, 8))) void k_slab_forward(NormArgs A, MapPlan P) {
     extern __shared__ double2 lds[];
     double2 *groups = lds + blockDim.x * (V == 2 ? 1 : 8);
     const Column c = my_column(P, 0);

@@ -619,3 +619,31 @@ def test_groups_of_a_row_of_quite_different_sizes(shape, groups):
         x.view(shape[0], groups, -1)[:, 0] += 3e8
     for p in (None, 0.3):
         _check(x, dy, w, b, groups, "silu", p, _rng())
+
+
+# ---- a mean far above the spread, in 16 bits ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("shape,groups", [((4, 512), 2), ((4, 8008), 1), ((4, 4011), 3), ((2, 20008), 1), ((3, 100, 80), 2), ((3, 200, 39), 3), ((2, 20000, 16), 2), ((2, 4096, 30), 3), ((2, 3000, 48), 2)], ids=ids)
+def test_few_elements_a_step_above_a_large_mean(shape, groups, dtype):
+    """Elements of 1000 (and of -1000), few of them a step of the type higher: the mean lies between two steps, and what separates most elements from it is far below both.  x - mean rounds once, relative to
+    itself; what the mean's first 24 bits leave out, below 2^-25 of it, is known to 24 bits of its own: e = 4 u |xh| + 2^-48 |mean| rstd before weight and bias (one rounding each, u of
+    the value), sums of a group in 64 bits."""
+    step = {torch.float32: 2.0 ** -13, torch.bfloat16: 4.0, torch.float16: 0.5}[dtype]
+    d = shape[-1] // groups
+    for sign in (1.0, -1.0):
+        g = _gen(31)
+        up = torch.rand(shape, generator=g) < 0.001
+        up.view(shape[0], -1, groups, d)[:, 0, :, 0] = True
+        x = (sign * (1000.0 + step * up)).to(dtype)
+        assert int((x.abs() > 1000).sum()) == int(up.sum())
+        w, b = torch.randn(shape[-1], generator=g) * 0.5 + 1, torch.randn(shape[-1], generator=g) * 0.5
+        for weight, bias in ((None, None), (w, b)):
+            y = R.group_norm_act(x.cuda(), groups, None if weight is None else weight.cuda(), None if bias is None else bias.cuda(), eps=1e-9, act="none")
+            ref = O.Norm(x, groups, weight, bias, 1e-9, "none")
+            mean, rstd = ref.stats
+            xh = ((x.double().view(shape[0], -1, groups, d) - mean) * rstd)
+            e = 4 * O.U * xh.abs() + 2.0 ** -48 * mean.abs() * rstd
+            e, xh = e.view(shape), xh.view(shape)
+            if weight is not None:
+                e = e * weight.double().abs() + 2 * O.U * ((xh * weight.double()).abs() + bias.double().abs())
+            O.inside("y", y, ref.y, e + O.half(dtype) * (ref.y.abs() + e) + O.tiny(dtype))
