@@ -192,7 +192,8 @@ struct WideLaunch { unsigned grid; dim3 params; bool stream; };
 // workgroup of the sums, apply_rows in one of the result; 2^lanes_log lanes join one group
 struct MapPlan { int q_log, ncol, bcol, col_blocks, R, splits, lanes_log, chan_log, join_log, param_z; int64_t rows, rows_per, apply_rows; float inv_bcol; };
 // slab: one workgroup does a slab by itself (the grid is `sums`, slabs along y)
-struct MapLaunch { MapPlan P; dim3 sums, apply; int NT, param_rows; unsigned stat_blocks; bool stream, slab, joins; };
+// walks: a workgroup of the sums goes over more than one slab
+struct MapLaunch { MapPlan P; dim3 sums, apply; int NT, param_rows; unsigned stat_blocks; bool stream, slab, joins, walks; };
 
 // one per pair of element types (x and results, parameters), in regularise_norm.hip
 struct NormEntry {
@@ -201,7 +202,7 @@ struct NormEntry {
     void (*wide_forward)(const NormArgs &, const WideLaunch &, hipStream_t);
     void (*wide_backward)(const NormArgs &, const WideLaunch &, float *part, hipStream_t);
     void (*map_forward)(const NormArgs &, const MapLaunch &, double2 *part, hipStream_t);
-    void (*map_backward)(const NormArgs &, const MapLaunch &, double2 *part, double2 *means, float *params, void *dw, void *db, hipStream_t);
+    void (*map_backward)(const NormArgs &, const MapLaunch &, double2 *part, double2 *means, float *params, double *running, void *dw, void *db, hipStream_t);
     void (*params)(const NormArgs &, const float *part, int rows, void *dw, void *db, hipStream_t);
 };
 const NormEntry &plenreg_norm_f32_f32();

@@ -183,6 +183,7 @@ static MapLaunch map_plan(const PlenRegNorm &a, bool backward) {
         m.sums = dim3(1, (unsigned)(a.N < 2048 ? a.N : 2048), 1);
         m.param_rows = (int)m.sums.y;
     }
+    m.walks = a.N > (m.slab ? m.sums.y : m.sums.z);
     // few partial pairs per slab: every workgroup of the result's launch joins them for itself (32 KB out of the caches at 2048 pairs), and there is no launch between.
     // Measured (us, so / with a launch of its own; bf16, pairs per slab): forward 8 x 4096 x 320 2048 18.4 / 19.5, 4096 19.1 / 19.4, 10240 22.5 / 19.5, 2 x 16384 x 128 2048 9.9 / 11.4,
     // 1 x 4096 x 512 16384 13.1 / 11.3; both passes 4 x 1089 x 195 455 36.4 / 38.5, 2275 37.2 / 39.0, 8 x 4096 x 320 2048 65.5 / 66.4, 4096 67.8 / 66.7
@@ -193,6 +194,8 @@ static MapLaunch map_plan(const PlenRegNorm &a, bool backward) {
     m.stat_blocks = (unsigned)(a.N * a.G < 4 * 65536 ? div_up(a.N * a.G, 4) : 65536);
     return m;
 }
+// bytes of a map launch's parameter sums: a row of 2 C per workgroup, and where it walks over slabs the same in 64 bits in front of them
+static int64_t sums_bytes(const PlenRegNorm &a, const MapLaunch &m) { return (int64_t)m.param_rows * 2 * a.C * (m.walks ? 12 : 4); }
 // bytes of the partial pairs of a map launch
 static int64_t part_bytes(const PlenRegNorm &a, const MapLaunch &m) { return a.N * a.G * m.P.splits * m.P.col_blocks * 16; }
 
@@ -238,8 +241,8 @@ int64_t plenreg_norm_workspace(const PlenRegNorm *a, int backward) {
     if (by_rows(*a)) return backward ? (int64_t)row_plan(*a, true).grid.x * 2 * a->C * 4 : 0;
     if (a->L == 1) return backward ? (int64_t)wide_plan(*a).params.y * 2 * a->C * 4 : 0;
     const MapLaunch m = map_plan(*a, backward);
-    if (m.slab) return backward ? (int64_t)m.param_rows * 2 * a->C * 4 : 0;
-    return part_bytes(*a, m) + a->N * a->G * 16 + (backward ? (int64_t)m.param_rows * 2 * a->C * 4 : 0);
+    if (m.slab) return backward ? sums_bytes(*a, m) : 0;
+    return part_bytes(*a, m) + a->N * a->G * 16 + (backward ? sums_bytes(*a, m) : 0);
 }
 
 int plenreg_norm_forward(const PlenRegNorm *a, void *stream) {
@@ -281,8 +284,9 @@ int plenreg_norm_backward(const PlenRegNorm *a, void *stream) {
     const MapLaunch m = map_plan(*a, true);
     char *ws = (char *)a->ws;
     double2 *means = (double2 *)(ws + part_bytes(*a, m));
-    float *sums = !params ? nullptr : m.slab ? (float *)ws : (float *)(means + a->N * a->G);
-    e.map_backward(k, m, (double2 *)ws, means, sums, a->dw, a->db, (hipStream_t)stream);
+    double *running = !params ? nullptr : m.slab ? (double *)ws : (double *)(means + a->N * a->G);
+    float *sums = (float *)(running && m.walks ? running + (int64_t)m.param_rows * 2 * a->C : running);
+    e.map_backward(k, m, (double2 *)ws, means, sums, running, a->dw, a->db, (hipStream_t)stream);
     return launched();
 }
 

@@ -920,8 +920,10 @@ template <int V, bool DROP> __device__ __forceinline__ void span_back_sums(const
     // (of the part's other elements dy is zero)
     if (V == 1 && off < t.lim) add(load_chunk<DT>(x + off, t.lim - off), load_chunk<DT>(dy + off, t.lim - off), t.lim - off);
 }
-// the workgroup's channel sums into `to`[0 / 1][C] = sums of dz xh, dz: written the first time, then added to (each thread to its own words)
-__device__ __forceinline__ void channel_sums(const double (&s1)[8], const double (&s2)[8], const NormArgs &A, const MapPlan &P, const Column &c, double2 *lds, float *to, bool first_time) {
+// the workgroup's channel sums over its slabs, to[0 / 1][C] = sums of dz xh, dz, written with the last slab; between two slabs they are in running[0 / 1][C], in 64 bits: a workgroup of a tensor of
+// 2^31 slabs walks over thousands of them.  (Each thread reads its own words there; with one slab to a workgroup there are none.)
+__device__ __forceinline__ void channel_sums(const double (&s1)[8], const double (&s2)[8], const NormArgs &A, const MapPlan &P, const Column &c, double2 *lds, float *to, double *running, bool first_time,
+                                             bool last_time) {
     const int NT = blockDim.x, lanes = 1 << P.chan_log, lane = threadIdx.x & (lanes - 1);
     __syncthreads();
     if (c.mine)
@@ -943,15 +945,15 @@ __device__ __forceinline__ void channel_sums(const double (&s1)[8], const double
             }
         lanes_sum2(s, q, P.chan_log);
         if (ch < last && lane == 0) {
-            float *word = to + ch;
-            word[0] = first_time ? (float)s : word[0] + (float)s;
-            word[A.C] = first_time ? (float)q : word[A.C] + (float)q;
+            if (!first_time) { s += running[ch]; q += running[A.C + ch]; }
+            if (last_time) { to[ch] = (float)s; to[A.C + ch] = (float)q; }
+            else { running[ch] = s; running[A.C + ch] = q; }
         }
     }
 }
 // Backward, first launch: 4 x 1089 x 195 f16 11.9 us, of it two joins in LDS; per workgroup the channel sums (params[workgroup][2][C]), per split their w-weighted group sums (part[n][g][split][column block] = sum w dz, sum w dz xh), in 64
 // bits.
-template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_sums(NormArgs A, MapPlan P, double2 *part, float *params) {
+template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_sums(NormArgs A, MapPlan P, double2 *part, float *params, double *running) {
     extern __shared__ double2 lds[];
     const Column c = my_column(P, blockIdx.y);
     const Span t = my_span(A, P, c, P.rows_per);
@@ -964,7 +966,10 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_map_back_su
         double s1[8] = {}, s2[8] = {};
         Constants<V> k;
         span_back_sums<V, DROP>(A, P, d, c, t, n, k, s1, s2);
-        if (params) channel_sums(s1, s2, A, P, c, lds, params + (row * gridDim.x + blockIdx.x) * 2 * A.C, n == blockIdx.z);
+        if (params) {
+            const int64_t at = (row * gridDim.x + blockIdx.x) * 2 * A.C;
+            channel_sums(s1, s2, A, P, c, lds, params + at, running + at, n == blockIdx.z, n + gridDim.z >= A.N);
+        }
         if (c.mine)
 #pragma unroll
             for (int e = 0; e < 8; e++) { s1[e] *= (double)k.w[e]; s2[e] *= (double)k.w[e]; }
@@ -1074,7 +1079,7 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) __attribute__((amd
         span_apply<V, DROP, false>(A, P, d, c, t, n, [&] { return groups; });
     }
 }
-template <int V, bool DROP> __global__ __launch_bounds__(512) void k_slab_backward(NormArgs A, MapPlan P, float *params) {
+template <int V, bool DROP> __global__ __launch_bounds__(512) void k_slab_backward(NormArgs A, MapPlan P, float *params, double *running) {
     extern __shared__ double2 lds[];
     double2 *groups = lds + blockDim.x * 8;
     const Column c = my_column(P, 0);
@@ -1087,7 +1092,8 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) void k_slab_backwa
         {
             Constants<V> k;
             span_back_sums<V, DROP>(A, P, d, c, t, n, k, s1, s2);
-            if (params) channel_sums(s1, s2, A, P, c, lds, params + (int64_t)blockIdx.y * 2 * A.C, n == blockIdx.y);
+            const int64_t at = (int64_t)blockIdx.y * 2 * A.C;
+            if (params) channel_sums(s1, s2, A, P, c, lds, params + at, running + at, n == blockIdx.y, n + gridDim.y >= A.N);
 #pragma unroll
             for (int e = 0; e < 8; e++) { s1[e] *= (double)k.w[e]; s2[e] *= (double)k.w[e]; }
         }
@@ -1155,13 +1161,13 @@ void map_forward(const NormArgs &a, const MapLaunch &m, double2 *part, hipStream
     if (one_group(a)) a.cut ? map_forward_v<2, true>(a, m, part, s) : map_forward_v<2, false>(a, m, part, s);
     else a.cut ? map_forward_v<1, true>(a, m, part, s) : map_forward_v<1, false>(a, m, part, s);
 }
-template <int V, bool DROP> void map_backward_v(const NormArgs &a, const MapLaunch &m, double2 *part, double2 *means, float *sums, void *dw, void *db, hipStream_t s) {
+template <int V, bool DROP> void map_backward_v(const NormArgs &a, const MapLaunch &m, double2 *part, double2 *means, float *sums, double *running, void *dw, void *db, hipStream_t s) {
     if (m.slab) {
-        k_slab_backward<V, DROP><<<m.sums, m.NT, (size_t)m.NT * 128 + a.G * 16, s>>>(a, m.P, sums);
+        k_slab_backward<V, DROP><<<m.sums, m.NT, (size_t)m.NT * 128 + a.G * 16, s>>>(a, m.P, sums, running);
         if (sums) params(a, sums, m.param_rows, dw, db, s);
         return;
     }
-    k_map_back_sums<V, DROP><<<m.sums, m.NT, (size_t)m.NT * 128, s>>>(a, m.P, part, sums);
+    k_map_back_sums<V, DROP><<<m.sums, m.NT, (size_t)m.NT * 128, s>>>(a, m.P, part, sums, running);
     MapPlan P = m.P;
     dim3 grid = m.apply;
     size_t lds = 0;
@@ -1181,9 +1187,9 @@ template <int V, bool DROP> void map_backward_v(const NormArgs &a, const MapLaun
     if (m.stream) k_map_back_apply<V, DROP, true><<<grid, m.NT, lds, s>>>(a, P, join, means, sums, m.param_rows, dw, db);
     else k_map_back_apply<V, DROP, false><<<grid, m.NT, lds, s>>>(a, P, join, means, sums, m.param_rows, dw, db);
 }
-void map_backward(const NormArgs &a, const MapLaunch &m, double2 *part, double2 *means, float *sums, void *dw, void *db, hipStream_t s) {
-    if (one_group(a)) a.cut ? map_backward_v<2, true>(a, m, part, means, sums, dw, db, s) : map_backward_v<2, false>(a, m, part, means, sums, dw, db, s);
-    else a.cut ? map_backward_v<1, true>(a, m, part, means, sums, dw, db, s) : map_backward_v<1, false>(a, m, part, means, sums, dw, db, s);
+void map_backward(const NormArgs &a, const MapLaunch &m, double2 *part, double2 *means, float *sums, double *running, void *dw, void *db, hipStream_t s) {
+    if (one_group(a)) a.cut ? map_backward_v<2, true>(a, m, part, means, sums, running, dw, db, s) : map_backward_v<2, false>(a, m, part, means, sums, running, dw, db, s);
+    else a.cut ? map_backward_v<1, true>(a, m, part, means, sums, running, dw, db, s) : map_backward_v<1, false>(a, m, part, means, sums, running, dw, db, s);
 }
 
 }  // namespace

@@ -647,3 +647,28 @@ def test_few_elements_a_step_above_a_large_mean(shape, groups, dtype):
             if weight is not None:
                 e = e * weight.double().abs() + 2 * O.U * ((xh * weight.double()).abs() + bias.double().abs())
             O.inside("y", y, ref.y, e + O.half(dtype) * (ref.y.abs() + e) + O.tiny(dtype))
+
+
+# ---- parameter gradients over very many slabs ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("shape,groups", [((1 << 21, 2, 8), 1), ((1 << 20, 2, 6), 2), ((9000, 520, 8), 1), ((9000, 420, 10), 2), ((70000, 3, 5), 1), ((4097, 2, 4104), 3)], ids=ids)
+def test_parameter_gradients_over_very_many_slabs(shape, groups):
+    """Gradients all alike, so that 32-bit sums round the same way each time.  Each dz xh is off by (6 + 1) u and what xh itself is off by (as in the oracle), and its sums are in 64 bits over
+    the slabs of a workgroup, rounded once, then in 64 bits again: 2 u of the sum of sizes."""
+    g = torch.Generator("cuda").manual_seed(5)
+    x = torch.randn(shape, device="cuda", generator=g)
+    w, b = torch.ones(shape[-1], device="cuda", requires_grad=True), torch.zeros(shape[-1], device="cuda", requires_grad=True)
+    dy = torch.full(shape, 1.0001, device="cuda")
+    y = R.group_norm_act(x, groups, w, b, act="none")
+    dw, db = torch.autograd.grad(y, (w, b), dy)
+    want = dy[0, 0, 0].item() * shape[0] * shape[1]
+    assert float((db.double() - want).abs().max()) <= 2 * O.U * want
+    total, bound = torch.zeros(2, shape[-1], dtype=torch.float64, device="cuda")
+    for part in x.split(max(1, (1 << 24) // (shape[1] * shape[2]))):
+        v = part.double().view(part.shape[0], -1, groups, shape[-1] // groups)
+        mean = v.mean((1, 3), keepdim=True)
+        rstd = 1 / torch.sqrt(((v - mean) ** 2).mean((1, 3), keepdim=True) + float(np.float32(1e-5)))
+        xh = ((v - mean) * rstd).reshape(part.shape)
+        size = ((v.abs() + mean.abs()) * rstd).reshape(part.shape)
+        total += (xh * dy[0, 0, 0].double()).sum((0, 1))
+        bound += ((6 * O.U * size + 3 * O.U * xh.abs()) * dy[0, 0, 0].double()).sum((0, 1))
+    assert bool(((dw.double() - total).abs() <= bound + O.U * total.abs()).all())
