@@ -12,6 +12,8 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include "../../include/plenreg.h"
 
@@ -52,6 +54,19 @@ variable_list once(variable_list out) {
 void check_alive(bool released) {
     TORCH_CHECK(!released, "Trying to backward through the graph a second time: the saved state of this operator has been released; pass retain_graph=True to the first backward");
 }
+// The nodes fill their results through raw pointers, which whoever records operations does not see: a traced call would return uninitialised memory.  Refused, as are tensors without memory of their own
+// (fake and functional ones, those of a functorch transform, subclasses that stand for others).
+void not_recorded() {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    using Key = c10::impl::TorchDispatchModeKey;
+    TORCH_CHECK(!torch::jit::tracer::isTracing() && !(Modes::any_modes_set() && (Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FUNCTIONAL))),
+                "plen_ml_walk_amd.regularise cannot be traced: its kernels are no library operations that a trace could record");
+}
+void own_memory(const Tensor &t) {
+    if (!t.defined()) return;
+    static const c10::DispatchKeySet wrappers({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::Batched, c10::DispatchKey::Functionalize});
+    TORCH_CHECK(!t.key_set().has_any(wrappers), "plen_ml_walk_amd.regularise needs tensors with memory of their own; functorch transforms (vmap, torch.func.grad), fake tensors and tensor subclasses are not supported");
+}
 void no_tangent(const Tensor &t) { TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "plen_ml_walk_amd.regularise has no forward-mode derivatives"); }
 
 // ---- dropout
@@ -90,6 +105,7 @@ struct DropoutNode : torch::autograd::Node {
         {
             std::lock_guard<std::mutex> lock(mutex_);
             check_alive(released);
+            not_recorded(); own_memory(dy[0]);
             const at::NoGradGuard off;
             if (dy[0].defined() && task_should_compute_output(0)) dx = run_dropout(dy[0], cut, used, site, Tensor());
         }
@@ -99,6 +115,7 @@ struct DropoutNode : torch::autograd::Node {
     std::string name() const override { return "RegulariseDropout"; }
 };
 Tensor dropout(const Tensor &x, int64_t cut, const Tensor &rng, int64_t site) {
+    not_recorded(); own_memory(x); own_memory(rng);
     no_tangent(x);
     if (!x.requires_grad() || !at::GradMode::is_enabled()) return run_dropout(x, cut, rng, site, Tensor());
     const std::shared_ptr<DropoutNode> node(new DropoutNode, torch::autograd::deleteNode);
@@ -171,6 +188,7 @@ struct NormNode : torch::autograd::Node {
         variable_list out(3);
         std::unique_lock<std::mutex> lock(mutex_);
         check_alive(released);
+        not_recorded(); own_memory(grads[0]);
         if (grads[0].defined()) {
             const at::NoGradGuard off;
             const Tensor x0 = x_.unpack(), w0 = w_.unpack(), b0 = b_.unpack();
@@ -207,6 +225,7 @@ struct NormNode : torch::autograd::Node {
 Tensor norm(const Tensor &x, const std::optional<Tensor> &weight, const std::optional<Tensor> &bias, int64_t groups, double eps, int64_t act, int64_t cut, const std::optional<Tensor> &rng_, int64_t site) {
     const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor()), rng = rng_.value_or(Tensor());
     const Form f = {groups, act, cut, site, eps};
+    not_recorded(); own_memory(x); own_memory(w); own_memory(b); own_memory(rng);
     no_tangent(x); no_tangent(w); no_tangent(b);
     if (!at::GradMode::is_enabled() || !(x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad())))
         return run_forward(x, w, b, f, rng, Tensor(), Tensor());
@@ -232,6 +251,7 @@ bool float_type(const Tensor &t) { const auto k = t.scalar_type(); return k == a
 bool good_x(PyObject *o) {
     if (!THPVariable_Check(o)) return false;
     const Tensor &x = THPVariable_Unpack(o);
+    own_memory(x);                                        // (before sizes are asked for, which may be symbols)
     return x.is_cuda() && x.layout() == at::kStrided && float_type(x);
 }
 bool to_int(PyObject *o, int64_t &v) {

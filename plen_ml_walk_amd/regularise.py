@@ -11,6 +11,9 @@ state; `advance` moves it on, once per iteration, as a kernel (so a captured gra
 forward's mask again from a 16-byte snapshot that the forward kernel takes.  (Who runs a forward pass a second time, as activation checkpointing does, has to do so before
 `advance`: it draws from the state as it then stands.)
 
+The kernels are no library operations: a call that is being traced (torch.jit.trace, make_fx, fake tensors) or transformed (vmap, torch.func.grad) is refused.  Under
+torch.compile the operators run as they are, between the compiled parts.
+
 CPU tensors take the same definitions as elementary torch operations (autograd differentiates them): the multi-process CPU path of td3.py."""
 import ctypes as C
 import importlib.util
@@ -120,6 +123,12 @@ def _check_draw(x, p, rng, site):
     return int(round(p * 65536))
 
 
+def _no_trace():
+    """The plain form reads the random state on the host: a trace would hold its mask as a constant.  (Device tensors: csrc/regularise_torch.cpp refuses any kind of recording.)"""
+    if torch.jit.is_tracing():
+        raise RuntimeError("plen_ml_walk_amd.regularise cannot be traced: the trace would draw one mask for ever")
+
+
 def _check_norm(x, groups, weight, bias, eps, act):
     if x.dim() < 2:
         raise ValueError("x has to be [N, C] or [N, ..., C], got %d dimension(s)" % x.dim())
@@ -190,6 +199,7 @@ def dropout(x, p, rng, site=0):
     _check_x(x)
     cut, site = _check_draw(x, p, rng, site), int(site)
     if x.device.type == "cpu":
+        _no_trace()
         return torch.where(_keep(x.shape, cut, rng, site), x.float() * _scale(cut), 0.0).to(x.dtype)
     return (_nodes or _load_nodes()).dropout(x, cut, rng, site)
 
@@ -220,5 +230,6 @@ def dropout_norm_act(x, p, rng, groups, weight=None, bias=None, site=0, eps=1e-5
     cut, site = _check_draw(x, p, rng, site), int(site)
     groups, eps = _check_norm(x, groups, weight, bias, eps, act), float(eps)
     if x.device.type == "cpu":
+        _no_trace()
         return _plain_norm(x, groups, weight, bias, eps, act, _keep(x.shape, cut, rng, site), cut)
     return (_nodes or _load_nodes()).norm(x, weight, bias, groups, eps, ACTS[act], cut, rng, site)

@@ -216,3 +216,47 @@ def test_missing_library_is_an_error(monkeypatch):
     monkeypatch.setattr(R, "LIB_PATH", "/nonexistent/libplenreg.so")
     with pytest.raises(R.PlenRegError):
         R.load()
+
+
+# ---- calls that are recorded or transformed
+def _nodes():
+    from plen_ml_walk_amd.build import build_regularise, build_regularise_nodes
+    build_regularise(), build_regularise_nodes()
+    return R._load_nodes()
+
+
+def recorded_calls(x, call):
+    """(kind, the call under it) for every way to record or to transform an operation."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def fake():
+        with FakeTensorMode() as mode:
+            return call(mode.from_tensor(x))
+
+    yield "trace", lambda: torch.jit.trace(call, x)
+    for mode in ("real", "fake", "symbolic"):
+        yield "make_fx " + mode, lambda mode=mode: make_fx(call, tracing_mode=mode)(x)
+    yield "fake", fake
+    yield "vmap", lambda: torch.vmap(call)(x[None].expand(3, *x.shape))
+    yield "grad", lambda: torch.func.grad(lambda v: call(v).sum())(x)
+    yield "functionalize", lambda: torch.func.functionalize(call)(x)
+
+
+@pytest.mark.parametrize("kind", ["dropout", "norm", "layer"])
+def test_the_nodes_refuse_to_be_recorded(kind):
+    """Before anything touches a device, so host tensors will do: what a trace recorded of the kernels' call would be the allocation of its result alone."""
+    nodes, x, rng, w = _nodes(), torch.randn(4, 8), R.new_rng("cpu", 1), torch.ones(8)
+    call = {"dropout": lambda v: nodes.dropout(v, 100, rng, 0), "norm": lambda v: nodes.norm(v, w, w, 2, 1e-5, 0, 0, None, 0), "layer": lambda v: nodes.norm(v, w, w, 2, 1e-5, 0, 100, rng, 0)}[kind]
+    for name, run in recorded_calls(x, call):
+        with pytest.raises(RuntimeError, match="plen_ml_walk_amd.regularise"):
+            run()
+
+
+def test_masks_are_not_traced_on_the_cpu():
+    x, rng, w = torch.randn(4, 8), R.new_rng("cpu", 1), torch.ones(8)
+    for call in (lambda v: R.dropout(v, 0.5, rng), lambda v: R.dropout_norm_act(v, 0.5, rng, 2, w)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, x)
+    traced, z = torch.jit.trace(lambda v: R.group_norm_act(v, 2, w), x), torch.randn(4, 8)
+    assert torch.equal(traced(z), R.group_norm_act(z, 2, w))

@@ -672,3 +672,18 @@ def test_parameter_gradients_over_very_many_slabs(shape, groups):
         total += (xh * dy[0, 0, 0].double()).sum((0, 1))
         bound += ((6 * O.U * size + 3 * O.U * xh.abs()) * dy[0, 0, 0].double()).sum((0, 1))
     assert bool(((dw.double() - total).abs() <= bound + O.U * total.abs()).all())
+
+
+@pytest.mark.parametrize("kind", ["dropout", "norm", "layer"])
+def test_calls_are_not_recorded(kind):
+    from test_regularise_cpu import recorded_calls
+    x, dy, w, b = _case((8, 64), 2, torch.float32)
+    rng = _rng()
+    call = {"dropout": lambda v: R.dropout(v, 0.3, rng), "norm": lambda v: R.group_norm_act(v, 2, w, b), "layer": lambda v: R.dropout_norm_act(v, 0.3, rng, 2, w, b)}[kind]
+    want = call(x)                                       # (the first call loads the library; the next ones take the short way in)
+    for name, run in recorded_calls(x.detach(), call):
+        with pytest.raises(RuntimeError, match="plen_ml_walk_amd.regularise"):
+            run()
+    with pytest.raises(RuntimeError, match="plen_ml_walk_amd.regularise"):
+        torch.autograd.grad(want, x, dy[None].expand(3, *dy.shape), is_grads_batched=True, retain_graph=True)
+    assert torch.equal(call(x), want)
