@@ -107,15 +107,16 @@ struct DropoutNode : torch::autograd::Node {
             check_alive(released);
             not_recorded(); own_memory(dy[0]);
             const at::NoGradGuard off;
-            if (dy[0].defined() && task_should_compute_output(0)) dx = run_dropout(dy[0], cut, used, site, Tensor());
+            if (dy[0].defined() && task_should_compute_output(0)) dx = run_dropout(dy[0].resolve_neg(), cut, used, site, Tensor());
         }
         return once({dx});
     }
     void release_variables() override { std::lock_guard<std::mutex> lock(mutex_); used.reset(); released = true; }
     std::string name() const override { return "RegulariseDropout"; }
 };
-Tensor dropout(const Tensor &x, int64_t cut, const Tensor &rng, int64_t site) {
-    not_recorded(); own_memory(x); own_memory(rng);
+Tensor dropout(const Tensor &x_, int64_t cut, const Tensor &rng_, int64_t site) {
+    not_recorded(); own_memory(x_); own_memory(rng_);
+    const Tensor x = x_.resolve_neg(), rng = rng_.resolve_neg();          // (a view whose memory holds the negatives, as the imaginary part of a conjugate)
     no_tangent(x);
     if (!x.requires_grad() || !at::GradMode::is_enabled()) return run_dropout(x, cut, rng, site, Tensor());
     const std::shared_ptr<DropoutNode> node(new DropoutNode, torch::autograd::deleteNode);
@@ -197,7 +198,7 @@ struct NormNode : torch::autograd::Node {
             Tensor dx = at::empty(x0.sizes(), x0.options().memory_format(at::MemoryFormat::Contiguous)), dw = want_w ? at::empty_like(w) : Tensor(), db = want_b ? at::empty_like(b) : Tensor();
             if (x0.numel()) {
                 int64_t xs, dys;
-                const Tensor x = as_slabs(x0, xs), dy = as_slabs(grads[0], dys);
+                const Tensor x = as_slabs(x0, xs), dy = as_slabs(grads[0].resolve_neg(), dys);
                 PlenRegNorm a = norm_args(x, w, b, f);
                 a.x = x.data_ptr(); a.x_stride = xs; a.dy = dy.data_ptr(); a.dy_stride = dys; a.out = dx.data_ptr(); a.stats = (double *)stats.data_ptr();
                 a.dw = want_w ? dw.data_ptr() : nullptr; a.db = want_b ? db.data_ptr() : nullptr;
@@ -222,10 +223,12 @@ struct NormNode : torch::autograd::Node {
     }
     std::string name() const override { return "RegulariseNormAct"; }
 };
-Tensor norm(const Tensor &x, const std::optional<Tensor> &weight, const std::optional<Tensor> &bias, int64_t groups, double eps, int64_t act, int64_t cut, const std::optional<Tensor> &rng_, int64_t site) {
-    const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor()), rng = rng_.value_or(Tensor());
+Tensor norm(const Tensor &x_, const std::optional<Tensor> &weight, const std::optional<Tensor> &bias, int64_t groups, double eps, int64_t act, int64_t cut, const std::optional<Tensor> &rng_, int64_t site) {
+    const auto values = [](const std::optional<Tensor> &t) { return t && t->defined() ? t->resolve_neg() : Tensor(); };
     const Form f = {groups, act, cut, site, eps};
-    not_recorded(); own_memory(x); own_memory(w); own_memory(b); own_memory(rng);
+    not_recorded(); own_memory(x_);
+    for (const auto *t : {&weight, &bias, &rng_}) if (*t) own_memory(**t);
+    const Tensor x = x_.resolve_neg(), w = values(weight), b = values(bias), rng = values(rng_);
     no_tangent(x); no_tangent(w); no_tangent(b);
     if (!at::GradMode::is_enabled() || !(x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad())))
         return run_forward(x, w, b, f, rng, Tensor(), Tensor());

@@ -687,3 +687,21 @@ def test_calls_are_not_recorded(kind):
     with pytest.raises(RuntimeError, match="plen_ml_walk_amd.regularise"):
         torch.autograd.grad(want, x, dy[None].expand(3, *dy.shape), is_grads_batched=True, retain_graph=True)
     assert torch.equal(call(x), want)
+
+
+def test_views_whose_memory_holds_the_negatives():
+    """The imaginary part of a conjugate is such a view; every tensor of a call may be one."""
+    rng = _rng()
+    one = torch.imag(torch.tensor([1.0 + 2.0j], device="cuda").conj())
+    assert one.is_neg() and R.dropout(one, 0.0, rng).item() == -2.0
+    x, dy, w, b = (t.detach() for t in _case((9, 48), 3, torch.float32))
+    neg = lambda t: torch._neg_view(-t)  # noqa: E731
+    assert neg(x).is_neg() and torch.equal(neg(x), x)
+    for call in (lambda x, w, b, r: R.dropout(x, 0.3, r), lambda x, w, b, r: R.group_norm_act(x, 3, w, b), lambda x, w, b, r: R.dropout_norm_act(x, 0.3, r, 3, w, b)):
+        for grad in (False, True):
+            leaf = x.clone().requires_grad_(grad)
+            want, got = call(leaf, w, b, rng), call(neg(leaf), neg(w), neg(b), neg(rng))
+            assert torch.equal(want, got)
+            if grad:
+                (a,), (c,) = torch.autograd.grad(want, leaf, dy), torch.autograd.grad(got, leaf, neg(dy))
+                assert torch.equal(a, c)
