@@ -20,6 +20,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.overrides import TorchFunctionMode
 
 from . import regularise as R
 
@@ -72,17 +73,27 @@ def _capturing(x):
     return x.is_cuda and torch.cuda.is_current_stream_capturing()
 
 
-def _linear(x, weight, bias):
+def _linear(x, weight, bias=None):
     """F.linear.  The library's bias gradient over many rows is a sum over several blocks that clears its counters with a memset, and such nodes leave wrong values from
     a captured graph's second replay on (at 4096 rows the biases' gradients were off by as much as they are large): while a stream is being captured the framework's own
     kernels take its place."""
-    if x.dim() == 2 and x.shape[0] > ONE_BLOCK and x.dtype == weight.dtype == torch.float32 and torch.is_grad_enabled() and weight.requires_grad and _capturing(x):
+    if x.dim() == 2 and x.shape[0] > ONE_BLOCK and x.dtype == weight.dtype == torch.float32 and bias is not None and torch.is_grad_enabled() and weight.requires_grad and _capturing(x):
         return _CapturedLinear.apply(x, weight, bias)
     return F.linear(x, weight, bias)
 
 
+class _CapturedForms(TorchFunctionMode):
+    """F.linear is _linear: within a module's own call, so that its hooks, or a forward that replaces its own, run as they do in an eager step."""
+
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        return (_linear if func is F.linear else func)(*args, **(kwargs or {}))
+
+
 def _layer(layer, x):
-    return _linear(x, layer.weight, layer.bias) if _capturing(x) else layer(x)
+    if not _capturing(x):
+        return layer(x)
+    with _CapturedForms():
+        return layer(x)
 
 
 def _mse(q, target):

@@ -124,3 +124,30 @@ def test_two_ranks_share_gradients_and_draw_their_own_masks(tmp_path):
     seeds = a["seeds"] + b["seeds"]
     assert len(set(seeds)) == 4
     assert a["mean_gradient_off"] <= 1e-6 * a["gradient"] + 1e-9          # the bucket is the mean of the two ranks' own gradients: two roundings of 2^-24
+
+
+@pytest.mark.parametrize("regularised", [False, True])
+def test_hooks_and_replaced_forwards_run_while_capturing(monkeypatch, regularised):
+    """A captured step calls the linear modules as an eager one does (here: the forward passes with the capture's switch on; gradients on the device in the GPU tests)."""
+    agent = _agent() if regularised else T.TD3Agent(26, 18, 1.0, device="cpu")
+    agent.critic.eval()
+    state, action, seen = torch.randn(300, 26), torch.rand(300, 18), []
+    modules = [agent.actor.fc1, agent.actor.fc3, agent.critic.fc2, agent.critic.fc6]
+    handles = [m.register_forward_hook(lambda m, i, o: seen.append(m) or 2 * o) for m in modules]
+    handles.append(agent.actor.fc2.register_forward_pre_hook(lambda m, i: seen.append(m)))
+    agent.critic.fc5.forward = lambda x: seen.append(agent.critic.fc5) or torch.nn.functional.linear(x, agent.critic.fc5.weight + 1, agent.critic.fc5.bias)
+    run = lambda: (agent.actor(state),) + tuple(agent.critic(state, action)) + (agent.critic.Q1(state, action),)  # noqa: E731
+    want, eager = run(), list(seen)
+    assert all(m in eager for m in modules + [agent.actor.fc2, agent.critic.fc5])
+    seen.clear()
+    monkeypatch.setattr(T, "_capturing", lambda x: True)
+    got = run()
+    assert seen == eager
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+    for h in handles:
+        h.remove()
+    assert "forward" not in vars(agent.actor.fc1)
+    bare = torch.nn.Linear(26, 5, bias=False)                   # a layer without a bias
+    (g,) = torch.autograd.grad(T._layer(bare, state).sum(), bare.weight)
+    assert torch.equal(g, torch.autograd.grad(bare(state).sum(), bare.weight)[0])

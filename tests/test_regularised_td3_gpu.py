@@ -125,3 +125,34 @@ def test_captured_policy_backward_equals_eager_at_every_replay(dropout, norm, B)
         torch.cuda.synchronize()
         assert float((agent._actor_grads.flat - want).abs().max()) <= 1.1e-3 * float(want.abs().max()), k
         assert abs(float(loss) - float(captured)) <= 1e-4
+
+
+@pytest.mark.parametrize("B,k,n", [(257, 26, 256), (4096, 256, 256), (4096, 256, 1), (9000, 44, 300)])
+def test_captured_layers_keep_their_hooks_and_their_gradients(B, k, n):
+    """One linear layer with a forward hook, forward and backward in a graph: the hook's work is part of it, and at every replay the gradients of weight and bias are their sums over the rows to the
+    roundings of the kernel's order: a quarter of one of 8 chunks of rows added one after the other, then the quarters and the chunks; the product rounds once."""
+    g = torch.Generator().manual_seed(B + n)
+    layer = torch.nn.Linear(k, n).cuda()
+    x, dy = torch.randn(B, k, generator=g).cuda(), torch.randn(B, n, generator=g).cuda()
+    calls = []
+    layer.register_forward_hook(lambda m, i, o: calls.append(m) or 2 * o)
+    step = lambda: torch.autograd.grad(T._layer(layer, x), (layer.weight, layer.bias), dy)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    calls.clear()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dw, db = step()
+    assert len(calls) == 1
+    depth = -(-B // 8) // 4 + 16 + 4 + 8 + 2
+    for replay in range(3):
+        x.normal_(), dy.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        x64, d64 = x.cpu().double(), 2 * dy.cpu().double()
+        for got, want, size in ((dw, d64.t() @ x64, d64.abs().t() @ x64.abs()), (db, d64.sum(0), d64.abs().sum(0))):
+            assert bool(((got.cpu().double() - want).abs() <= depth * 2.0 ** -24 * size).all()), replay
+        assert torch.isfinite(torch.randn(1 << 20, device="cuda").sum())              # the program's own work between replays
