@@ -169,7 +169,10 @@ class RegularisedCritic(Critic):
 
     The names fc1..fc6 are Critic's; norm1 / norm2 hold the weight and bias of the first / second hidden layers, [Q1's h | Q2's h].  Every forward in training mode
     draws new masks from the device state `rng` = {seed, calls} and moves it on by one call, on the device: a captured forward draws new masks at each replay.  eval()
-    leaves the dropout out.  `rng` is no part of the state_dict: ranks and target networks keep streams of their own (`seed_masks`)."""
+    leaves the dropout out.  `rng` is no part of the state_dict: ranks and target networks keep streams of their own (`seed_masks`).
+
+A forward pass that is run again within a backward pass, as activation checkpointing does, would draw other masks than the first one did: it is refused where there is dropout.  fc1 and fc4 are read, not called
+(their hooks do not run in `forward`, which multiplies by both at once)."""
 
     def __init__(self, state_dim, action_dim, dropout=0.0, norm=False, seed=0):
         super(RegularisedCritic, self).__init__(state_dim, action_dim)
@@ -187,6 +190,8 @@ class RegularisedCritic(Critic):
     def _hidden(self, x, layer, groups):
         """dropout -> layer norm -> ReLU of the `groups` networks' rows of hidden layer `layer` (0 or 1)."""
         drop = self.training and self.dropout > 0
+        if drop and torch._C._current_graph_task_id() != -1:
+            raise RuntimeError("a forward pass of RegularisedCritic within a backward pass (activation checkpointing) would draw other masks than the pass it repeats")
         if not self.norm:
             return F.relu(R.dropout(x, self.dropout, self.rng, site=layer) if drop else x)
         m = self.norm2 if layer else self.norm1

@@ -151,3 +151,23 @@ def test_hooks_and_replaced_forwards_run_while_capturing(monkeypatch, regularise
     bare = torch.nn.Linear(26, 5, bias=False)                   # a layer without a bias
     (g,) = torch.autograd.grad(T._layer(bare, state).sum(), bare.weight)
     assert torch.equal(g, torch.autograd.grad(bare(state).sum(), bare.weight)[0])
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpointed_critics_do_not_get_other_masks(reentrant):
+    """Activation checkpointing runs the forward pass again inside the backward pass, when the mask stream has moved on: other masks, and wrong gradients.  It is an error; without dropout it works."""
+    from torch.utils.checkpoint import checkpoint
+    g = torch.Generator().manual_seed(1)
+    state, action = torch.randn(20, 26, generator=g), torch.rand(20, 18, generator=g).requires_grad_()
+    for run in (lambda c: checkpoint(lambda s, a: sum(c(s, a)), state, action, use_reentrant=reentrant), lambda c: checkpoint(c.Q1, state, action, use_reentrant=reentrant)):
+        critic = _agent(0.3, True).critic
+        with pytest.raises(RuntimeError, match="mask"):
+            run(critic).sum().backward()
+        plain = _agent(0.0, True).critic
+        critic.eval()
+        for p in list(critic.parameters()) + list(plain.parameters()):
+            p.grad = None
+        run(plain).sum().backward()
+        run(critic).sum().backward()
+        for p, q in zip(critic.parameters(), plain.parameters()):
+            assert (p.grad is None) == (q.grad is None) and (p.grad is None or torch.equal(p.grad, q.grad))
