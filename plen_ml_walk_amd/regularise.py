@@ -101,6 +101,11 @@ def advance(rng):
     rng[1:].add_(1)
 
 
+def steps(p):
+    """The probability as the masks hold it, in steps of 2^-16: elements whose 16 bits are below this are dropped."""
+    return int(round(float(p) * 65536))
+
+
 # ---- argument checks -------------------------------------------------------------------------------------------------------------------------
 def _check_x(x):
     if not isinstance(x, torch.Tensor) or x.dtype not in DTYPES:
@@ -120,7 +125,7 @@ def _check_draw(x, p, rng, site):
         raise ValueError("site has to be in [0, 2^31 - 16), got %r" % (site,))
     if x.numel() > MAX_DRAWN:
         raise ValueError("a mask has at most 2^35 elements, x has %d" % x.numel())
-    return int(round(p * 65536))
+    return steps(p)
 
 
 def _no_trace():

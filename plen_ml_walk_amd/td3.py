@@ -178,6 +178,8 @@ A forward pass that is run again within a backward pass, as activation checkpoin
         super(RegularisedCritic, self).__init__(state_dim, action_dim)
         if not 0.0 <= float(dropout) < 1.0:
             raise ValueError("dropout has to be in [0, 1), got %r" % (dropout,))
+        if dropout and R.steps(dropout) in (0, 65536):
+            raise ValueError("dropout is held in steps of 2^-16: %r would drop nothing or everything" % (dropout,))
         self.dropout, self.norm = float(dropout), bool(norm)
         if self.norm:
             self.norm1, self.norm2 = _HiddenNorm(2 * self.fc1.out_features), _HiddenNorm(2 * self.fc2.out_features)

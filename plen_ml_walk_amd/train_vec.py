@@ -158,9 +158,12 @@ def main(argv=None):
     ap.add_argument("--critic-dropout", type=float, default=0.0, help="dropout on the critics' hidden layers (td3.RegularisedCritic; the autograd update, captured with --graphs 1)")
     ap.add_argument("--critic-norm", action="store_true", help="layer norm on the critics' hidden layers")
     a = ap.parse_args(argv)
+    from .regularise import steps
     regularised = bool(a.critic_dropout or a.critic_norm)
     if not 0.0 <= a.critic_dropout < 1.0:
         ap.error("--critic-dropout has to be in [0, 1)")
+    if a.critic_dropout and steps(a.critic_dropout) in (0, 65536):
+        ap.error("--critic-dropout is held in steps of 2^-16: %r would drop nothing or everything" % a.critic_dropout)
     if regularised and a.schedule == "pipelined":
         ap.error("--schedule pipelined runs the fused update of the plain critics; --critic-dropout and --critic-norm need --schedule sync")
     from . import sharding

@@ -171,3 +171,22 @@ def test_checkpointed_critics_do_not_get_other_masks(reentrant):
         run(critic).sum().backward()
         for p, q in zip(critic.parameters(), plain.parameters()):
             assert (p.grad is None) == (q.grad is None) and (p.grad is None or torch.equal(p.grad, q.grad))
+
+
+def test_dropout_that_its_steps_round_away_is_refused():
+    """The masks hold p in steps of 2^-16: what would drop nothing, or everything, is no regularisation."""
+    for bad in (1e-6, 2.0 ** -17, 1 - 2.0 ** -17, 1 - 1e-7, 0.9999999):
+        with pytest.raises(ValueError, match="dropout"):
+            T.TD3Agent(26, 18, 1.0, device="cpu", critic_dropout=bad)
+        with pytest.raises(ValueError, match="dropout"):
+            T.RegularisedCritic(26, 18, bad, True)
+    for good in (2.0 ** -16, 1 - 2.0 ** -16, 0.0):
+        assert T.RegularisedCritic(26, 18, good, True).dropout == good
+
+
+def test_train_vec_refuses_dropout_that_its_steps_round_away(capsys):
+    from plen_ml_walk_amd import train_vec
+    for bad in ("1e-6", "0.999999"):
+        with pytest.raises(SystemExit):
+            train_vec.main(["--critic-dropout", bad])
+        assert "2^-16" in capsys.readouterr().err
