@@ -705,3 +705,22 @@ def test_views_whose_memory_holds_the_negatives():
             if grad:
                 (a,), (c,) = torch.autograd.grad(want, leaf, dy), torch.autograd.grad(got, leaf, neg(dy))
                 assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("shape,groups", GROUPED + ROW_GROUPED, ids=ids)
+def test_a_bad_gradient_spoils_its_own_group_only(shape, groups):
+    """NaN and infinity in dy at the first channel of a group behind another, and at the last element: dx of every other group, dw and db of every other channel are those of the clean gradient."""
+    d = shape[-1] // groups
+    x, dy, w, b = _case(shape, groups, torch.float32)
+    for act, p, bad in (("silu", None, float("nan")), ("relu", 0.3, float("inf")), ("none", None, -float("inf"))):
+        clean = _layer(x, dy, w, b, groups, act, p)
+        for g, at in ((1, (0, 0)), (groups - 1, (-1, -1))):
+            spoilt = dy.clone()
+            spoilt[1].view(-1, groups, d)[:, g][at] = bad
+            hit = torch.zeros((shape[0], dy[0].numel() // shape[-1], groups, d), dtype=torch.bool, device="cuda")
+            hit[1, :, g] = True
+            chan = torch.zeros(groups, d, dtype=torch.bool, device="cuda")
+            chan[g, at[1]] = True
+            got = _layer(x, spoilt, w, b, groups, act, p)
+            for name, a, c, rest in zip(("y", "dx", "dw", "db"), got, clean, (torch.ones_like(hit).view(shape), ~hit.view(shape), ~chan.view(-1), ~chan.view(-1))):
+                assert torch.equal(a[rest], c[rest]), (name, act, bad, g)
