@@ -192,8 +192,8 @@ struct WideLaunch { unsigned grid; dim3 params; bool stream; };
 // workgroup of the sums, apply_rows in one of the result; 2^lanes_log lanes join one group
 struct MapPlan { int q_log, ncol, bcol, col_blocks, R, splits, lanes_log, chan_log, join_log, param_z; int64_t rows, rows_per, apply_rows; float inv_bcol; };
 // slab: one workgroup does a slab by itself (the grid is `sums`, slabs along y)
-// walks: a workgroup of the sums goes over more than one slab
-struct MapLaunch { MapPlan P; dim3 sums, apply; int NT, param_rows; unsigned stat_blocks; bool stream, slab, joins, walks; };
+// walks: a workgroup of the sums goes over more than one slab; lean: more than two workgroups of them to a compute unit (span_sums)
+struct MapLaunch { MapPlan P; dim3 sums, apply; int NT, param_rows; unsigned stat_blocks; bool stream, slab, joins, walks, lean; };
 
 // one per pair of element types (x and results, parameters), in regularise_norm.hip
 struct NormEntry {

@@ -183,6 +183,7 @@ static MapLaunch map_plan(const PlenRegNorm &a, bool backward) {
         m.sums = dim3(1, (unsigned)(a.N < 2048 ? a.N : 2048), 1);
         m.param_rows = (int)m.sums.y;
     }
+    m.lean = (int64_t)m.sums.x * m.sums.y * m.sums.z > 512;
     m.walks = a.N > (m.slab ? m.sums.y : m.sums.z);
     // few partial pairs per slab: every workgroup of the result's launch joins them for itself (32 KB out of the caches at 2048 pairs), and there is no launch between.
     // Measured (us, so / with a launch of its own; bf16, pairs per slab): forward 8 x 4096 x 320 2048 18.4 / 19.5, 4096 19.1 / 19.4, 10240 22.5 / 19.5, 2 x 16384 x 128 2048 9.9 / 11.4,

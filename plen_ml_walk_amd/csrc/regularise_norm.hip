@@ -733,8 +733,8 @@ template <int V, bool DROP> __device__ __forceinline__ void load_shifts(const No
 }
 
 // s, q += the sums of (x - s), (x - s)^2 of a span of slab n, per virtual channel.  LEAN: a chunk's eight shifts stay in 32 bits until their use; carried in 64 bits through the loop they cost
-// one or two waves a SIMD (split sums of 1024 x 512 x 320: both forward launches 199 -> 176 us; slabs of one workgroup with dropout, 20000 x 16 x 66: 371 -> 332; without, small ones lose: 8 x 32 x 320
-// 6.9 -> 7.1)
+// one or two waves a SIMD, converted at each use 8 instructions a chunk.  Split sums with more than two workgroups a compute unit, 1024 x 512 x 320: both forward launches 199 -> 176 us; slabs of one
+// workgroup with dropout, 20000 x 16 x 66: 371 -> 332.  Where fewer waves are there it loses: split sums of 8 x 4096 x 320 8.1 -> 8.6, slabs 8 x 32 x 320 without dropout 6.9 -> 7.1.
 template <int V, bool DROP, bool LEAN> __device__ __forceinline__ void span_sums(const NormArgs &A, const Draw &d, const Column &c, const Span &t, int64_t n, double2 *lds, double (&s)[8], double (&q)[8]) {
     const T *x = (const T *)A.x + n * A.x_stride + t.base;
     int off = t.off;
@@ -764,7 +764,7 @@ template <int V, bool DROP, bool LEAN> __device__ __forceinline__ void span_sums
 }
 // part[n][g][split][column block] = sums of (x - s), (x - s)^2.  Grid: splits, column blocks, slabs.  2 x 262144 x 128 bf16 26 us = 5.2 TB/s (memory; a kernel that only reads gets to 6.3);
 // 8 x 4096 x 320 7.7 us, latency: 5.4 for the reading by 2.5 waves a SIMD, the rest the join.  (Two or three chunks on their way instead of one: no faster.)
-template <int V, bool DROP> __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(DROP ? 5 : 6, 8))) void k_map_sums(NormArgs A, MapPlan P, double2 *part) {
+template <int V, bool DROP, bool LEAN> __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(DROP || !LEAN ? 5 : 6, 8))) void k_map_sums(NormArgs A, MapPlan P, double2 *part) {
     extern __shared__ double2 lds[];
     const Column c = my_column(P, blockIdx.y);
     const Span t = my_span(A, P, c, P.rows_per);
@@ -773,7 +773,7 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) __attribute__((amd
 #pragma unroll 1
     for (int64_t n = blockIdx.z; n < A.N; n += gridDim.z) {
         double s[8] = {}, q[8] = {};
-        span_sums<V, DROP, true>(A, d, c, t, n, lds, s, q);
+        span_sums<V, DROP, LEAN>(A, d, c, t, n, lds, s, q);
         const int64_t parts = (int64_t)P.splits * P.col_blocks;
         double2 *out = part + n * A.G * parts + blockIdx.x * P.col_blocks + blockIdx.y;
         join_groups<V>(s, q, A, P, c, lds, Nothing(), [&](int g, float, double a, double b) { out[g * parts] = double2{a, b}; });
@@ -1150,7 +1150,8 @@ bool one_group(const NormArgs &a) { return a.C % 8 == 0 && a.D % 8 == 0; }
 template <int V, bool DROP> void map_forward_v(const NormArgs &a, const MapLaunch &m, double2 *part, hipStream_t s) {
     const size_t lds = (size_t)m.NT * (V == 2 ? 16 : 128);
     if (m.slab) { k_slab_forward<V, DROP><<<m.sums, m.NT, lds + a.G * 16, s>>>(a, m.P); return; }
-    k_map_sums<V, DROP><<<m.sums, m.NT, lds, s>>>(a, m.P, part);
+    if (V == 2 || DROP || m.lean) k_map_sums<V, DROP, true><<<m.sums, m.NT, lds, s>>>(a, m.P, part);
+    else k_map_sums<V, DROP, V == 2 || DROP><<<m.sums, m.NT, lds, s>>>(a, m.P, part);
     if (!m.joins) k_map_stats<DROP><<<m.stat_blocks, 256, 0, s>>>(a, m.P.splits * m.P.col_blocks, part);
     const size_t stats = m.joins ? (size_t)a.G * 16 : 0;
     const double2 *join = m.joins ? part : nullptr;

@@ -515,7 +515,7 @@ def test_rows_wider_than_a_workgroup_holds(shape, groups, dtype):
 # ---- what one group holds is nothing to the others ---------------------------------------------------------------------------------------------
 # slabs by one workgroup, split ones joined in the result's launch and before it, of chunks that hold one group, two and more
 GROUPED = [((3, 50, 24), 3), ((3, 50, 30), 3), ((3, 50, 12), 4), ((300, 3, 2), 2), ((2, 20000, 16), 2),
-           ((2, 4096, 320), 32), ((2, 777, 195), 13), ((2, 4096, 64), 64), ((2, 4096, 512), 16), ((40, 2, 4096), 4096), ((300, 1000, 40), 8)]
+           ((2, 4096, 320), 32), ((2, 777, 195), 13), ((2, 4096, 64), 64), ((2, 4096, 512), 16), ((40, 2, 4096), 4096), ((300, 1000, 40), 8), ((530, 2, 4098), 683)]
 
 
 def _layer(x, dy, w, b, groups, act, p):
