@@ -1,7 +1,8 @@
 /*
  * plenreg.h -- C ABI of libplenreg.so: the regularisation operators of the Q networks' hidden layers as hand-written HIP kernels (gfx950):
  * dropout whose mask is drawn from the counter-based generator and never stored, group norm with an activation over channels-last data,
- * and the two in one pass, each with its gradient.  Bound with ctypes by plen_ml_walk_amd/regularise.py.
+ * and the two in one pass, each with its gradient.  plen_ml_walk_amd/regularise.py loads the library and hands its entry points to the autograd nodes of
+ * csrc/regularise_torch.cpp, which call them.
  *
  * Conventions: every pointer is a caller-owned DEVICE pointer; work is enqueued on the hipStream_t passed as `stream` and is capturable in a
  * hipGraph; nothing is allocated and no state is kept between calls.  Outputs overlap neither inputs nor each other.  Return 0, or a negative HIP error code (-1 = hipErrorInvalidValue:
@@ -62,7 +63,8 @@ typedef struct PlenRegNorm {
 } PlenRegNorm;
 #define PLENREG_MAX_C 32768            /* widest row with L = 1 */
 #define PLENREG_MAX_C_LONG 8192        /* widest row with L > 1 */
-/* y = act(((d(x) - mean) rstd) w + b), d = dropout (cut > 0) or the identity; mean and variance over the L x (C / G) elements of each (n, group) */
+/* y = act(((d(x) - mean) rstd) w + b), d = dropout (cut > 0) or the identity; mean and variance over the L x (C / G) elements of each (n, group).  What one group holds (NaN, infinity, any size)
+ * changes no other group's results, in either pass. */
 int plenreg_norm_forward(const PlenRegNorm *args, void *stream);
 /* dx, dw, db of the above from dy, x and stats */
 int plenreg_norm_backward(const PlenRegNorm *args, void *stream);

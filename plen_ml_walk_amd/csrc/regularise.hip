@@ -3,7 +3,8 @@
 #include "regularise.h"
 
 #define DROPOUT_SMALL (1 << 18)
-#define STREAM_BYTES ((int64_t)64 << 20)     // tensors from here on go past the caches where nobody reads them next (2 x 262144 x 128 bf16: sums 47 -> 26 us, result 42 -> 40)
+#define STREAM_BYTES ((int64_t)64 << 20)     // last readings and results of tensors from here on go past the caches (2 x 262144 x 128 bf16, passes back to back: sums 47 -> 26 us, since no results of the pass
+                                             // before have to be written back meanwhile; result 42 -> 40.  By size alone: what a later reader of the result pays was not measured)
 #define MAP_MAX_SPAN ((int64_t)1 << 28)      // elements of a slab that one workgroup walks over
 #define ROW_MAX 8192                    // widest group that the lanes of one workgroup hold: 256 lanes of 4 chunks, or in the backward pass (which holds four times as much) 512 of one or two
 
@@ -78,7 +79,7 @@ static int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static int log2_up(int64_t v) { int k = 0; while (((int64_t)1 << k) < v) k++; return k; }
 
 static bool by_rows(const PlenRegNorm &a) { return a.L == 1 && a.C / a.G <= ROW_MAX; }
-// is a tensor of x's shape beyond what the caches keep for whoever reads it next?
+// is a tensor of x's shape beyond what the caches keep?
 static bool streams(const PlenRegNorm &a) { return a.N * a.L * a.C * (a.dtype == PLENREG_F32 ? 4 : 2) >= STREAM_BYTES; }
 static RowLaunch row_plan(const PlenRegNorm &a, bool backward) {
     const int64_t chunks = div_up(a.C / a.G, 8);
@@ -144,7 +145,7 @@ static MapLaunch map_plan(const PlenRegNorm &a, bool backward) {
     m.P.bcol = (int)div_up(m.P.ncol, m.P.col_blocks);
     m.P.inv_bcol = 1.f / (float)m.P.bcol;
     // one workgroup per slab: one launch instead of two or three, and the slab is read once from memory; but only as many compute units work as there are slabs, and nothing goes past
-    // the caches.  Measured (us, slab / split; N x L x C bf16): forward 8 x 32 x 320 6.3 / 8.2, 8 x 128 x 195 8.1 / 8.5, 8 x 1024 x 32 7.5 / 6.7, 64 x 128 x 320 10.8 / 11.0, 64 x 512 x 128
+    // the caches.  Measured (us, slab / split; N x L x C bf16; before each group had its own shift, which costs both forms 1-5 %): forward 8 x 32 x 320 6.3 / 8.2, 8 x 128 x 195 8.1 / 8.5, 8 x 1024 x 32 7.5 / 6.7, 64 x 128 x 320 10.8 / 11.0, 64 x 512 x 128
     // 12.4 / 9.5, 256 x 128 x 320 13.6 / 16.5, 256 x 512 x 320 42.9 / 44.2, 2048 x 64 x 320 47 / 53, 20000 x 16 x 64 32 / 77, beyond what the caches hold 1024 x 512 x 320 203 / 170,
     // 8192 x 256 x 64 145 / 132.  Backward, groups that share chunks: 8 x 32 x 320 14.0 / 13.7, 64 x 128 x 195 26.7 / 23.4, 256 x 32 x 320 16.4 / 27.8, 256 x 512 x 320 77 / 123, 1024 x 512 x 320
     // 329 / 418; groups of whole chunks: 256 x 512 x 128 38.1 / 35.9, 2048 x 256 x 64 91 / 67, 20000 x 49 x 96 522 / 454, 20000 x 16 x 64 106 / 164.

@@ -763,7 +763,7 @@ template <int V, bool DROP, bool LEAN> __device__ __forceinline__ void span_sums
     if (V == 1 && off < t.lim) add(load_chunk<DT>(x + off, t.lim - off), t.lim - off);
 }
 // part[n][g][split][column block] = sums of (x - s), (x - s)^2.  Grid: splits, column blocks, slabs.  2 x 262144 x 128 bf16 26 us = 5.2 TB/s (memory; a kernel that only reads gets to 6.3);
-// 8 x 4096 x 320 7.7 us, latency: 5.4 for the reading by 2.5 waves a SIMD, the rest the join.  (Two or three chunks on their way instead of one: no faster.)
+// 8 x 4096 x 320 8.2 us, latency: 5.4 for the reading by 2.5 waves a SIMD, the rest the groups' shifts (0.3) and the join.  (Two or three chunks on their way instead of one: no faster.)
 template <int V, bool DROP, bool LEAN> __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(DROP || !LEAN ? 5 : 6, 8))) void k_map_sums(NormArgs A, MapPlan P, double2 *part) {
     extern __shared__ double2 lds[];
     const Column c = my_column(P, blockIdx.y);
@@ -867,7 +867,7 @@ template <int V, bool DROP, bool STREAM, class F> __device__ __forceinline__ voi
     }
     if (V == 1 && off < t.lim) { result(load_chunk<DT>(x + off, t.lim - off), f); store_chunk<DT>(y + off, t.lim - off, f); }
 }
-// The result: x once more, out of the caches where it fits.  2 x 262144 x 128 bf16 42 us = 6.4 TB/s read and written (memory); 8 x 4096 x 320 10.6 us, of it ~1.6 the join: latency.
+// The result: x once more, out of the caches where it fits.  2 x 262144 x 128 bf16 42 us = 6.4 TB/s read and written (memory); 8 x 4096 x 320 11.0 us, of it ~1.6 the join: latency.
 // part: the sums' partial pairs, joined by every workgroup for itself (the first of a slab writes the statistics down), or null: the statistics are there already
 // (Waves per SIMD asked for, here, in k_map_sums and in k_slab_forward: the compiler's own choice took a register or two more and lost one of six, 1024 x 512 x 320 178 -> 214 us.)
 template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(DT == PLENREG_F32 || DROP ? 5 : 6, 8))) void k_map_apply(NormArgs A, MapPlan P, const double2 *part) {
@@ -1059,7 +1059,7 @@ __global__ __launch_bounds__(512) void k_map_back_apply(NormArgs A, MapPlan P, c
 }
 
 // ---- slabs that one workgroup goes over by itself: the same passes in one launch, the second reading out of the nearer caches.
-//      256 x 512 x 320 bf16: forward 43 us, both passes 120 (split 44 and 167); 8 x 32 x 320 forward 6.3 (8.2).  `lds`: the join's space, then G pairs.
+//      256 x 512 x 320 bf16: forward 45 us, both passes 123 (split 44 and 167); 8 x 32 x 320 forward 7.0 (8.2).  `lds`: the join's space, then G pairs.
 template <int V, bool DROP> __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(DT == PLENREG_F32 ? 4 : 5, 8))) void k_slab_forward(NormArgs A, MapPlan P) {
     extern __shared__ double2 lds[];
     double2 *groups = lds + blockDim.x * (V == 2 ? 1 : 8);

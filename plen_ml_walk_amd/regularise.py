@@ -37,7 +37,7 @@ class PlenRegError(RuntimeError):
 
 
 class DropoutArgs(C.Structure):
-    """Mirror of PlenRegDropout (include/plenreg.h)."""
+    """Mirror of PlenRegDropout (include/plenreg.h), for callers of the C entry points (the operators below go through csrc/regularise_torch.cpp)."""
     _fields_ = ([(n, C.c_void_p) for n in ("x", "y", "rng", "used")] + [(n, C.c_int64) for n in ("rows", "cols", "x_stride")]
                 + [("dtype", C.c_int32), ("cut", C.c_uint32), ("site", C.c_int32)])
 
