@@ -173,7 +173,7 @@ struct NormArgs {
     const uint64_t *rng;
     uint64_t *used;
     int64_t N, x_stride, dy_stride, size;          // size = L C
-    double inv_count, scale, eps;                  // 1 / (L D); dropout's factor
+    double count, inv_count, scale, eps;           // L D and 1 / (L D); dropout's factor
     int C, G, D, act, site;
     uint32_t cut;
     float inv_D, inv_C;

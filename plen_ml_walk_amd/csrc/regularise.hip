@@ -211,7 +211,7 @@ static NormArgs kernel_args(const PlenRegNorm &a) {
     k.x = a.x; k.dy = a.dy; k.w = a.w; k.b = a.b; k.out = a.out; k.stats = (double2 *)a.stats; k.rng = a.rng; k.used = a.used;
     k.N = a.N; k.x_stride = a.x_stride; k.dy_stride = a.dy_stride; k.size = a.L * a.C;
     k.C = a.C; k.G = a.G; k.D = a.C / a.G; k.act = a.act; k.site = a.site; k.cut = a.cut;
-    k.inv_count = 1.0 / ((double)a.L * k.D); k.scale = drop_scale(a.cut); k.eps = (double)a.eps;
+    k.count = (double)a.L * k.D; k.inv_count = 1.0 / k.count; k.scale = drop_scale(a.cut); k.eps = (double)a.eps;
     k.inv_D = 1.f / (float)k.D; k.inv_C = 1.f / (float)a.C;
     return k;
 }

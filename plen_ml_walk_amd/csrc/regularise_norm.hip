@@ -40,8 +40,9 @@ __device__ __forceinline__ double inverse_sqrt(double v) {
     return fma(0.5 * r, fma(-v * r, r, 1.0), r);
 }
 // sums of (x - s), (x - s)^2 -> the pair that NormArgs.stats holds
-__device__ __forceinline__ double2 finish_stats(const NormArgs &A, double s, double sum, double squares) {
-    const double m = sum * A.inv_count;
+__device__ __forceinline__ double2 finish_stats(const NormArgs &A, double count, double s, double sum, double squares) {
+    double m = sum * A.inv_count;
+    m = fma(fma(-m, count, sum), A.inv_count, m);          // the quotient to its last bit: an element that is exactly the mean has z = 0, and without a bias a shut gate
     double var = fma(-m, m, squares * A.inv_count);
     if (var < 0.0) var = 0.0;
     return double2{s + m, A.scale * inverse_sqrt(fma(var, A.scale * A.scale, A.eps))};
@@ -279,7 +280,7 @@ template <int V, int K, int NT, bool DROP, bool STREAM> __global__ __launch_boun
             s += !V || valid[k] ? sk : 0.0; q += !V || valid[k] ? qk : 0.0;
         }
         team_sum2<NT>(s, q, P.team_log, turn, lds);
-        const double2 st = finish_stats(A, shift, s, q);
+        const double2 st = finish_stats(A, A.count, shift, s, q);
         if (on) {
             if (A.stats && p.lane == 0) A.stats[st_at] = st;
             const float mean = (float)st.x, rstd = (float)st.y, offset = -(float)(st.x - (double)mean) * rstd;
@@ -463,7 +464,7 @@ template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(WIDE_NT) v
             }
         }
         team_sum2<WIDE_NT>(s, q, WIDE_LOG, turn, lds);
-        const double2 st = finish_stats(A, shift, s, q);
+        const double2 st = finish_stats(A, A.count, shift, s, q);
         if (A.stats && threadIdx.x == 0) A.stats[item] = st;
         const float mean = (float)st.x, rstd = (float)st.y, offset = -(float)(st.x - (double)mean) * rstd;
         T *y = (T *)A.out + n * A.C + c0;
@@ -633,7 +634,9 @@ struct Nothing { __device__ __forceinline__ float operator()(int) const { return
 // (8 x 4096 x 320 with 32 groups, forward sums: 9.1 us with eight pairs always and the copies of a row one after the other; without any join 5.4.)
 template <int V, class B, class F>
 __device__ __forceinline__ void join_groups(const double (&a)[8], const double (&b)[8], const NormArgs &A, const MapPlan &P, const Column &c, double2 *lds, B before, F result) {
-    const int NT = blockDim.x, at = c.r * P.bcol + c.col - c.first;
+    const int NT = blockDim.x;
+    int at = c.r * P.bcol + c.col - c.first;
+    asm volatile("" : "+v"(at));                     // (hidden, as the column in load_constants: in a loop over slabs the addresses would be kept)
     const bool two = V == 1 && A.D >= 8;
     __syncthreads();
     if (c.mine) {
@@ -654,12 +657,14 @@ __device__ __forceinline__ void join_groups(const double (&a)[8], const double (
     }
     __syncthreads();
     // a group's entries: copy k of the row, row r, and u: its chunks, or (groups of less than 8 channels) its channels
-    const int lane = threadIdx.x & ((1 << P.lanes_log) - 1), teams = NT >> P.lanes_log, units = V == 2 ? A.D >> 3 : two ? (A.D + 14) >> 3 : A.D, entries = units * P.R << P.q_log;
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));
+    const int lane = thread & ((1 << P.lanes_log) - 1), teams = NT >> P.lanes_log, units = V == 2 ? A.D >> 3 : two ? (A.D + 14) >> 3 : A.D, entries = units * P.R << P.q_log;
     const int end = c.first + P.bcol < P.ncol ? c.first + P.bcol : P.ncol;
     const float inv_units = 1.f / (float)units, inv_R = 1.f / (float)P.R;
 #pragma unroll 1
     for (int g0 = 0; g0 < A.G; g0 += teams) {                        // (every lane takes every turn: the exchange needs them all)
-        const int g = g0 + (threadIdx.x >> P.lanes_log);
+        const int g = g0 + (thread >> P.lanes_log);
         const float first = before(g < A.G ? g : A.G - 1);
         double s = 0.0, q = 0.0;
         if (g < A.G)
@@ -724,7 +729,9 @@ template <int V, bool DROP> __device__ __forceinline__ void load_shifts(const No
         float *all = (float *)lds;
         if (DROP) {
             __syncthreads();
-            for (int g = threadIdx.x; g < A.G; g += blockDim.x) all[g] = group_shift<DROP>(A, d, n, g);
+            int g = threadIdx.x;
+            asm volatile("" : "+v"(g));
+            for (; g < A.G; g += blockDim.x) all[g] = group_shift<DROP>(A, d, n, g);
             __syncthreads();
         }
 #pragma unroll
@@ -787,7 +794,7 @@ template <bool DROP> __global__ __launch_bounds__(256) void k_map_stats(NormArgs
         const int64_t n = item / A.G;
         const double shift = group_shift<DROP>(A, d, n, (int)(item - n * A.G));
         const double2 t = join_splits(part + item * splits, splits);
-        if ((threadIdx.x & 63) == 0) A.stats[item] = finish_stats(A, shift, t.x, t.y);
+        if ((threadIdx.x & 63) == 0) A.stats[item] = finish_stats(A, A.count, shift, t.x, t.y);
     }
 }
 // statistics and parameters of a thread's 8 virtual channels (V = 2: one group, statistics in element 0).
@@ -883,7 +890,7 @@ template <int V, bool DROP, bool STREAM> __global__ __launch_bounds__(512) __att
             const bool writes = A.stats && blockIdx.x == 0 && blockIdx.y == 0;
             __syncthreads();
             join_slab(A, P, part + n * A.G * P.splits * P.col_blocks, [&](int g) { return group_shift<DROP>(A, d, n, g); }, [&](int g, float shift, double sum, double squares) {
-                lds[g] = finish_stats(A, (double)shift, sum, squares);
+                lds[g] = finish_stats(A, A.count, (double)shift, sum, squares);
                 if (writes) A.stats[n * A.G + g] = lds[g];
             });
             __syncthreads();
@@ -1072,7 +1079,7 @@ template <int V, bool DROP> __global__ __launch_bounds__(512) __attribute__((amd
         double s[8] = {}, q[8] = {};
         span_sums<V, DROP, DROP>(A, d, c, t, n, lds, s, q);
         join_groups<V>(s, q, A, P, c, lds, [&](int g) { return group_shift<DROP>(A, d, n, g); }, [&](int g, float shift, double sum, double squares) {
-            groups[g] = finish_stats(A, (double)shift, sum, squares);
+            groups[g] = finish_stats(A, A.count, (double)shift, sum, squares);
             if (A.stats) A.stats[n * A.G + g] = groups[g];
         });
         __syncthreads();

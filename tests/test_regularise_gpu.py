@@ -724,3 +724,26 @@ def test_a_bad_gradient_spoils_its_own_group_only(shape, groups):
             got = _layer(x, spoilt, w, b, groups, act, p)
             for name, a, c, rest in zip(("y", "dx", "dw", "db"), got, clean, (torch.ones_like(hit).view(shape), ~hit.view(shape), ~chan.view(-1), ~chan.view(-1))):
                 assert torch.equal(a[rest], c[rest]), (name, act, bad, g)
+
+
+@pytest.mark.parametrize("shape,groups", [((4000, 9), 1), ((3000, 27), 3), ((500, 49), 1), ((60, 1001), 7), ((40, 3003), 1), ((3, 9001), 1), ((900, 3, 5), 1), ((300, 7, 30), 3), ((40, 11, 24), 3), ((2, 3001, 10), 2), ((2, 9001, 24), 3),
+                                          ((4, 4003, 7), 7)], ids=ids)
+def test_elements_that_are_their_groups_mean(shape, groups):
+    """Whole numbers, one of each group set so that another of its elements is exactly the mean (counts without a power of two): its normalised value is 0, and without a bias its ReLU is shut.  The sums are exact in
+    64 bits, so the mean has to be the quotient to its last bit."""
+    d = shape[-1] // groups
+    x, dy, w, _ = _case(shape, groups, torch.float32)
+    v = torch.randint(-500, 500, shape, generator=_gen(41)).double()
+    flat = v.view(shape[0], -1, groups, d).permute(0, 2, 1, 3).reshape(shape[0] * groups, -1)
+    n = flat.shape[1]
+    assert n & (n - 1)
+    flat[:, 1] = torch.randint(-3, 4, (flat.shape[0],), generator=_gen(42)).double()          # (small, so that the last one stays within 24 bits)
+    flat[:, -1] += n * flat[:, 1] - flat.sum(1)                  # the sum is n times element 1
+    v = flat.view(shape[0], groups, -1, d).permute(0, 2, 1, 3).reshape(shape)
+    x = v.float()
+    assert torch.equal(x.double(), v)
+    ref = O.Norm(x, groups, w, None, 1e-5, "none")
+    tie = (ref.y == 0).view(shape[0], -1, groups, d)
+    assert tie.any(3).any(1).all()                               # the oracle has them too
+    for offset in (0.0, 4096.0):
+        _check((x + offset).cuda().requires_grad_(), dy, w, None, groups, "relu", None, _rng())
